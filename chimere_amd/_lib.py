@@ -9,6 +9,7 @@ import os
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libchimere_hip.so")
 
+F32, F16, BF16 = 0, 1, 30      # float rows
 Q4_0, Q8_0, Q4_K, Q5_K, Q6_K, IQ3_S, MXFP4 = 2, 8, 12, 13, 14, 21, 39
 TYPE_NAMES = {Q4_0: "q4_0", Q8_0: "q8_0", IQ3_S: "iq3s", Q4_K: "q4k", Q5_K: "q5k", Q6_K: "q6k", MXFP4: "mxfp4"}
 
@@ -58,6 +59,15 @@ SIGNATURES = [
     ("chimere_moe_prefill", None, [vp, vp, vp, i32, vp, vp, vp, szt, vp]),
     ("chimere_fused_moe_iq3s_workspace_size", szt, [i32, i32, i32]),
     ("chimere_fused_moe_iq3s", None, [vp, vp, vp, vp, vp, vp, vp, i32, i32, i64, i64, i64, i32, vp, szt, vp]),
+    ("chimere_quantize_i8", None, [i32, vp, i64, vp, i64, vp, i64, i32, vp]),
+    ("chimere_gemm_i8", None, [vp, i64, vp, vp, i64, vp, vp, i32, vp, i64, i32, i32, i32, vp]),
+    ("chimere_linear_i8_workspace_size", szt, [i32, i32]),
+    ("chimere_linear_i8", None, [i32, vp, i64, vp, i64, vp, vp, i32, vp, i64, i32, i32, i32, vp, szt, vp]),
+    ("chimere_moe_i8_workspace_size", szt, [vp, i32, i32]),
+    ("chimere_moe_i8", None, [vp, i32, vp, i64, vp, vp, i32, i32, vp, i64, i32, vp, szt, vp]),
+    ("chimere_balance_loss_workspace_size", szt, [i32, i32]),
+    ("chimere_balance_loss", None, [i32, vp, i64, vp, i32, vp, vp, vp, vp, vp, i32, i32, vp, szt, vp]),
+    ("chimere_balance_loss_grad", None, [i32, vp, i64, vp, vp, vp, vp, i32, vp, i64, i32, i32, vp]),
     ("chimere_quantize_weights", None, [i32, vp, vp, i64, vp]),
     ("chimere_dbg_block_dots", None, [i32, vp, vp, vp, i32, i32, vp]),
     ("chimere_hip_get_last_error", i32, []),
@@ -73,6 +83,13 @@ class MoeLayerC(C.Structure):
                 ("gate_exps", vp), ("up_exps", vp), ("down_exps", vp),
                 ("gate_stride", C.c_int64), ("up_stride", C.c_int64), ("down_stride", C.c_int64),
                 ("sh_gate", vp), ("sh_up", vp), ("sh_down", vp), ("sh_gate_w", vp)]
+
+
+class MoeI8LayerC(C.Structure):
+    """Mirror of ``struct chimere_moe_i8_layer``."""
+    _fields_ = [("hidden", C.c_int), ("ffn", C.c_int), ("n_experts", C.c_int),
+                ("gate", vp), ("up", vp), ("down", vp),
+                ("gate_scale", vp), ("up_scale", vp), ("down_scale", vp)]
 
 
 _lib = None

@@ -32,6 +32,11 @@ extern "C" {
 #define CHIMERE_TYPE_Q8_0 8
 #define CHIMERE_TYPE_IQ3_S 21
 
+/* float rows of the 8-bit integer and balance-loss entry points */
+#define CHIMERE_TYPE_F32 0
+#define CHIMERE_TYPE_F16 1
+#define CHIMERE_TYPE_BF16 30
+
 /* error codes returned by chimere_hip_get_last_error() */
 #define CHIMERE_OK 0
 #define CHIMERE_ERR_ARG 1      /* rejected argument (shape, alignment, null, range) */
@@ -277,6 +282,87 @@ void chimere_fused_moe_iq3s(const float *hidden, const void *gate_exps, const vo
                             float *output, int hidden_size, int expert_ffn, int64_t expert_bytes_gate,
                             int64_t expert_bytes_up, int64_t expert_bytes_down, int top_k,
                             void *workspace, size_t workspace_bytes, hipStream_t stream);
+
+/* ------------------------------------ 8-bit integers, one scale per row */
+/* No reference counterpart: dense products of any number of tokens, and the
+ * routed experts', over weights in 8-bit integers with one f32 scale per
+ * output channel and tokens with one scale each.  Float rows are F32, F16 or
+ * BF16 (CHIMERE_TYPE_*, strides in elements, the elements of a row next to
+ * each other); rows of 8-bit integers start 16-byte aligned (pointer and
+ * stride, in bytes), and what lies between their ncols integers and the next
+ * multiple of 16 is read but does not matter.  Outputs may not overlap
+ * inputs.  ntok = 0 launches nothing.  Sums of products are exact (int32), so
+ * results repeat bit for bit and do not depend on ntok. */
+
+/* scale[r] = max |x[r]| / 127, q[r][c] = x[r][c] / scale[r] rounded to the
+ * nearest integer, ties to even (0 where the scale is 0).  A row that holds
+ * an infinity or a NaN gets it as scale, and zeros.  Only the ncols integers
+ * of a row are written.  For tokens and for weights (rows = channels). */
+void chimere_quantize_i8(int type, const void *x, int64_t x_stride, int8_t *q, int64_t q_stride,
+                         float *scale, int64_t nrows, int ncols, hipStream_t stream);
+/* out[t][r] = (sum_c a[t][c] w[r][c]) * a_scale[t] * w_scale[r] (+ bias[r]
+ * unless NULL), rounded to out_type.  ncols at most 131071. */
+void chimere_gemm_i8(const int8_t *a, int64_t a_stride, const float *a_scale, const int8_t *w,
+                     int64_t w_stride, const float *w_scale, const float *bias, int out_type,
+                     void *out, int64_t out_stride, int ntok, int nrows, int ncols,
+                     hipStream_t stream);
+/* The same for float tokens, quantized as above within the call.  Workspace:
+ * chimere_linear_i8_workspace_size(>= ntok, ncols) bytes, 256-byte aligned,
+ * needs no initialisation. */
+size_t chimere_linear_i8_workspace_size(int max_ntok, int ncols);
+void chimere_linear_i8(int type, const void *x, int64_t x_stride, const int8_t *w, int64_t w_stride,
+                       const float *w_scale, const float *bias, int out_type, void *out,
+                       int64_t out_stride, int ntok, int nrows, int ncols, void *workspace,
+                       size_t workspace_bytes, hipStream_t stream);
+
+/* Routed experts' FFN for ntok tokens whose ids and weights [ntok][top_k] are
+ * given (chimere_topk_softmax): out[t] = sum over k, ascending, of
+ * weights[t][k] * D_e hq_e with e = ids[t][k], h_e = silu(G_e xq) * (U_e xq)
+ * in f32, xq and hq the rows of x and h quantized as above.  An id that is no
+ * expert (-1: a pair dropped for capacity) adds nothing.  Neither router nor
+ * shared expert are part of it. */
+typedef struct chimere_moe_i8_layer {
+    int hidden;              /* H, multiple of 16 */
+    int ffn;                 /* F, multiple of 16 */
+    int n_experts;           /* E <= 1024; top_k <= 16 */
+    const int8_t *gate, *up; /* [E][F][H], 16-byte aligned */
+    const int8_t *down;      /* [E][H][F] */
+    const float *gate_scale, *up_scale; /* [E][F] */
+    const float *down_scale; /* [E][H] */
+} chimere_moe_i8_layer;
+/* Workspace for up to max_ntok tokens (0: shape out of range), 256-byte
+ * aligned, needs no initialisation.  Calls sharing one must not overlap. */
+size_t chimere_moe_i8_workspace_size(const chimere_moe_i8_layer *layer, int top_k, int max_ntok);
+void chimere_moe_i8(const chimere_moe_i8_layer *layer, int type, const void *x, int64_t x_stride,
+                    const int *ids, const float *weights, int top_k, int out_type, void *out,
+                    int64_t out_stride, int ntok, void *workspace, size_t workspace_bytes,
+                    hipStream_t stream);
+
+/* ---------------------------------------------- balance of a router's choice */
+/* No reference counterpart.  Over the tokens t whose mask[t] is not 0 (all of
+ * them where mask is NULL), N in number (*tokens):
+ *   counts[e] = pairs (t, k) with ids[t][k] = e (ids that are no expert are
+ *               not counted),
+ *   probs[e]  = mean of softmax(logits[t])[e],
+ *   *loss     = E * sum_e counts[e] / (N top_k) * probs[e],
+ * all 0 where N is 0.  A row of logits that are all -inf has probabilities
+ * of 0; rows that the mask leaves out are not read.  logits [ntok][E] with
+ * logits_stride elements between rows, F32 / F16 / BF16; ids [ntok][top_k];
+ * E <= 1024.  Sums have a fixed order: results repeat bit for bit. */
+size_t chimere_balance_loss_workspace_size(int n_experts, int max_ntok);
+void chimere_balance_loss(int type, const void *logits, int64_t logits_stride, const int *ids,
+                          int top_k, const uint8_t *mask, float *loss, float *probs, int *counts,
+                          int *tokens, int n_experts, int ntok, void *workspace,
+                          size_t workspace_bytes, hipStream_t stream);
+/* grad[t][j] = *grad_loss * d loss / d logits[t][j]
+ *            = *grad_loss * E / N * p_tj * (f_j - sum_e f_e p_te),
+ * p_t = softmax(logits[t]), f_e = counts[e] / (N top_k) (constant: the choice
+ * has no gradient); 0 in rows that the mask leaves out.  grad has the type of
+ * the logits; counts and tokens are chimere_balance_loss's. */
+void chimere_balance_loss_grad(int type, const void *logits, int64_t logits_stride,
+                               const uint8_t *mask, const int *counts, const int *tokens,
+                               const float *grad_loss, int top_k, void *grad, int64_t grad_stride,
+                               int n_experts, int ntok, hipStream_t stream);
 
 /* ----------------------------------------------- weight quantizers (GPU) */
 /* Not part of the reference's ABI (its weights come pre-quantized from GGUF);
