@@ -6,44 +6,132 @@
 
 namespace chimere {
 
-// Row quantizer: scale = max |x| / 127, q = x / scale rounded to the nearest
-// integer, ties to even (IEEE divisions).  A row that holds an infinity or a
-// NaN keeps it in the scale and 0 in its integers, so its products are NaN.
-// One work-group per row, two passes over it.
-template <typename T>
-__global__ __launch_bounds__(256) void k_i8_quantize(const T* __restrict__ x, int64_t xs, int8_t* __restrict__ q,
-                                                     int64_t qs, float* __restrict__ scale, int ncols) {
-    __shared__ uint32_t part[4];
-    const T* row = x + (int64_t)blockIdx.x * xs;
-    // |x| as bits: a NaN is larger than an infinity, and both than any number
-    uint32_t m = 0;
-    for (int c = threadIdx.x; c < ncols; c += 256)
-        m = max(m, __builtin_bit_cast(uint32_t, load_f(row + c)) & 0x7FFFFFFFu);
+// the integer of x in a row of scale d
+__device__ __forceinline__ int i8_quant(float x, float d) {
+    return d > 0.0f && d < __builtin_huge_valf() ? (int)__builtin_rintf(x / d) : 0;
+}
+
+// N integers packed into bytes
+template <int N>
+__device__ __forceinline__ void i8_pack(const float (&x)[N], float d, uint32_t (&q)[N / 4]) {
+#pragma unroll
+    for (int k = 0; k < N; k += 4)
+        q[k / 4] = (uint32_t)(uint8_t)i8_quant(x[k], d) | (uint32_t)(uint8_t)i8_quant(x[k + 1], d) << 8 |
+                   (uint32_t)(uint8_t)i8_quant(x[k + 2], d) << 16 | (uint32_t)(uint8_t)i8_quant(x[k + 3], d) << 24;
+}
+
+// Elements c .. c + V - 1 of a row as f32, one 16-byte load where `wide`; those
+// from ncols on are 0
+template <int V, typename T>
+__device__ __forceinline__ void i8_load(const T* row, int c, int ncols, bool wide, float (&x)[V]) {
+    typedef T vec __attribute__((ext_vector_type(V)));
+    if (wide && c + V <= ncols) {
+        const vec v = *(const vec*)(row + c);
+#pragma unroll
+        for (int k = 0; k < V; k++) x[k] = (float)v[k];
+    } else {
+#pragma unroll
+        for (int k = 0; k < V; k++) x[k] = c + k < ncols ? load_f(row + c + k) : 0.0f;
+    }
+}
+
+// max |x| as bits: a NaN is larger than an infinity, and both than any number
+template <int V>
+__device__ __forceinline__ uint32_t i8_amax(uint32_t m, const float (&x)[V]) {
+#pragma unroll
+    for (int k = 0; k < V; k++) m = max(m, __builtin_bit_cast(uint32_t, x[k]) & 0x7FFFFFFFu);
+    return m;
+}
+__device__ __forceinline__ uint32_t wave_amax(uint32_t m) {
     m = max(m, (uint32_t)xlane<32>((int)m));
     m = max(m, (uint32_t)xlane<16>((int)m));
     m = max(m, (uint32_t)xlane<8>((int)m));
     m = max(m, (uint32_t)xlane<4>((int)m));
     m = max(m, (uint32_t)xlane<2>((int)m));
-    m = max(m, (uint32_t)xlane<1>((int)m));
-    if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = m;
-    __syncthreads();
-    m = max(max(part[0], part[1]), max(part[2], part[3]));
+    return max(m, (uint32_t)xlane<1>((int)m));
+}
+
+// Row quantizer: scale = max |x| / 127, q = x / scale rounded to the nearest
+// integer, ties to even (IEEE divisions).  A row that holds an infinity or a
+// NaN keeps it in the scale and 0 in its integers, so its products are NaN.
+// Bound by the row's bytes.  W waves per row (rows of up to 1024 columns one,
+// longer ones four: 4 W rows' worth of latency is hidden by the other
+// work-groups), 16 elements of each lane stay in registers between the
+// maximum and the integers; columns past 1024 W are read twice.
+template <typename T, int W>
+__global__ __launch_bounds__(256) void k_i8_quantize(const T* __restrict__ x, int64_t xs, int8_t* __restrict__ q,
+                                                     int64_t qs, float* __restrict__ scale, int64_t nrows, int ncols,
+                                                     bool wide) {
+    constexpr int V = 16 / sizeof(T), KEEP = 16 / V, STEP = 64 * W * V;
+    __shared__ uint32_t part[4];
+    const int wave = threadIdx.x >> 6;
+    const int64_t r = (int64_t)blockIdx.x * (4 / W) + wave / W;
+    if (r >= nrows) return;   // W = 1 only: no barrier follows
+    const T* row = x + r * xs;
+    const int c0 = (threadIdx.x & (64 * W - 1)) * V;
+    float v[KEEP][V];
+    uint32_t m = 0;
+#pragma unroll
+    for (int i = 0; i < KEEP; i++) {
+        i8_load<V>(row, c0 + i * STEP, ncols, wide, v[i]);
+        m = i8_amax(m, v[i]);
+    }
+    for (int c = c0 + KEEP * STEP; c < ncols; c += STEP) {
+        float u[V];
+        i8_load<V>(row, c, ncols, wide, u);
+        m = i8_amax(m, u);
+    }
+    m = wave_amax(m);
+    if constexpr (W == 4) {
+        if ((threadIdx.x & 63) == 0) part[wave] = m;
+        __syncthreads();
+        m = max(max(part[0], part[1]), max(part[2], part[3]));
+    }
     const float d = __builtin_bit_cast(float, m) / 127.0f;
-    const bool zero = m >= 0x7F800000u || d == 0.0f;
-    for (int c = threadIdx.x; c < ncols; c += 256)
-        q[(int64_t)blockIdx.x * qs + c] = zero ? 0 : (int8_t)(int)__builtin_rintf(load_f(row + c) / d);
-    if (threadIdx.x == 0) scale[blockIdx.x] = d;
+    if (c0 == 0) scale[r] = d;
+    int8_t* to = q + r * qs;
+    auto put = [&](int c, const float(&u)[V]) {
+        uint32_t p[V / 4];
+        i8_pack<V>(u, d, p);
+        if (c + V <= ncols) {
+            typedef uint32_t words __attribute__((ext_vector_type(V / 4)));
+            words o;
+#pragma unroll
+            for (int k = 0; k < V / 4; k++) o[k] = p[k];
+            *(words*)(to + c) = o;
+        } else {
+#pragma unroll
+            for (int k = 0; k < V; k++)
+                if (c + k < ncols) to[c + k] = (int8_t)(p[k / 4] >> (8 * (k & 3)));
+        }
+    };
+#pragma unroll
+    for (int i = 0; i < KEEP; i++)
+        if (c0 + i * STEP < ncols) put(c0 + i * STEP, v[i]);
+    for (int c = c0 + KEEP * STEP; c < ncols; c += STEP) {
+        float u[V];
+        i8_load<V>(row, c, ncols, wide, u);
+        put(c, u);
+    }
+}
+
+template <typename T>
+static void launch_i8_quantize(const T* x, int64_t xs, int8_t* q, int64_t qs, float* scale, int64_t nrows, int ncols,
+                               hipStream_t s) {
+    const bool wide = (((uintptr_t)x | (uintptr_t)(xs * sizeof(T))) & 15) == 0;
+    if (ncols <= 1024)
+        hipLaunchKernelGGL((k_i8_quantize<T, 1>), dim3((unsigned)((nrows + 3) / 4)), dim3(256), 0, s, x, xs, q, qs, scale,
+                           nrows, ncols, wide);
+    else
+        hipLaunchKernelGGL((k_i8_quantize<T, 4>), dim3((unsigned)nrows), dim3(256), 0, s, x, xs, q, qs, scale, nrows,
+                           ncols, wide);
 }
 
 void launch_i8_quantize(int type, const void* x, int64_t xs, int8_t* q, int64_t qs, float* scale, int64_t nrows,
                         int ncols, hipStream_t s) {
-    const dim3 grid((unsigned)nrows);
-    if (type == T_F32)
-        hipLaunchKernelGGL(k_i8_quantize<float>, grid, dim3(256), 0, s, (const float*)x, xs, q, qs, scale, ncols);
-    else if (type == T_F16)
-        hipLaunchKernelGGL(k_i8_quantize<_Float16>, grid, dim3(256), 0, s, (const _Float16*)x, xs, q, qs, scale, ncols);
-    else
-        hipLaunchKernelGGL(k_i8_quantize<__bf16>, grid, dim3(256), 0, s, (const __bf16*)x, xs, q, qs, scale, ncols);
+    if (type == T_F32) launch_i8_quantize((const float*)x, xs, q, qs, scale, nrows, ncols, s);
+    else if (type == T_F16) launch_i8_quantize((const _Float16*)x, xs, q, qs, scale, nrows, ncols, s);
+    else launch_i8_quantize((const __bf16*)x, xs, q, qs, scale, nrows, ncols, s);
 }
 
 struct I8Gemm {
@@ -52,13 +140,23 @@ struct I8Gemm {
     void* out;
     int64_t lda, ldw, ldo;
     int M, N, C;
+    const void* x;     // float tokens that the kernel quantizes itself, or null
+    int64_t ldx;
 };
 
-template <typename T, typename Tile>
-__global__ __launch_bounds__(64 * Tile::NW) void k_i8_gemm(I8Gemm g) {
-    extern __shared__ __align__(16) uint8_t lds[];
-    const int tm = (g.M + Tile::BM - 1) / Tile::BM;
-    const int m0 = blockIdx.x % tm * Tile::BM, n0 = blockIdx.x / tm * Tile::BN;
+// Many tokens: one tile per work-group.  Tiles go to the XCDs in contiguous
+// eighths (work-groups are dealt round-robin), four token tiles against all
+// weight tiles in turn, so the tiles that an XCD works on at a time share
+// their rows in its L2.
+template <typename T, typename Tile, int WAVES_PER_SIMD>
+__global__ __launch_bounds__(64 * Tile::NW, WAVES_PER_SIMD) void k_i8_gemm(I8Gemm g) {
+    __shared__ __align__(16) uint8_t lds[Tile::LDS];
+    constexpr int VEC = sizeof(T) == 4 ? 4 : 8, GM = 4;
+    const int tm = (g.M + Tile::BM - 1) / Tile::BM, tn = (g.N + Tile::BN - 1) / Tile::BN;
+    const int per = (tm * tn + 7) / 8, tile = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
+    if (tile >= tm * tn) return;
+    const int grp = tile / (GM * tn), rows = min(GM, tm - grp * GM), at = tile - grp * GM * tn;
+    const int m0 = (grp * GM + at % rows) * Tile::BM, n0 = at / rows * Tile::BN;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     uint32_t aoff[Tile::PM], woff[Tile::PN];
 #pragma unroll
@@ -67,31 +165,223 @@ __global__ __launch_bounds__(64 * Tile::NW) void k_i8_gemm(I8Gemm g) {
 #pragma unroll
     for (int p = 0; p < Tile::PN; p++)
         woff[p] = (uint32_t)(min((wave * Tile::PN + p) * 8 + (lane >> 3), g.N - 1 - n0) * g.ldw);
-    constexpr int MT = Tile::MTILES, NT = Tile::NTILES;
-    v16i acc[MT][NT];
+    const float as = threadIdx.x < Tile::BM ? g.as[min(m0 + (int)threadIdx.x, g.M - 1)] : 0.0f;
+    v16i acc[Tile::MTILES][Tile::NTILES];
     const int8_t* w = g.w + n0 * g.ldw;
     Tile::run(g.a + m0 * g.lda, w, w, aoff, woff, g.C, lds, acc);
-    const int wm = wave / Tile::WAVES_N, wn = wave % Tile::WAVES_N;
+    const int n = n0 + Tile::template first_col<VEC>();
+    float ws[VEC], b[VEC];
 #pragma unroll
-    for (int j = 0; j < NT; j++) {
-        const int n = n0 + (wn * NT + j) * 32 + (lane & 31);
-        if (n >= g.N) continue;
-        const float s = g.ws[n], b = g.bias ? g.bias[n] : 0.0f;
+    for (int k = 0; k < VEC; k++) {
+        const int nk = min(n + k, g.N - 1);
+        ws[k] = g.ws[nk];
+        b[k] = g.bias ? g.bias[nk] : 0.0f;
+    }
+    const bool wide = (((uintptr_t)g.out | (uintptr_t)(g.ldo * sizeof(T))) & 15) == 0;
+    Tile::template rows<VEC>(lds, acc, make_float2(as, 0.0f), [&](int r, const int(&x)[VEC], float2 of_row) {
+        if (m0 + r >= g.M || n >= g.N) return;
+        float v[VEC];
 #pragma unroll
-        for (int i = 0; i < MT; i++)
+        for (int k = 0; k < VEC; k++) v[k] = (float)x[k] * of_row.x * ws[k] + b[k];
+        store_row((T*)g.out + (m0 + r) * g.ldo + n, v, g.N - n, wide);
+    });
+}
+
+// Few tokens: 16 MB of them against 16 NB weight rows per work-group, the
+// columns in steps of 128 dealt to its eight waves (v_mfma_i32_16x16x64_i8,
+// fragments straight from memory: no weight byte is used by two waves), whose
+// int32 sums are joined in LDS.  With X, tokens are floats that every
+// work-group quantizes for itself (one launch less); their integers lie in
+// LDS, cleared up to whole steps.
+constexpr int FEW_WAVES = 8, FEW_KEEP = 16;   // elements that a thread quantizes at most
+
+template <typename T, typename X, int MB, int NB>
+__global__ __launch_bounds__(64 * FEW_WAVES) void k_i8_few(I8Gemm g) {
+    constexpr bool QUANT = !std::is_same<X, int8_t>::value;
+    extern __shared__ __align__(16) uint8_t lds[];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int m0 = blockIdx.y * 16 * MB, n0 = blockIdx.x * 16 * NB;
+    const int S = (g.C + I8_BK - 1) / I8_BK, last = (g.C + 15) / 16 - 1;
+    const int r = lane & 15, pc = (lane >> 4) * 2;
+    const int lda = S * I8_BK + 16;   // of the integers in LDS: rows 4 banks apart
+    const int M = min(g.M - m0, 16 * MB);
+    const int8_t* arow[MB];
+    const int8_t* wrow[NB];
 #pragma unroll
-            for (int v = 0; v < 16; v++) {
-                const int m = m0 + (wm * MT + i) * 32 + Tile::reg_row(v);
-                if (m < g.M) store_f((T*)g.out + m * g.ldo + n, (float)acc[i][j][v] * g.as[m] * s + b);
+    for (int j = 0; j < NB; j++) wrow[j] = g.w + (int64_t)min(n0 + j * 16 + r, g.N - 1) * g.ldw;
+    v4i fw[NB][2];
+    auto load_w = [&](int s) {
+#pragma unroll
+        for (int j = 0; j < NB; j++)
+#pragma unroll
+            for (int h = 0; h < 2; h++) fw[j][h] = *(const v4i*)(wrow[j] + min(8 * s + pc + h, last) * 16);
+    };
+    if (wave < S) load_w(wave);
+    float* as = (float*)lds;   // [16 MB]
+    uint8_t* aq = lds + 16 * MB * 4;
+    if constexpr (QUANT) {
+        // pieces of V elements, row by row, over all threads; each row's maximum
+        // through an LDS atomic (any order gives the same)
+        constexpr int V = 16 / sizeof(X), KEEP = FEW_KEEP / V;
+        uint32_t* bits = (uint32_t*)lds;
+        const bool wide = (((uintptr_t)g.x | (uintptr_t)(g.ldx * sizeof(X))) & 15) == 0;
+        const int per = (S * I8_BK) / V, n = M * per;
+        if (tid < 16 * MB) bits[tid] = 0;
+        __syncthreads();
+        float v[KEEP][V];
+#pragma unroll
+        for (int i = 0; i < KEEP; i++) {
+            const int at = tid + i * 64 * FEW_WAVES, m = min(at / per, M - 1);
+            uint32_t top = 0;
+            if (at < n) {
+                i8_load<V>((const X*)g.x + m * g.ldx, (at - m * per) * V, g.C, wide, v[i]);
+                top = i8_amax(0u, v[i]);
             }
+            if (M == 1) {
+                top = wave_amax(top);
+                if (lane == 0) atomicMax(&bits[0], top);
+            } else if (at < n) {
+                atomicMax(&bits[m], top);
+            }
+        }
+        __syncthreads();
+        if (tid < M) as[tid] = __builtin_bit_cast(float, bits[tid]) / 127.0f;
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < KEEP; i++) {
+            const int at = tid + i * 64 * FEW_WAVES, m = min(at / per, M - 1);
+            if (at < n) {
+                uint32_t p[V / 4];
+                i8_pack<V>(v[i], as[m], p);
+#pragma unroll
+                for (int k = 0; k < V / 4; k++) *(uint32_t*)(aq + m * lda + (at - m * per) * V + 4 * k) = p[k];
+            }
+        }
+        __syncthreads();
+    } else {
+        if (tid < 16 * MB) as[tid] = g.as[m0 + min(tid, M - 1)];
+    }
+#pragma unroll
+    for (int i = 0; i < MB; i++) {
+        const int m = min(i * 16 + r, M - 1);
+        arow[i] = QUANT ? (const int8_t*)aq + m * lda : g.a + (m0 + m) * g.lda;
+    }
+    v4i acc[MB][NB] = {};
+    for (int s = wave; s < S; s += FEW_WAVES) {
+        v4i fa[MB][2], w[NB][2];
+#pragma unroll
+        for (int i = 0; i < MB; i++)
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+                if constexpr (QUANT) {
+                    fa[i][h] = *(const v4i*)(arow[i] + (8 * s + pc + h) * 16);
+                } else {
+                    fa[i][h] = *(const v4i*)(arow[i] + min(8 * s + pc + h, last) * 16);
+                    if ((s + 1) * I8_BK > g.C) fa[i][h] = clear_tail(fa[i][h], (8 * s + pc + h) * 16, g.C);
+                }
+            }
+#pragma unroll
+        for (int j = 0; j < NB; j++)
+#pragma unroll
+            for (int h = 0; h < 2; h++) w[j][h] = fw[j][h];
+        if (s + FEW_WAVES < S) load_w(s + FEW_WAVES);
+#pragma unroll
+        for (int i = 0; i < MB; i++)
+#pragma unroll
+            for (int j = 0; j < NB; j++)
+#pragma unroll
+                for (int h = 0; h < 2; h++)
+                    acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(fa[i][h], w[j][h], acc[i][j], 0, 0, 0);
+    }
+    __syncthreads();   // aq has been read
+    int* part = (int*)(lds + 16 * MB * 4);
+#pragma unroll
+    for (int i = 0; i < MB; i++)
+#pragma unroll
+        for (int j = 0; j < NB; j++) *(v4i*)(part + ((wave * MB + i) * NB + j) * 256 + lane * 4) = acc[i][j];
+    __syncthreads();
+    for (int o = tid; o < MB * NB * 256; o += 64 * FEW_WAVES) {
+        // register v of lane l in a block: token 4 (l / 16) + v, weight row l % 16
+        const int i = o / (NB * 256), v = o >> 6 & 3, l = o & 63, j = o / 256 % NB;
+        const int m = i * 16 + 4 * (l >> 4) + v, n = n0 + j * 16 + (l & 15);
+        if (m >= M || n >= g.N) continue;
+        int sum = 0;
+#pragma unroll
+        for (int w = 0; w < FEW_WAVES; w++) sum += part[((w * MB + i) * NB + j) * 256 + l * 4 + v];
+        store_f((T*)g.out + (m0 + m) * g.ldo + n, (float)sum * as[m] * g.ws[n] + (g.bias ? g.bias[n] : 0.0f));
     }
 }
 
+template <typename T, typename X, int MB, int NB>
+static void launch_few(const I8Gemm& g, hipStream_t s) {
+    const size_t aq = std::is_same<X, int8_t>::value
+                          ? 0 : (size_t)(g.M < 16 * MB ? g.M : 16 * MB) * (pad_to(g.C, I8_BK) + 16);
+    const size_t part = (size_t)FEW_WAVES * MB * NB * 256 * 4;
+    const dim3 grid((g.N + 16 * NB - 1) / (16 * NB), (g.M + 16 * MB - 1) / (16 * MB));
+    hipLaunchKernelGGL((k_i8_few<T, X, MB, NB>), grid, dim3(64 * FEW_WAVES), 16 * MB * 4 + (aq > part ? aq : part), s, g);
+}
+
+template <typename T, typename Tile, int WAVES_PER_SIMD>
+static void launch_tiles(const I8Gemm& g, hipStream_t s) {
+    const int64_t tiles = (int64_t)((g.M + Tile::BM - 1) / Tile::BM) * ((g.N + Tile::BN - 1) / Tile::BN);
+    hipLaunchKernelGGL((k_i8_gemm<T, Tile, WAVES_PER_SIMD>), dim3((unsigned)((tiles + 7) / 8 * 8)), dim3(64 * Tile::NW),
+                       0, s, g);
+}
+
+// Which kernel takes a product, by how many work-groups its tiles make for the
+// 256 CUs: a larger tile reads its rows fewer times (all CUs together draw about
+// 13 TB/s from L2: 128 x 128 tiles of 4096 x 8192 x 4096 take 148 us, 256 x 256
+// 121), a smaller one puts more CUs to work, and where two work-groups fit a CU
+// two stages are enough, with one the third hides the weights' way from HBM.
+// Microseconds, weights from HBM, tokens x rows x columns (bf16 out):
+//   few tokens   16 x 1 / 16 x 2 rows   1x4096x2048 3.9 / 4.5  1x16384x4096 16.6 / 16.6  1x151936x2048 58 / 51
+//                16x16384x2048 10.3 / 9.0; 64 x 64 tiles 1x4096x2048 13
+//   24x4096x2048     32 x 16 5.0, 32 x 32 6.0, 64 x 64 7.3    100x4096x2048  32 x 32 10.0, 64 x 64 7.4
+//   100x2048x4096    32 x 16 13.0, 32 x 32 9.8, 64 x 64 11.1
+//   512x2048x2048    64 x 64 with two stages 10, four 7.1; 64 x 128 8.2, 128 x 128 11.1
+//   256x8192x4096    64 x 64 21.2, 64 x 128 18.5, 128 x 128 22.4    48x151936x2048 64 x 64 71, 64 x 128 63, 128 x 128 77
+//   512x8192x2048    64 x 64 22, 64 x 128 17.6, 128 x 128 with two stages 17.7, three 13.9, 256 x 256 29
+//   1000x8192x8192   128 x 128 with two stages 75, three 86, 256 x 256 94
+constexpr int FEW_N = 8192;
 template <typename T>
 static void launch_gemm(const I8Gemm& g, hipStream_t s) {
-    typedef I8Tile<2, 2, 1, 1> Tile;
-    const int64_t tiles = (int64_t)((g.M + Tile::BM - 1) / Tile::BM) * ((g.N + Tile::BN - 1) / Tile::BN);
-    hipLaunchKernelGGL((k_i8_gemm<T, Tile>), dim3((unsigned)tiles), dim3(64 * Tile::NW), Tile::LDS, s, g);
+    auto tiles = [&](int bm, int bn) { return (int64_t)((g.M + bm - 1) / bm) * ((g.N + bn - 1) / bn); };
+    const bool short_rows = (g.M + 255) / 256 * 256 > (g.M + 127) / 128 * 160;   // over a quarter of 256-row tiles empty
+    if (g.M <= 16) {
+        if (g.N <= FEW_N) launch_few<T, int8_t, 1, 1>(g, s);
+        else launch_few<T, int8_t, 1, 2>(g, s);
+    } else if (tiles(64, 64) <= 64) {
+        if (g.M <= 32) launch_few<T, int8_t, 2, 1>(g, s);
+        else launch_few<T, int8_t, 2, 2>(g, s);
+    } else if (tiles(64, 64) <= 256) {
+        launch_tiles<T, I8Tile<2, 2, 1, 1, 4>, 1>(g, s);
+    } else if (g.M <= 64 || tiles(64, 128) <= 256) {
+        launch_tiles<T, I8Tile<2, 4, 1, 1, 3>, 2>(g, s);
+    } else if (tiles(128, 128) <= 256) {
+        launch_tiles<T, I8Tile<2, 4, 2, 1, 3>, 2>(g, s);
+    } else if (tiles(128, 128) <= 512 || short_rows) {
+        launch_tiles<T, I8Tile<2, 4, 2, 1, 2>, 4>(g, s);
+    } else {
+        launch_tiles<T, I8Tile<2, 4, 4, 2, 2>, 2>(g, s);
+    }
+}
+
+// One or two float tokens: quantized by every work-group (1x4096x2048 5.7 us
+// against 6.6 in two launches, 2x4096x2048 5.9 / 6.7, 4x4096x2048 7.3 / 6.8),
+// as long as they fit its threads' registers.
+static bool quantizes_itself(int ntok, int ncols) {
+    return ntok <= 2 && ntok * pad_to(ncols, I8_BK) <= 64 * FEW_WAVES * FEW_KEEP;
+}
+template <typename T, typename X>
+static void launch_few_quantizing(const I8Gemm& g, hipStream_t s) {
+    if (g.N <= FEW_N) launch_few<T, X, 1, 1>(g, s);
+    else launch_few<T, X, 1, 2>(g, s);
+}
+template <typename T>
+static void launch_few_quantizing(int type, const I8Gemm& g, hipStream_t s) {
+    if (type == T_F32) launch_few_quantizing<T, float>(g, s);
+    else if (type == T_F16) launch_few_quantizing<T, _Float16>(g, s);
+    else launch_few_quantizing<T, __bf16>(g, s);
 }
 
 static void launch_gemm(int type, const I8Gemm& g, hipStream_t s) {
@@ -151,7 +441,7 @@ void chimere_gemm_i8(const int8_t* a, int64_t a_stride, const float* a_scale, co
                     (long long)a_stride);
     CHIMERE_REQUIRE((((uintptr_t)a | (uintptr_t)a_stride) & 15) == 0, CHIMERE_ERR_ARG,
                     "gemm_i8: rows of 8-bit integers must be 16-byte aligned");
-    launch_gemm(out_type, I8Gemm{a, w, a_scale, w_scale, bias, out, a_stride, w_stride, out_stride, ntok, nrows, ncols},
+    launch_gemm(out_type, I8Gemm{a, w, a_scale, w_scale, bias, out, a_stride, w_stride, out_stride, ntok, nrows, ncols, nullptr, 0},
                 stream);
     check_launch("gemm_i8");
 }
@@ -174,8 +464,15 @@ void chimere_linear_i8(int type, const void* x, int64_t x_stride, const int8_t* 
     const int64_t lda = pad_to(ncols, 16);
     int8_t* q = (int8_t*)workspace;
     float* as = (float*)((uint8_t*)workspace + al256((size_t)ntok * lda));
-    launch_i8_quantize(type, x, x_stride, q, lda, as, ntok, ncols, stream);
-    launch_gemm(out_type, I8Gemm{q, w, as, w_scale, bias, out, lda, w_stride, out_stride, ntok, nrows, ncols}, stream);
+    const I8Gemm g{q, w, as, w_scale, bias, out, lda, w_stride, out_stride, ntok, nrows, ncols, x, x_stride};
+    if (quantizes_itself(ntok, ncols)) {
+        if (out_type == T_F32) launch_few_quantizing<float>(type, g, stream);
+        else if (out_type == T_F16) launch_few_quantizing<_Float16>(type, g, stream);
+        else launch_few_quantizing<__bf16>(type, g, stream);
+    } else {
+        launch_i8_quantize(type, x, x_stride, q, lda, as, ntok, ncols, stream);
+        launch_gemm(out_type, g, stream);
+    }
     check_launch("linear_i8");
 }
 

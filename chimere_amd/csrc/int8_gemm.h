@@ -13,6 +13,8 @@
 // not stored, and the columns behind C are cleared in the token fragments of
 // the last step (their product with whatever the weight rows hold is 0).
 #pragma once
+#include <type_traits>
+
 #include "float_rows.h"
 
 namespace chimere {
@@ -25,14 +27,14 @@ typedef int v4i __attribute__((ext_vector_type(4)));
 typedef int v16i __attribute__((ext_vector_type(16)));
 
 // One 16-byte asynchronous copy per lane from base + off (off: 32 bits per
-// lane) to lds_wave + 16 * lane; see copy16_lds_untracked.
-__device__ __forceinline__ void copy16_lds_base(const void* base, uint32_t off, void* lds_wave) {
-    const uint32_t m = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)lds_wave);
+// lane) to LDS offset lds_wave + 16 * lane; not tracked by the compiler, as
+// copy16_lds_untracked.
+__device__ __forceinline__ void copy16_lds_base(const void* base, uint32_t off, uint32_t lds_wave) {
     uint32_t saved;
     __asm__ volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %3\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2\n\t"
                      "s_mov_b32 m0, %0"
                      : "=&s"(saved)
-                     : "v"(off), "s"(base), "s"(m)
+                     : "v"(off), "s"(base), "s"(lds_wave)
                      : "memory");
 }
 
@@ -46,12 +48,12 @@ __device__ __forceinline__ v4i clear_tail(v4i v, int k0, int C) {
     return v;
 }
 
-// WM x WN waves, each MT x NT blocks of 32 x 32
-template <int WM, int WN, int MT, int NT>
+// WM x WN waves, each MT x NT blocks of 32 x 32; NS stages
+template <int WM, int WN, int MT, int NT, int NS = 2>
 struct I8Tile {
     static constexpr int BM = WM * MT * 32, BN = WN * NT * 32, NW = WM * WN;
     static constexpr int WAVES_N = WN, MTILES = MT, NTILES = NT;
-    static constexpr int STAGE = (BM + BN) * I8_BK, LDS = 2 * STAGE;
+    static constexpr int STAGE = (BM + BN) * I8_BK, LDS = NS * STAGE;
     static constexpr int PM = BM / 8 / NW, PN = BN / 8 / NW;   // pieces of 8 rows that a wave copies
     static_assert(PM * 8 * NW == BM && PN * 8 * NW == BN, "tile rows over waves");
 
@@ -63,57 +65,139 @@ struct I8Tile {
                                                uint8_t* lds, v16i (&acc)[MT][NT]) {
         const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
         const int wm = wave / WN, wn = wave % WN;
-        const int S = (C + I8_BK - 1) / I8_BK, last = (C + 15) / 16 - 1, pc = (lane & 7) ^ (lane >> 3);
-        auto stage = [&](int s) {
-            uint8_t* at = lds + (s & 1) * STAGE;
-            const uint32_t k = (uint32_t)min(8 * s + pc, last) * 16u;
+        const int S = (C + I8_BK - 1) / I8_BK, last = (C + 15) / 16 - 1, pc = (lane & 7) ^ (lane >> 4);
+        const uint32_t lds0 = (uint32_t)(uintptr_t)(lds_void_t*)lds;
+        // copies of step s into stage `to`; past the last step the same columns
+        // again, so that the count of copies in flight stays the same
+        auto stage = [&](int s, int to) {
+            const uint32_t at = lds0 + to * STAGE;
+            const uint32_t k0 = (uint32_t)min(8 * s + pc, last) * 16u, k1 = (uint32_t)min(8 * s + (pc ^ 4), last) * 16u;
 #pragma unroll
-            for (int p = 0; p < PM; p++) copy16_lds_base(a, aoff[p] + k, at + (wave * PM + p) * 1024);
+            for (int p = 0; p < PM; p++)
+                copy16_lds_base(a, aoff[p] + ((wave * PM + p) & 1 ? k1 : k0), at + (wave * PM + p) * 1024);
 #pragma unroll
-            for (int p = 0; p < PN; p++) 
-                copy16_lds_base((wave * PN + p) & 4 ? w2 : w, woff[p] + k, at + BM * I8_BK + (wave * PN + p) * 1024);
+            for (int p = 0; p < PN; p++)
+                copy16_lds_base((wave * PN + p) & 4 ? w2 : w, woff[p] + ((wave * PN + p) & 1 ? k1 : k0),
+                                at + BM * I8_BK + (wave * PN + p) * 1024);
         };
 #pragma unroll
         for (int i = 0; i < MT; i++)
 #pragma unroll
             for (int j = 0; j < NT; j++) acc[i][j] = v16i{};
-        stage(0);
+#pragma unroll
+        for (int s = 0; s < NS - 1; s++) stage(s, s);
         const int r = lane & 31, g = lane >> 5;
-        for (int s = 0; s < S; s++) {
-            if (s + 1 < S) {
-                stage(s + 1);
-                wait_vm<PM + PN>();
-            } else {
-                wait_vm<0>();
-            }
-            lds_barrier();
-            const uint8_t* at = lds + (s & 1) * STAGE;
-            const bool tail = s + 1 == S && (C & (I8_BK - 1));
+        int cur = 0, nxt = NS - 1;
+        auto step = [&](int s, auto tail) {
+            wait_vm<(NS - 2) * (PM + PN)>();   // this wave's copies of step s have landed,
+            lds_barrier();                     // every wave's; and step s - 1 has been read by all
+            stage(s + NS - 1, nxt);
+            const uint8_t* at = lds + cur * STAGE;
+            cur = cur + 1 == NS ? 0 : cur + 1;
+            nxt = nxt + 1 == NS ? 0 : nxt + 1;
+            // the fragments of columns 32 (q + 1) are read while those of 32 q multiply
+            v4i fa[2][MT], fw[2][NT];
+            auto read = [&](int q) {
+                const int c = 2 * q + g, piece = (c ^ (r >> 1 & 7)) * 16;
 #pragma unroll
-            for (int q = 0; q < 4; q++) {
-                const int c = 2 * q + g, piece = (c ^ (r & 7)) * 16;
-                v4i fa[MT], fw[NT];
-#pragma unroll
-                for (int i = 0; i < MT; i++) fa[i] = *(const v4i*)(at + ((wm * MT + i) * 32 + r) * I8_BK + piece);
+                for (int i = 0; i < MT; i++)
+                    fa[q & 1][i] = *(const v4i*)(at + ((wm * MT + i) * 32 + r) * I8_BK + piece);
 #pragma unroll
                 for (int j = 0; j < NT; j++)
-                    fw[j] = *(const v4i*)(at + (BM + (wn * NT + j) * 32 + r) * I8_BK + piece);
+                    fw[q & 1][j] = *(const v4i*)(at + (BM + (wn * NT + j) * 32 + r) * I8_BK + piece);
                 if (tail) {
 #pragma unroll
-                    for (int i = 0; i < MT; i++) fa[i] = clear_tail(fa[i], s * I8_BK + c * 16, C);
+                    for (int i = 0; i < MT; i++) fa[q & 1][i] = clear_tail(fa[q & 1][i], s * I8_BK + c * 16, C);
                 }
+            };
+            read(0);
+#pragma unroll
+            for (int q = 0; q < 4; q++) {
+                if (q < 3) read(q + 1);
+                __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
                 for (int i = 0; i < MT; i++)
 #pragma unroll
                     for (int j = 0; j < NT; j++)
-                        acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(fa[i], fw[j], acc[i][j], 0, 0, 0);
+                        acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(fa[q & 1][i], fw[q & 1][j], acc[i][j], 0, 0, 0);
+                __builtin_amdgcn_sched_barrier(0);
             }
-            lds_barrier();   // the next step's copies write the stage that was read here
+        };
+        const int full = C / I8_BK;
+        for (int s = 0; s < full; s++) step(s, std::false_type{});
+        if (full < S) step(full, std::true_type{});
+        wait_vm<0>();   // no copy may land in LDS that another work-group then owns
+    }
+    // The tile's sums, a row at a time: a wave lays 16 rows at a time of its
+    // blocks out in LDS (in the stages, that run() is done with) and each lane
+    // takes VEC neighbouring columns of one row, the same columns of every row
+    // (first_col()), so that a row's stores are 16 bytes wide:
+    // emit(row, sums, of_row) with the row counted within the tile and of_row the
+    // value that thread `row` handed in (a scale that is loaded once, ahead of
+    // the loop: loaded where it is used, each load's latency was paid 16 times
+    // per tile, 17 us of a 256 x 256 tile).  PAIR (w and w2): columns are
+    // counted over w's blocks 0, 2, .. and emit gets the sums of both,
+    // emit(row, sums, sums2, of_row).
+    static constexpr int PAD = NT * 32 + 8;   // dwords per row: the two half-waves write 4 rows apart, 32 banks apart
+    static_assert(NW * 16 * PAD * 4 + BM * 8 <= LDS && 64 * NW >= BM, "the layout fits the stages, a thread per row");
+    template <int VEC, bool PAIR = false>
+    static __device__ __forceinline__ int first_col() {
+        constexpr int COLS = PAIR ? NT * 16 : NT * 32;
+        return (int)(threadIdx.x >> 6) % WN * COLS + (threadIdx.x & 63) % (COLS / VEC) * VEC;
+    }
+    template <int VEC, bool PAIR = false, typename Emit>
+    static __device__ __forceinline__ void rows(uint8_t* lds, const v16i (&acc)[MT][NT], float2 of_row, Emit emit) {
+        constexpr int COLS = PAIR ? NT * 16 : NT * 32, LANES = COLS / VEC, ROWS = 64 / LANES;
+        static_assert(ROWS <= 16, "16 rows at a time");
+        const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+        const int wm = wave / WN;
+        float2* each = (float2*)lds;
+        int* at = (int*)(lds + BM * 8) + wave * 16 * PAD;
+        lds_barrier();   // every wave has read its last stage
+        if (threadIdx.x < BM) each[threadIdx.x] = of_row;
+        lds_barrier();
+#pragma unroll
+        for (int h = 0; h < 2 * MT; h++) {
+            // register v of a block: row 8 (v / 4) + 4 (lane / 32) + v % 4, column lane % 32
+#pragma unroll
+            for (int j = 0; j < NT; j++)
+#pragma unroll
+                for (int v = 0; v < 8; v++)
+                    at[(8 * (v >> 2) + 4 * (lane >> 5) + (v & 3)) * PAD + j * 32 + (lane & 31)] =
+                        acc[h >> 1][j][8 * (h & 1) + v];
+#pragma unroll
+            for (int q = 0; q < 16 / ROWS; q++) {
+                const int r = q * ROWS + lane / LANES, c = lane % LANES * VEC, m = wm * MT * 32 + h * 16 + r;
+                int x[VEC], y[VEC];
+                const int* p = at + r * PAD + (PAIR ? (c >> 5) * 64 + (c & 31) : c);
+#pragma unroll
+                for (int k = 0; k < VEC; k += 4) {
+                    *(v4i*)(x + k) = *(const v4i*)(p + k);
+                    if constexpr (PAIR) *(v4i*)(y + k) = *(const v4i*)(p + 32 + k);
+                }
+                if constexpr (PAIR) emit(m, x, y, each[m]);
+                else emit(m, x, each[m]);
+            }
         }
     }
-    // row of register i of a 32 x 32 block (column: lane & 31)
-    static __device__ __forceinline__ int reg_row(int i) { return 8 * (i >> 2) + 4 * ((threadIdx.x & 63) >> 5) + (i & 3); }
 };
+
+// n values at p (of which `count` are inside the row) as the type of p, in one
+// store of up to 16 bytes where `wide`
+template <int N, typename T>
+__device__ __forceinline__ void store_row(T* p, const float (&v)[N], int count, bool wide) {
+    typedef T vec __attribute__((ext_vector_type(N)));
+    if (wide && count >= N) {
+        vec o;
+#pragma unroll
+        for (int k = 0; k < N; k++) o[k] = (T)v[k];
+        *(vec*)p = o;
+    } else {
+#pragma unroll
+        for (int k = 0; k < N; k++)
+            if (k < count) p[k] = (T)v[k];
+    }
+}
 
 // row quantizer (int8.hip), for float rows of a type on the device
 void launch_i8_quantize(int type, const void* x, int64_t xs, int8_t* q, int64_t qs, float* scale, int64_t nrows,

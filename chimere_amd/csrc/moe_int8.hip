@@ -66,19 +66,18 @@ __global__ __launch_bounds__(1024) void k_i8_plan(MoeI8 a) {
     }
 }
 
-typedef I8Tile<2, 2, 1, 2> GuTile;    // 64 pairs x 64 columns of F, gate and up
-typedef I8Tile<2, 2, 1, 1> DnTile;    // 64 pairs x 64 columns of H
+typedef I8Tile<2, 2, 2, 2> GuTile;    // 128 pairs x 64 columns of F, gate and up
+typedef I8Tile<2, 2, 2, 2> DnTile;    // 128 pairs x 128 columns of H
 
 // Gate and up: the weight rows of a tile alternate in blocks of 32 between
-// gate and up, so a lane holds g and u of the same (pair, column).
+// gate and up, so g and u of the same (pair, column) meet in a lane.
 __global__ __launch_bounds__(64 * GuTile::NW) void k_i8_gate_up(MoeI8 a) {
-    extern __shared__ __align__(16) uint8_t lds[];
     typedef GuTile Tile;
+    __shared__ __align__(16) uint8_t lds[Tile::LDS];
     const int fb = (a.F + Tile::BN / 2 - 1) / (Tile::BN / 2), tile = blockIdx.x / fb;
     if (tile >= a.total[1]) return;
     const int4 t = a.tiles[tile];
     const int f0 = (blockIdx.x - tile * fb) * (Tile::BN / 2), lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int8_t* gate = a.gate + (int64_t)t.x * a.F * a.H;
     uint32_t aoff[Tile::PM], woff[Tile::PN];
 #pragma unroll
     for (int p = 0; p < Tile::PM; p++) {
@@ -90,31 +89,31 @@ __global__ __launch_bounds__(64 * GuTile::NW) void k_i8_gate_up(MoeI8 a) {
         const int r = (wave * Tile::PN + p) * 8 + (lane >> 3);
         woff[p] = (uint32_t)(min(f0 + (r >> 6) * 32 + (r & 31), a.F - 1)) * (uint32_t)a.H;
     }
-    constexpr int MT = Tile::MTILES, NT = Tile::NTILES;
-    v16i acc[MT][NT];
-    Tile::run(a.xq, gate, a.up + (int64_t)t.x * a.F * a.H, aoff, woff, a.H, lds, acc);
-    const int wm = wave / Tile::WAVES_N, wn = wave % Tile::WAVES_N;
-#pragma unroll
-    for (int j = 0; j < NT; j += 2) {
-        const int f = f0 + (wn * NT + j) / 2 * 32 + (lane & 31);
-        if (f >= a.F) continue;
-        const float sg = a.gate_s[(int64_t)t.x * a.F + f], su = a.up_s[(int64_t)t.x * a.F + f];
-#pragma unroll
-        for (int i = 0; i < MT; i++)
-#pragma unroll
-            for (int v = 0; v < 16; v++) {
-                const int r = (wm * MT + i) * 32 + Tile::reg_row(v);
-                if (r >= t.z) continue;
-                const float xs = a.xs[a.order[t.y + r] / a.K];
-                const float g = (float)acc[i][j][v] * xs * sg, u = (float)acc[i][j + 1][v] * xs * su;
-                a.h[(int64_t)(t.y + r) * a.F + f] = det_silu(g) * u;
-            }
-    }
+    const int64_t e = t.x;
+    const float xs = threadIdx.x < Tile::BM ? a.xs[a.order[t.y + min((int)threadIdx.x, t.z - 1)] / a.K] : 0.0f;
+    v16i acc[Tile::MTILES][Tile::NTILES];
+    Tile::run(a.xq, a.gate + e * a.F * a.H, a.up + e * a.F * a.H, aoff, woff, a.H, lds, acc);
+    constexpr int VEC = 4;
+    const int f = f0 + Tile::first_col<VEC, true>();
+    const bool in = f < a.F;   // F is a multiple of 16: all four columns or none
+    const float4 sg = in ? *(const float4*)(a.gate_s + e * a.F + f) : float4{};
+    const float4 su = in ? *(const float4*)(a.up_s + e * a.F + f) : float4{};
+    Tile::rows<VEC, true>(lds, acc, make_float2(xs, 0.0f),
+                          [&](int r, const int(&g)[VEC], const int(&u)[VEC], float2 of_row) {
+        if (r >= t.z || !in) return;
+        const float s = of_row.x;
+        float4 h;
+        h.x = det_silu((float)g[0] * s * sg.x) * ((float)u[0] * s * su.x);
+        h.y = det_silu((float)g[1] * s * sg.y) * ((float)u[1] * s * su.y);
+        h.z = det_silu((float)g[2] * s * sg.z) * ((float)u[2] * s * su.z);
+        h.w = det_silu((float)g[3] * s * sg.w) * ((float)u[3] * s * su.w);
+        *(float4*)(a.h + (int64_t)(t.y + r) * a.F + f) = h;
+    });
 }
 
 __global__ __launch_bounds__(64 * DnTile::NW) void k_i8_down(MoeI8 a) {
-    extern __shared__ __align__(16) uint8_t lds[];
     typedef DnTile Tile;
+    __shared__ __align__(16) uint8_t lds[Tile::LDS];
     const int hb = (a.H + Tile::BN - 1) / Tile::BN, tile = blockIdx.x / hb;
     if (tile >= a.total[1]) return;
     const int4 t = a.tiles[tile];
@@ -126,24 +125,23 @@ __global__ __launch_bounds__(64 * DnTile::NW) void k_i8_down(MoeI8 a) {
 #pragma unroll
     for (int p = 0; p < Tile::PN; p++)
         woff[p] = (uint32_t)min(n0 + (wave * Tile::PN + p) * 8 + (lane >> 3), a.H - 1) * (uint32_t)a.F;
-    constexpr int MT = Tile::MTILES, NT = Tile::NTILES;
-    v16i acc[MT][NT];
-    const int8_t* w = a.down + (int64_t)t.x * a.H * a.F;
+    const int64_t e = t.x;
+    const int row = t.y + min((int)threadIdx.x, t.z - 1);
+    const float2 mine = threadIdx.x < Tile::BM ? make_float2(a.hs[row], __builtin_bit_cast(float, a.order[row]))
+                                               : float2{};
+    v16i acc[Tile::MTILES][Tile::NTILES];
+    const int8_t* w = a.down + e * a.H * a.F;
     Tile::run(a.hq + (int64_t)t.y * a.F, w, w, aoff, woff, a.F, lds, acc);
-    const int wm = wave / Tile::WAVES_N, wn = wave % Tile::WAVES_N;
-#pragma unroll
-    for (int j = 0; j < NT; j++) {
-        const int n = n0 + (wn * NT + j) * 32 + (lane & 31);
-        if (n >= a.H) continue;
-        const float s = a.down_s[(int64_t)t.x * a.H + n];
-#pragma unroll
-        for (int i = 0; i < MT; i++)
-#pragma unroll
-            for (int v = 0; v < 16; v++) {
-                const int r = (wm * MT + i) * 32 + Tile::reg_row(v);
-                if (r < t.z) a.y[(int64_t)a.order[t.y + r] * a.H + n] = (float)acc[i][j][v] * a.hs[t.y + r] * s;
-            }
-    }
+    constexpr int VEC = 4;
+    const int n = n0 + Tile::first_col<VEC>();
+    const bool in = n < a.H;   // H is a multiple of 16: all four columns or none
+    const float4 sd = in ? *(const float4*)(a.down_s + e * a.H + n) : float4{};
+    Tile::rows<VEC>(lds, acc, mine, [&](int r, const int(&x)[VEC], float2 of_row) {
+        if (r >= t.z || !in) return;
+        const float s = of_row.x;
+        *(float4*)(a.y + (int64_t)__builtin_bit_cast(int, of_row.y) * a.H + n) =
+            make_float4((float)x[0] * s * sd.x, (float)x[1] * s * sd.y, (float)x[2] * s * sd.z, (float)x[3] * s * sd.w);
+    });
 }
 
 // out[t] = sum over k, ascending, of w[t][k] y[t][k]; a pair whose id is no
@@ -211,8 +209,9 @@ void chimere_moe_i8(const chimere_moe_i8_layer* L, int type, const void* x, int6
                     L->hidden, L->ffn, L->n_experts, top_k, ntok);
     CHIMERE_REQUIRE(L->gate && L->up && L->down && L->gate_scale && L->up_scale && L->down_scale, CHIMERE_ERR_ARG,
                     "moe_i8: null weight pointer");
-    CHIMERE_REQUIRE((((uintptr_t)L->gate | (uintptr_t)L->up | (uintptr_t)L->down) & 15) == 0, CHIMERE_ERR_ARG,
-                    "moe_i8: weights must be 16-byte aligned");
+    CHIMERE_REQUIRE((((uintptr_t)L->gate | (uintptr_t)L->up | (uintptr_t)L->down | (uintptr_t)L->gate_scale |
+                      (uintptr_t)L->up_scale | (uintptr_t)L->down_scale) & 15) == 0, CHIMERE_ERR_ARG,
+                    "moe_i8: weights and scales must be 16-byte aligned");
     if (ntok == 0) return;
     CHIMERE_REQUIRE(x && ids && weights && out && workspace, CHIMERE_ERR_ARG, "moe_i8: null pointer");
     CHIMERE_REQUIRE(x_stride >= 0 && out_stride >= L->hidden, CHIMERE_ERR_ARG, "moe_i8: bad strides %lld %lld",
@@ -234,9 +233,9 @@ void chimere_moe_i8(const chimere_moe_i8_layer* L, int type, const void* x, int6
     launch_i8_quantize(type, x, x_stride, (int8_t*)a.xq, H, (float*)a.xs, ntok, H, stream);
     hipLaunchKernelGGL(k_i8_plan, dim3(1), dim3(1024), 0, stream, a);
     const int fb = (F + GuTile::BN / 2 - 1) / (GuTile::BN / 2), hb = (H + DnTile::BN - 1) / DnTile::BN;
-    hipLaunchKernelGGL(k_i8_gate_up, dim3((unsigned)(p.max_tiles * fb)), dim3(64 * GuTile::NW), GuTile::LDS, stream, a);
+    hipLaunchKernelGGL(k_i8_gate_up, dim3((unsigned)(p.max_tiles * fb)), dim3(64 * GuTile::NW), 0, stream, a);
     launch_i8_quantize(T_F32, a.h, F, a.hq, F, a.hs, (int64_t)ntok * top_k, F, stream);
-    hipLaunchKernelGGL(k_i8_down, dim3((unsigned)(p.max_tiles * hb)), dim3(64 * DnTile::NW), DnTile::LDS, stream, a);
+    hipLaunchKernelGGL(k_i8_down, dim3((unsigned)(p.max_tiles * hb)), dim3(64 * DnTile::NW), 0, stream, a);
     const dim3 grid((unsigned)((H + 255) / 256) * ntok);
     if (out_type == T_F32) hipLaunchKernelGGL(k_i8_combine<float>, grid, dim3(256), 0, stream, a);
     else if (out_type == T_F16) hipLaunchKernelGGL(k_i8_combine<_Float16>, grid, dim3(256), 0, stream, a);

@@ -327,7 +327,7 @@ typedef struct chimere_moe_i8_layer {
     int n_experts;           /* E <= 1024; top_k <= 16 */
     const int8_t *gate, *up; /* [E][F][H], 16-byte aligned */
     const int8_t *down;      /* [E][H][F] */
-    const float *gate_scale, *up_scale; /* [E][F] */
+    const float *gate_scale, *up_scale; /* [E][F], 16-byte aligned as well */
     const float *down_scale; /* [E][H] */
 } chimere_moe_i8_layer;
 /* Workspace for up to max_ntok tokens (0: shape out of range), 256-byte
