@@ -119,7 +119,7 @@ def lib():
 def check():
     """Raise ChimereError if the last C-ABI call on this thread recorded an error."""
     L = lib()
-    msg = L.chimere_hip_get_last_error_string()
     code = L.chimere_hip_get_last_error()
     if code != 0:
+        msg = L.chimere_hip_get_last_error_string()
         raise ChimereError(code, msg.decode() if msg else "")

@@ -1,12 +1,12 @@
 // balance.hip -- per-expert counts and the balance loss of a router's choice,
 // and the gradient of its logits.  No counterpart in the reference.
+#include <type_traits>
+
 #include "api_internal.h"
 #include "float_rows.h"
 #include "moe_common.h"
 
 namespace chimere {
-
-constexpr int BAL_COLS = MAX_E / 64;    // columns per lane
 
 struct Balance {
     const int* ids;
@@ -17,141 +17,337 @@ struct Balance {
     int E, K, T, groups;
     float* psum;     // [groups][E]
     int *pcnt, *pn;  // [groups][E], [groups]
+    float* lpart;    // parts of the loss, one per work-group of k_balance_loss
+    int* done;       // how many of them have ended
     float *loss, *probs;
     int *counts_out, *tokens_out;
+    bool wide;       // rows of logits (and grad) start on multiples of four elements
 };
 
-__device__ __forceinline__ float wave_sum(float v) {
-    v += xlane<32>(v);
-    v += xlane<16>(v);
-    v += xlane<8>(v);
-    v += xlane<4>(v);
-    v += xlane<2>(v);
-    return v + xlane<1>(v);
-}
-__device__ __forceinline__ float wave_max(float v) {
-    v = __builtin_fmaxf(v, xlane<32>(v));
-    v = __builtin_fmaxf(v, xlane<16>(v));
-    v = __builtin_fmaxf(v, xlane<8>(v));
-    v = __builtin_fmaxf(v, xlane<4>(v));
-    v = __builtin_fmaxf(v, xlane<2>(v));
-    return __builtin_fmaxf(v, xlane<1>(v));
+// e^x for x <= 0 (x a difference from the maximum): 2^(x log2 e) by the
+// hardware's exponential, with what the product x log2 e is off by (exactly
+// known from the fma, log2 e in two parts) put right to first order: about 2
+// units in the last place, at half of det_exp's instructions, and the sums over
+// rows are bound by these.  Below e^-86 it comes to 0.
+__device__ __forceinline__ float bal_exp(float x) {
+    constexpr float HI = 0x1.715476p+0f, LO = 0x1.4ae0cp-26f, LN2 = 0x1.62e430p-1f;
+    x = x < -120.0f ? -120.0f : x;   // (not a maximum: a NaN stays)
+    const float t = x * HI, off = __builtin_fmaf(x, LO, __builtin_fmaf(x, HI, -t));
+    const float e = __builtin_amdgcn_exp2f(t);
+    return __builtin_fmaf(e, off * LN2, e);
 }
 
-// softmax of one row by one wave (lane l: columns l, l + 64, ...); a row of
-// -inf alone has no probabilities: zeros
-template <typename T>
-__device__ __forceinline__ void softmax_row(const T* row, int E, float (&p)[BAL_COLS]) {
-    const int lane = threadIdx.x & 63;
-    float m = -__builtin_huge_valf();
-#pragma unroll
-    for (int i = 0; i < BAL_COLS; i++) {
-        p[i] = lane + 64 * i < E ? load_f(row + lane + 64 * i) : -__builtin_huge_valf();
-        m = __builtin_fmaxf(m, p[i]);
-    }
-    m = wave_max(m);
-    float s = 0.0f;
-    bool nan = false;
-#pragma unroll
-    for (int i = 0; i < BAL_COLS; i++) nan |= p[i] != p[i];
-    const bool none = m == -__builtin_huge_valf() && !__any(nan);
-#pragma unroll
-    for (int i = 0; i < BAL_COLS; i++) {
-        p[i] = lane + 64 * i < E && !none ? det_exp(p[i] - m) : 0.0f;
-        s += p[i];
-    }
-    s = wave_sum(s);
-    const float r = none ? 0.0f : 1.0f / s;
-#pragma unroll
-    for (int i = 0; i < BAL_COLS; i++) p[i] *= r;
-}
+// Sixteen lanes per row, lane l of them the columns 64 i + 4 l .. + 3 for
+// i < NV: a row of E = 256 is four loads of 16 bytes per lane, and the sums
+// over a row are four DPP steps for four rows at once (one wave per row: six
+// steps each).
+template <int NV>
+struct BalRow {
+    float v[4 * NV];
 
-template <typename T>
-__global__ __launch_bounds__(256) void k_balance_sums(Balance b, const T* __restrict__ logits) {
-    __shared__ float part[4][MAX_E];
-    __shared__ int cnt[MAX_E], n;
-    const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
-    for (int e = tid; e < b.E; e += 256) cnt[e] = 0;
-    if (tid == 0) n = 0;
-    __syncthreads();
-    float sum[BAL_COLS] = {};
-    int rows = 0;
-    for (int t = blockIdx.x * 4 + wave; t < b.T; t += b.groups * 4) {
-        if (b.mask && !b.mask[t]) continue;
-        rows++;
-        float p[BAL_COLS];
-        softmax_row(logits + t * b.ld, b.E, p);
+    template <typename T>
+    __device__ __forceinline__ void load(const T* row, int E, bool wide) {
+        typedef T vec __attribute__((ext_vector_type(4)));
+        const int l = threadIdx.x & 15;
 #pragma unroll
-        for (int i = 0; i < BAL_COLS; i++) sum[i] += p[i];
-        for (int k = lane; k < b.K; k += 64) {
-            const int e = b.ids[(int64_t)t * b.K + k];
-            if ((unsigned)e < (unsigned)b.E) atomicAdd(&cnt[e], 1);
+        for (int i = 0; i < NV; i++) {
+            const int c = 64 * i + 4 * l;
+            if (wide && c + 4 <= E) {
+                const vec x = *(const vec*)(row + c);
+#pragma unroll
+                for (int k = 0; k < 4; k++) v[4 * i + k] = (float)x[k];
+            } else {
+#pragma unroll
+                for (int k = 0; k < 4; k++) v[4 * i + k] = c + k < E ? load_f(row + c + k) : -__builtin_huge_valf();
+            }
         }
     }
+    // softmax of the loaded row; one of -inf alone has no probabilities: zeros
+    __device__ __forceinline__ void softmax() {
+        float m = v[0];
+        bool nan = false;
 #pragma unroll
-    for (int i = 0; i < BAL_COLS; i++) part[wave][lane + 64 * i] = sum[i];
-    if (lane == 0) atomicAdd(&n, rows);
-    __syncthreads();
-    for (int e = tid; e < b.E; e += 256) {
-        b.psum[(int64_t)blockIdx.x * b.E + e] = (part[0][e] + part[1][e]) + (part[2][e] + part[3][e]);
-        b.pcnt[(int64_t)blockIdx.x * b.E + e] = cnt[e];
+        for (int i = 0; i < 4 * NV; i++) {
+            m = __builtin_fmaxf(m, v[i]);
+            nan |= v[i] != v[i];
+        }
+        m = __builtin_fmaxf(m, xlane<8>(m));
+        m = __builtin_fmaxf(m, xlane<4>(m));
+        m = __builtin_fmaxf(m, xlane<2>(m));
+        m = __builtin_fmaxf(m, xlane<1>(m));
+        // where all are -inf: 0 instead, so that every exponential is 0 (a NaN among them stays one)
+        const float from = m == -__builtin_huge_valf() ? 0.0f : m;
+        float s = 0.0f;
+#pragma unroll
+        for (int i = 0; i < NV; i++) {
+#pragma unroll
+            for (int k = 0; k < 4; k++) v[4 * i + k] = bal_exp(v[4 * i + k] - from);
+            s += (v[4 * i] + v[4 * i + 1]) + (v[4 * i + 2] + v[4 * i + 3]);
+        }
+        s = slot_reduce16(s);
+        const float r = s == 0.0f ? 0.0f : 1.0f / s;
+#pragma unroll
+        for (int i = 0; i < 4 * NV; i++) v[i] *= r;
     }
-    if (tid == 0) b.pn[blockIdx.x] = n;
+};
+
+// Columns past E hold exponentials of -inf: 0.
+
+// threads of a work-group of the sums: 16 waves, for more than 512 experts (64
+// values and as many sums per lane) eight, so that none is spilled
+template <int NV>
+constexpr int BAL_THREADS = NV > 8 ? 512 : 1024;
+
+// Probabilities and pairs summed over the rows of each work-group (row t of
+// round i: (i * groups + group) * 64 + ..), every sum in a fixed order: a lane
+// over its rows, four rows of a wave, the waves.  Counts are integers: LDS
+// atomics in any order.  With one work-group the results follow at once.
+template <typename T, int NV, bool ONE>
+__global__ __launch_bounds__(BAL_THREADS<NV>) void k_balance_sums(Balance b, const T* __restrict__ logits) {
+    constexpr int THREADS = BAL_THREADS<NV>, ROWS = THREADS / 16;
+    __shared__ float part[THREADS / 64][64 * NV];
+    __shared__ float lpart[THREADS / 64];
+    __shared__ int cnt[64 * NV], n;
+    const int tid = threadIdx.x, wave = tid >> 6;
+    for (int e = tid; e < 64 * NV; e += THREADS) cnt[e] = 0;
+    if (tid == 0) n = 0;
+    if (!ONE && blockIdx.x == 0 && tid == 0) *b.done = 0;   // for k_balance_loss, that follows
+    __syncthreads();
+    float sum[4 * NV] = {};
+    int rows = 0;
+    // the next round's row is loaded while this one's is summed up
+    BalRow<NV> row, next;
+    auto fetch = [&](int t, BalRow<NV>& r) {
+        const bool on = t < b.T && (!b.mask || b.mask[t]);
+        if (on) r.load(logits + t * b.ld, b.E, b.wide);
+        return on;
+    };
+    bool on = fetch(blockIdx.x * ROWS + (tid >> 4), row);
+    for (int t0 = blockIdx.x * ROWS; t0 < b.T; t0 += b.groups * ROWS) {
+        const bool more = fetch(t0 + b.groups * ROWS + (tid >> 4), next);
+        const int pairs = min(ROWS, b.T - t0) * b.K;
+        const int* ids = b.ids + (int64_t)t0 * b.K;
+        for (int p = tid; p < pairs; p += THREADS) {
+            const int e = ids[p];
+            if ((unsigned)e < (unsigned)b.E && (!b.mask || b.mask[t0 + p / b.K])) atomicAdd(&cnt[e], 1);
+        }
+        if (on) {
+            row.softmax();
+#pragma unroll
+            for (int i = 0; i < 4 * NV; i++) sum[i] += row.v[i];
+            rows += (tid & 15) == 0;
+        }
+        row = next;
+        on = more;
+    }
+#pragma unroll
+    for (int i = 0; i < 4 * NV; i++) {
+        sum[i] += xlane<16>(sum[i]);
+        sum[i] += xlane<32>(sum[i]);
+    }
+    if ((tid & 63) < 16)
+#pragma unroll
+        for (int i = 0; i < NV; i++)
+            *(float4*)&part[wave][64 * i + 4 * (tid & 15)] =
+                make_float4(sum[4 * i], sum[4 * i + 1], sum[4 * i + 2], sum[4 * i + 3]);
+    if (rows) atomicAdd(&n, rows);
+    __syncthreads();
+    auto psum = [&](int e) {
+        float v = 0.0f;
+#pragma unroll
+        for (int w = 0; w < THREADS / 64; w++) v += part[w][e];
+        return v;
+    };
+    if constexpr (ONE) {
+        float l = 0.0f;
+        for (int e = tid; e < b.E; e += THREADS) {
+            const float p = n ? psum(e) / (float)n : 0.0f;
+            b.probs[e] = p;
+            b.counts_out[e] = cnt[e];
+            l += n ? (float)cnt[e] / ((float)n * (float)b.K) * p : 0.0f;
+        }
+        l = slot_reduce16(l);
+        l += xlane<16>(l);
+        l += xlane<32>(l);
+        if ((tid & 63) == 0) lpart[wave] = l;
+        __syncthreads();
+        if (tid == 0) {
+            float v = 0.0f;
+            for (int i = 0; i < THREADS / 64; i++) v += lpart[i];
+            *b.loss = (float)b.E * v;
+            *b.tokens_out = n;
+        }
+    } else {
+        for (int e = tid; e < b.E; e += THREADS) {
+            b.psum[(int64_t)blockIdx.x * b.E + e] = psum(e);
+            b.pcnt[(int64_t)blockIdx.x * b.E + e] = cnt[e];
+        }
+        if (tid == 0) b.pn[blockIdx.x] = n;
+    }
 }
 
-__global__ __launch_bounds__(1024) void k_balance_loss(Balance b) {
-    __shared__ float part[16];
-    __shared__ int n;
-    const int e = threadIdx.x;
-    if (e == 0) {
-        n = 0;
-        for (int g = 0; g < b.groups; g++) n += b.pn[g];
-    }
+// The work-groups' sums joined, 32 experts per work-group by eight segments of
+// them (one work-group for all experts read 256 x 256 sums in 7 us); the last
+// work-group to end adds up the parts of the loss, in their order.
+constexpr int BAL_JOIN = 32;
+__global__ __launch_bounds__(256) void k_balance_loss(Balance b) {
+    __shared__ float ps[256], part[MAX_E / BAL_JOIN];
+    __shared__ int pc[256], n, last;
+    const int tid = threadIdx.x, seg = tid / BAL_JOIN, e = blockIdx.x * BAL_JOIN + tid % BAL_JOIN;
+    if (tid == 0) n = 0;
     __syncthreads();
     float s = 0.0f;
     int c = 0;
     if (e < b.E) {
-        for (int g = 0; g < b.groups; g++) {
+#pragma unroll 8
+        for (int g = seg; g < b.groups; g += 256 / BAL_JOIN) {
             s += b.psum[(int64_t)g * b.E + e];
             c += b.pcnt[(int64_t)g * b.E + e];
+        }
+    }
+    ps[tid] = s;
+    pc[tid] = c;
+    if (tid < b.groups) atomicAdd(&n, b.pn[tid]);
+    __syncthreads();
+    float l = 0.0f;
+    if (tid < BAL_JOIN && e < b.E) {
+#pragma unroll
+        for (int i = 1; i < 256 / BAL_JOIN; i++) {
+            s += ps[i * BAL_JOIN + tid];
+            c += pc[i * BAL_JOIN + tid];
         }
         s = n ? s / (float)n : 0.0f;
         b.probs[e] = s;
         b.counts_out[e] = c;
+        l = n ? (float)c / ((float)n * (float)b.K) * s : 0.0f;
     }
-    const float l = wave_sum(n ? (float)c / ((float)n * (float)b.K) * s : 0.0f);
-    if ((e & 63) == 0) part[e >> 6] = l;
+    l = slot_reduce16(l);
+    l += xlane<16>(l);
+    if (tid == 0) {
+        // visible to the whole device before the count says so
+        __hip_atomic_store(&b.lpart[blockIdx.x], l, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        last = __hip_atomic_fetch_add(b.done, 1, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT) == (int)gridDim.x - 1;
+    }
     __syncthreads();
-    if (e == 0) {
+    if (!last) return;
+    if (tid < gridDim.x) part[tid] = __hip_atomic_load(&b.lpart[tid], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    __syncthreads();
+    if (tid == 0) {
         float v = 0.0f;
-        for (int i = 0; i < 16; i++) v += part[i];
+        for (int i = 0; i < (int)gridDim.x; i++) v += part[i];
         *b.loss = (float)b.E * v;
         *b.tokens_out = n;
     }
 }
 
-template <typename T>
+template <typename T, int NV>
 __global__ __launch_bounds__(256) void k_balance_grad(Balance b, const T* __restrict__ logits, T* __restrict__ grad) {
-    const int lane = threadIdx.x & 63;
-    const int n = *b.tokens;
+    typedef T vec __attribute__((ext_vector_type(4)));
+    const int l = threadIdx.x & 15, n = *b.tokens;
     const float all = n ? 1.0f / ((float)n * (float)b.K) : 0.0f;
     const float c = n ? *b.grad_loss * (float)b.E / (float)n : 0.0f;
-    float f[BAL_COLS];
+    float f[4 * NV];
 #pragma unroll
-    for (int i = 0; i < BAL_COLS; i++) f[i] = lane + 64 * i < b.E ? (float)b.counts[lane + 64 * i] * all : 0.0f;
-    for (int t = blockIdx.x * 4 + (threadIdx.x >> 6); t < b.T; t += gridDim.x * 4) {
-        float p[BAL_COLS] = {}, d = 0.0f;
-        if (!b.mask || b.mask[t]) softmax_row(logits + t * b.ld, b.E, p);
+    for (int i = 0; i < NV; i++) {
+        const int e = 64 * i + 4 * l;
+        int4 x = make_int4(0, 0, 0, 0);
+        if (e + 4 <= b.E && ((uintptr_t)b.counts & 15) == 0) {
+            x = *(const int4*)(b.counts + e);
+        } else {
+            if (e < b.E) x.x = b.counts[e];
+            if (e + 1 < b.E) x.y = b.counts[e + 1];
+            if (e + 2 < b.E) x.z = b.counts[e + 2];
+            if (e + 3 < b.E) x.w = b.counts[e + 3];
+        }
+        f[4 * i] = (float)x.x * all;
+        f[4 * i + 1] = (float)x.y * all;
+        f[4 * i + 2] = (float)x.z * all;
+        f[4 * i + 3] = (float)x.w * all;
+    }
+    BalRow<NV> p, next;
+    auto fetch = [&](int t, BalRow<NV>& r) {
+        const bool on = t < b.T && (!b.mask || b.mask[t]);
+        if (on) r.load(logits + t * b.ld, b.E, b.wide);
+        return on;
+    };
+    const int first = blockIdx.x * 16 + (threadIdx.x >> 4);
+    bool on = fetch(first, p);
+    for (int t = first; t < b.T; t += gridDim.x * 16) {
+        const bool more = fetch(t + gridDim.x * 16, next);
+        float d = 0.0f;
+        if (on) {
+            p.softmax();
 #pragma unroll
-        for (int i = 0; i < BAL_COLS; i++) d = __builtin_fmaf(f[i], p[i], d);
-        d = wave_sum(d);
+            for (int i = 0; i < 4 * NV; i += 4)
+                d += __builtin_fmaf(f[i], p.v[i], f[i + 1] * p.v[i + 1]) +
+                     __builtin_fmaf(f[i + 2], p.v[i + 2], f[i + 3] * p.v[i + 3]);
+            d = slot_reduce16(d);
+        }
+        T* to = grad + t * b.ldg;
 #pragma unroll
-        for (int i = 0; i < BAL_COLS; i++)
-            if (lane + 64 * i < b.E) store_f(grad + t * b.ldg + lane + 64 * i, c * p[i] * (f[i] - d));
+        for (int i = 0; i < NV; i++) {
+            const int e = 64 * i + 4 * l;
+            float o[4];
+#pragma unroll
+            for (int k = 0; k < 4; k++) o[k] = on ? c * p.v[4 * i + k] * (f[4 * i + k] - d) : 0.0f;
+            if (b.wide && e + 4 <= b.E) {
+                vec x;
+#pragma unroll
+                for (int k = 0; k < 4; k++) x[k] = (T)o[k];
+                *(vec*)(to + e) = x;
+            } else {
+#pragma unroll
+                for (int k = 0; k < 4; k++)
+                    if (e + k < b.E) store_f(to + e + k, o[k]);
+            }
+        }
+        p = next;
+        on = more;
     }
 }
 
-static int balance_groups(int T) { return T < 1024 ? (T + 3) / 4 : 256; }
+// Work-groups of the sums of T rows: one, that also finishes, up to BAL_ONE rows.
+constexpr int BAL_ONE = 256, BAL_GROUPS = 256, BAL_GRAD = 1024;
+static int balance_groups(int T, int E) {
+    const int n = (T + (E > 512 ? 31 : 63)) / (E > 512 ? 32 : 64);
+    return T <= BAL_ONE ? 1 : n < BAL_GROUPS ? n : BAL_GROUPS;
+}
+
+template <typename T, int NV>
+static void launch_balance(const Balance& b, const void* logits, hipStream_t s) {
+    if (b.groups == 1) {
+        hipLaunchKernelGGL((k_balance_sums<T, NV, true>), dim3(1), dim3(BAL_THREADS<NV>), 0, s, b, (const T*)logits);
+    } else {
+        hipLaunchKernelGGL((k_balance_sums<T, NV, false>), dim3(b.groups), dim3(BAL_THREADS<NV>), 0, s, b, (const T*)logits);
+        hipLaunchKernelGGL(k_balance_loss, dim3((b.E + BAL_JOIN - 1) / BAL_JOIN), dim3(256), 0, s, b);
+    }
+}
+
+template <typename T, int NV>
+static void launch_balance_grad(const Balance& b, const void* logits, void* grad, hipStream_t s) {
+    const int n = (b.T + 15) / 16;
+    hipLaunchKernelGGL((k_balance_grad<T, NV>), dim3(n < BAL_GRAD ? n : BAL_GRAD), dim3(256), 0, s, b, (const T*)logits, (T*)grad);
+}
+
+// f(type of the rows, NV of E columns)
+template <typename F>
+static void balance_kind(int type, int E, F f) {
+    auto width = [&](auto t) {
+        if (E <= 64) f(t, std::integral_constant<int, 1>{});
+        else if (E <= 128) f(t, std::integral_constant<int, 2>{});
+        else if (E <= 256) f(t, std::integral_constant<int, 4>{});
+        else if (E <= 512) f(t, std::integral_constant<int, 8>{});
+        else f(t, std::integral_constant<int, 16>{});
+    };
+    if (type == T_F32) width((float*)nullptr);
+    else if (type == T_F16) width((_Float16*)nullptr);
+    else width((__bf16*)nullptr);
+}
+
+static bool balance_wide(int type, const void* p, int64_t ld) {
+    const int size = type == T_F32 ? 4 : 2;
+    return (((uintptr_t)p | (uintptr_t)(ld * size)) & (4 * size - 1)) == 0;
+}
 
 }  // namespace chimere
 
@@ -161,8 +357,9 @@ extern "C" {
 
 size_t chimere_balance_loss_workspace_size(int n_experts, int max_ntok) {
     if (n_experts < 1 || n_experts > MAX_E || max_ntok < 0) return 0;
-    const size_t g = balance_groups(max_ntok) + 1;
-    return 2 * al256(g * n_experts * 4) + al256(g * 4);
+    const size_t g = balance_groups(max_ntok, n_experts);
+    if (g == 1) return 0;
+    return 2 * al256(g * n_experts * 4) + al256(g * 4) + 256;
 }
 
 static bool balance_args(const char* what, int type, const void* logits, int64_t ld, int E, int K, int T) {
@@ -181,27 +378,24 @@ void chimere_balance_loss(int type, const void* logits, int64_t logits_stride, c
                           const uint8_t* mask, float* loss, float* probs, int* counts, int* tokens, int n_experts,
                           int ntok, void* workspace, size_t workspace_bytes, hipStream_t stream) {
     if (!balance_args("balance_loss", type, logits, logits_stride, n_experts, top_k, ntok)) return;
-    CHIMERE_REQUIRE(loss && probs && counts && tokens && workspace && (ids || ntok == 0), CHIMERE_ERR_ARG,
-                    "balance_loss: null pointer");
     const size_t need = chimere_balance_loss_workspace_size(n_experts, ntok);
+    CHIMERE_REQUIRE(loss && probs && counts && tokens && (workspace || !need) && (ids || ntok == 0), CHIMERE_ERR_ARG,
+                    "balance_loss: null pointer");
     CHIMERE_REQUIRE(workspace_bytes >= need && ((uintptr_t)workspace & 255) == 0, CHIMERE_ERR_WORKSPACE,
                     "balance_loss: workspace %zu bytes < %zu (or not 256-byte aligned)", workspace_bytes, need);
     Balance b{};
     b.ids = ids; b.mask = mask; b.ld = logits_stride;
-    b.E = n_experts; b.K = top_k; b.T = ntok; b.groups = balance_groups(ntok);
+    b.E = n_experts; b.K = top_k; b.T = ntok; b.groups = balance_groups(ntok, n_experts);
     uint8_t* w = (uint8_t*)workspace;
-    const size_t one = al256((size_t)(b.groups + 1) * n_experts * 4);
+    const size_t one = al256((size_t)b.groups * n_experts * 4);
     b.psum = (float*)w; b.pcnt = (int*)(w + one); b.pn = (int*)(w + 2 * one);
+    b.lpart = (float*)(w + 2 * one + al256((size_t)b.groups * 4));
+    b.done = (int*)(b.lpart + MAX_E / BAL_JOIN);
     b.loss = loss; b.probs = probs; b.counts_out = counts; b.tokens_out = tokens;
-    if (b.groups) {
-        if (type == T_F32)
-            hipLaunchKernelGGL(k_balance_sums<float>, dim3(b.groups), dim3(256), 0, stream, b, (const float*)logits);
-        else if (type == T_F16)
-            hipLaunchKernelGGL(k_balance_sums<_Float16>, dim3(b.groups), dim3(256), 0, stream, b, (const _Float16*)logits);
-        else
-            hipLaunchKernelGGL(k_balance_sums<__bf16>, dim3(b.groups), dim3(256), 0, stream, b, (const __bf16*)logits);
-    }
-    hipLaunchKernelGGL(k_balance_loss, dim3(1), dim3(1024), 0, stream, b);
+    b.wide = balance_wide(type, logits, logits_stride);
+    balance_kind(type, n_experts, [&](auto t, auto nv) {
+        launch_balance<std::remove_pointer_t<decltype(t)>, decltype(nv)::value>(b, logits, stream);
+    });
     check_launch("balance_loss");
 }
 
@@ -214,13 +408,10 @@ void chimere_balance_loss_grad(int type, const void* logits, int64_t logits_stri
     Balance b{};
     b.mask = mask; b.counts = counts; b.tokens = tokens; b.grad_loss = grad_loss;
     b.ld = logits_stride; b.ldg = grad_stride; b.E = n_experts; b.K = top_k; b.T = ntok;
-    const dim3 grid(ntok < 8192 ? (ntok + 3) / 4 : 2048);
-    if (type == T_F32)
-        hipLaunchKernelGGL(k_balance_grad<float>, grid, dim3(256), 0, stream, b, (const float*)logits, (float*)grad);
-    else if (type == T_F16)
-        hipLaunchKernelGGL(k_balance_grad<_Float16>, grid, dim3(256), 0, stream, b, (const _Float16*)logits, (_Float16*)grad);
-    else
-        hipLaunchKernelGGL(k_balance_grad<__bf16>, grid, dim3(256), 0, stream, b, (const __bf16*)logits, (__bf16*)grad);
+    b.wide = balance_wide(type, logits, logits_stride) && balance_wide(type, grad, grad_stride);
+    balance_kind(type, n_experts, [&](auto t, auto nv) {
+        launch_balance_grad<std::remove_pointer_t<decltype(t)>, decltype(nv)::value>(b, logits, grad, stream);
+    });
     check_launch("balance_loss_grad");
 }
 

@@ -447,7 +447,7 @@ void chimere_gemm_i8(const int8_t* a, int64_t a_stride, const float* a_scale, co
 }
 
 size_t chimere_linear_i8_workspace_size(int max_ntok, int ncols) {
-    if (max_ntok < 1 || ncols < 1 || ncols > I8_MAX_C) return 0;
+    if (max_ntok < 1 || ncols < 1 || ncols > I8_MAX_C || quantizes_itself(max_ntok, ncols)) return 0;
     return al256((size_t)max_ntok * pad_to(ncols, 16)) + al256((size_t)max_ntok * 4);
 }
 
@@ -456,9 +456,9 @@ void chimere_linear_i8(int type, const void* x, int64_t x_stride, const int8_t* 
                        int nrows, int ncols, void* workspace, size_t workspace_bytes, hipStream_t stream) {
     CHIMERE_REQUIRE(float_type(type), CHIMERE_ERR_ARG, "linear_i8: unsupported type %d", type);
     if (!gemm_args("linear_i8", w, w_stride, w_scale, out_type, out, out_stride, ntok, nrows, ncols) || ntok == 0) return;
-    CHIMERE_REQUIRE(x && workspace, CHIMERE_ERR_ARG, "linear_i8: null pointer");
-    CHIMERE_REQUIRE(x_stride >= 0, CHIMERE_ERR_ARG, "linear_i8: bad stride %lld", (long long)x_stride);
     const size_t need = chimere_linear_i8_workspace_size(ntok, ncols);
+    CHIMERE_REQUIRE(x && (workspace || !need), CHIMERE_ERR_ARG, "linear_i8: null pointer");
+    CHIMERE_REQUIRE(x_stride >= 0, CHIMERE_ERR_ARG, "linear_i8: bad stride %lld", (long long)x_stride);
     CHIMERE_REQUIRE(workspace_bytes >= need && ((uintptr_t)workspace & 255) == 0, CHIMERE_ERR_WORKSPACE,
                     "linear_i8: workspace %zu bytes < %zu (or not 256-byte aligned)", workspace_bytes, need);
     const int64_t lda = pad_to(ncols, 16);

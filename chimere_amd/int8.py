@@ -24,33 +24,48 @@ from ._lib import BF16, F16, F32, MoeI8LayerC, check, lib
 FLOAT_TYPES = {torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16}
 
 
-def on_device(*tensors):
-    """The device that all tensors (Nones apart) lie on, as a guard for the launch."""
-    dev = tensors[0].device
-    if dev.type != "cuda":
-        raise ValueError(f"tensors on a ROCm device are wanted, not on {dev}")
-    for t in tensors:
-        if t is not None and t.device != dev:
-            raise ValueError(f"tensors on {dev} and on {t.device}")
-    return torch.cuda.device(dev)
+def device_of(first, *more):
+    """The index of the ROCm device that all tensors (Nones apart) lie on."""
+    dev = first.get_device()
+    if dev < 0:
+        raise ValueError(f"tensors on a ROCm device are wanted, not on {first.device}")
+    for t in more:
+        if t is not None and t.get_device() != dev:
+            raise ValueError(f"tensors on {first.device} and on {t.device}")
+    return dev
+
+
+def launch(dev, fn, *args):
+    """fn(*args, stream) with device dev's current torch stream, dev being the current device meanwhile."""
+    stream = torch._C._cuda_getCurrentRawStream(dev)    # torch.cuda.current_stream(dev).cuda_stream, 1.7 us less
+    if dev == torch.cuda.current_device():
+        fn(*args, stream)
+    else:
+        with torch.cuda.device(dev):
+            fn(*args, stream)
+    check()
 
 
 def float_type(t):
-    if t.dtype not in FLOAT_TYPES:
+    kind = FLOAT_TYPES.get(t.dtype)
+    if kind is None:
         raise ValueError(f"float32, float16 or bfloat16 is wanted, not {t.dtype}")
-    return FLOAT_TYPES[t.dtype]
+    return kind
 
 
 def rows_of(t, what, ncols=None):
     """(rows, columns, row stride) of a matrix whose rows' elements lie next to each other."""
-    if t.dim() != 2 or (t.stride(1) != 1 and t.shape[1] > 1):
-        raise ValueError(f"{what}: a matrix with contiguous rows is wanted, not {tuple(t.shape)} strides {t.stride()}")
-    if ncols is not None and t.shape[1] != ncols:
-        raise ValueError(f"{what}: {t.shape[1]} columns, {ncols} are wanted")
-    return t.shape[0], t.shape[1], t.stride(0) if t.shape[0] > 1 else max(t.stride(0), t.shape[1])
+    if t.dim() != 2:
+        raise ValueError(f"{what}: a matrix is wanted, not {tuple(t.shape)}")
+    (n, c), (ld, one) = t.shape, t.stride()
+    if one != 1 and c > 1:
+        raise ValueError(f"{what}: contiguous rows are wanted, not {tuple(t.shape)} with strides {t.stride()}")
+    if ncols is not None and c != ncols:
+        raise ValueError(f"{what}: {c} columns, {ncols} are wanted")
+    return n, c, ld if n > 1 else max(ld, c)
 
 
-def _vector(t, n, what, dtype=torch.float32):
+def vector(t, n, what, dtype=torch.float32):
     if t.dtype != dtype or t.numel() != n or not t.is_contiguous():
         raise ValueError(f"{what}: {n} contiguous {dtype} are wanted, not {tuple(t.shape)} {t.dtype}")
     return t.data_ptr()
@@ -60,19 +75,21 @@ def _int8(t, what, ncols=None):
     if t.dtype != torch.int8:
         raise ValueError(f"{what}: int8 is wanted, not {t.dtype}")
     n, c, ld = rows_of(t, what, ncols)
-    return n, c, ld if n > 1 else (max(ld, c) + 15) // 16 * 16
+    return n, c, ld if n > 1 else (ld + 15) // 16 * 16      # one row has no next one
 
 
 def _out(out, dtype, n, rows, dev):
+    """(out, its row stride), made where it is None."""
     if out is None:
-        return torch.empty(n, rows, dtype=dtype, device=dev)
-    if out.shape != (n, rows):
-        raise ValueError(f"out: {(n, rows)} is wanted, not {tuple(out.shape)}")
-    return out
+        return torch.empty(n, rows, dtype=dtype, device=dev), rows
+    on, oc, ld = rows_of(out, "out")
+    if on != n or oc != rows:
+        raise ValueError(f"out: {(n, rows)} is wanted, not {(on, oc)}")
+    return out, ld
 
 
-def stream_of(t):
-    return torch.cuda.current_stream(t.device).cuda_stream
+def _bias(bias, n):
+    return None if bias is None else vector(bias, n, "bias")
 
 
 def quantize_i8(x, q=None, scale=None):
@@ -86,10 +103,8 @@ def quantize_i8(x, q=None, scale=None):
     qn, _, ldq = _int8(q, "q", c)
     if qn != n:
         raise ValueError(f"q: {n} rows are wanted, not {qn}")
-    with on_device(x, q, scale):
-        lib().chimere_quantize_i8(float_type(x), x.data_ptr(), ld, q.data_ptr(), ldq, _vector(scale, n, "scale"), n, c,
-                                  stream_of(x))
-    check()
+    launch(device_of(x, q, scale), lib().chimere_quantize_i8, float_type(x), x.data_ptr(), ld, q.data_ptr(), ldq,
+           vector(scale, n, "scale"), n, c)
     return q, scale
 
 
@@ -98,14 +113,10 @@ def gemm_i8(a, a_scale, w, w_scale, bias=None, out=None, dtype=torch.float32):
     with their scales, out of type ``dtype`` unless given."""
     n, c, lda = _int8(a, "a")
     rows, _, ldw = _int8(w, "w", c)
-    out = _out(out, dtype, n, rows, a.device)
-    _, _, ldo = rows_of(out, "out")
-    with on_device(a, a_scale, w, w_scale, bias, out):
-        lib().chimere_gemm_i8(a.data_ptr(), lda, _vector(a_scale, n, "a_scale"), w.data_ptr(), ldw,
-                              _vector(w_scale, rows, "w_scale"),
-                              None if bias is None else _vector(bias, rows, "bias"), float_type(out), out.data_ptr(),
-                              ldo, n, rows, c, stream_of(a))
-    check()
+    out, ldo = _out(out, dtype, n, rows, a.device)
+    launch(device_of(a, a_scale, w, w_scale, bias, out), lib().chimere_gemm_i8, a.data_ptr(), lda,
+           vector(a_scale, n, "a_scale"), w.data_ptr(), ldw, vector(w_scale, rows, "w_scale"), _bias(bias, rows),
+           float_type(out), out.data_ptr(), ldo, n, rows, c)
     return out
 
 
@@ -114,15 +125,13 @@ def linear_i8(x, w, w_scale, bias=None, out=None, dtype=None):
     ``out`` says otherwise."""
     n, c, ld = rows_of(x, "x")
     rows, _, ldw = _int8(w, "w", c)
-    out = _out(out, dtype or x.dtype, n, rows, x.device)
-    _, _, ldo = rows_of(out, "out")
-    with on_device(x, w, w_scale, bias, out):
-        need = lib().chimere_linear_i8_workspace_size(n, c)
-        ws = torch.empty(need, dtype=torch.uint8, device=x.device)
-        lib().chimere_linear_i8(float_type(x), x.data_ptr(), ld, w.data_ptr(), ldw, _vector(w_scale, rows, "w_scale"),
-                                None if bias is None else _vector(bias, rows, "bias"), float_type(out), out.data_ptr(),
-                                ldo, n, rows, c, ws.data_ptr(), need, stream_of(x))
-    check()
+    out, ldo = _out(out, dtype or x.dtype, n, rows, x.device)
+    dev = device_of(x, w, w_scale, bias, out)
+    need = lib().chimere_linear_i8_workspace_size(n, c)
+    ws = torch.empty(need, dtype=torch.uint8, device=x.device) if need else None
+    launch(dev, lib().chimere_linear_i8, float_type(x), x.data_ptr(), ld, w.data_ptr(), ldw,
+           vector(w_scale, rows, "w_scale"), _bias(bias, rows), float_type(out), out.data_ptr(), ldo, n, rows, c,
+           ws.data_ptr() if need else None, need)
     return out
 
 
@@ -138,13 +147,13 @@ class Int8Experts:
         for name, t in (("gate", gate), ("up", up), ("down", down)):
             if t.dtype != torch.int8 or not t.is_contiguous():
                 raise ValueError(f"{name}: contiguous int8 is wanted")
-        on_device(gate, gate_scale, up, up_scale, down, down_scale)
-        self.device = gate.device
+        self.device = device_of(gate, gate_scale, up, up_scale, down, down_scale)
         self.tensors = [gate, gate_scale, up, up_scale, down, down_scale]
         self.c = MoeI8LayerC(self.H, self.F, self.E, gate.data_ptr(), up.data_ptr(), down.data_ptr(),
-                             _vector(gate_scale, self.E * self.F, "gate_scale"),
-                             _vector(up_scale, self.E * self.F, "up_scale"),
-                             _vector(down_scale, self.E * self.H, "down_scale"))
+                             vector(gate_scale, self.E * self.F, "gate_scale"),
+                             vector(up_scale, self.E * self.F, "up_scale"),
+                             vector(down_scale, self.E * self.H, "down_scale"))
+        self.ref = C.byref(self.c)
 
     @classmethod
     def from_float(cls, gate, up, down):
@@ -161,18 +170,17 @@ class Int8Experts:
         """x [T, H] float, ids [T, K] int32 and wts [T, K] float32 as ``gpu_topk_softmax`` gives them -> out [T, H],
         of x's type unless ``dtype`` or ``out`` says otherwise.  An id outside [0, E) adds nothing."""
         n, _, ld = rows_of(x, "x", self.H)
-        out = _out(out, dtype or x.dtype, n, self.H, x.device)
-        _, _, ldo = rows_of(out, "out")
-        if ids.dim() != 2 or ids.shape[0] != n:
-            raise ValueError(f"ids: [{n}, top_k] is wanted, not {tuple(ids.shape)}")
-        k = ids.shape[1]
-        with on_device(self.tensors[0], x, ids, wts, out):
-            need = lib().chimere_moe_i8_workspace_size(C.byref(self.c), k, n)
-            ws = torch.empty(need, dtype=torch.uint8, device=x.device)
-            lib().chimere_moe_i8(C.byref(self.c), float_type(x), x.data_ptr(), ld,
-                                 _vector(ids, n * k, "ids", torch.int32), _vector(wts, n * k, "wts"), k,
-                                 float_type(out), out.data_ptr(), ldo, n, ws.data_ptr(), need, stream_of(x))
-        check()
+        out, ldo = _out(out, dtype or x.dtype, n, self.H, x.device)
+        ni, k, _ = rows_of(ids, "ids")
+        if ni != n:
+            raise ValueError(f"ids: {n} rows are wanted, not {ni}")
+        if device_of(x, ids, wts, out) != self.device:
+            raise ValueError(f"x on {x.device}, the experts on cuda:{self.device}")
+        need = lib().chimere_moe_i8_workspace_size(self.ref, k, n)
+        ws = torch.empty(need, dtype=torch.uint8, device=x.device)
+        launch(self.device, lib().chimere_moe_i8, self.ref, float_type(x), x.data_ptr(), ld,
+               vector(ids, n * k, "ids", torch.int32), vector(wts, n * k, "wts"), k, float_type(out), out.data_ptr(),
+               ldo, n, ws.data_ptr(), need)
         return out
 
 

@@ -16,8 +16,8 @@ pass; nothing is recorded for autograd.  Stream, device and errors as in
 """
 import torch
 
-from ._lib import check, lib
-from .int8 import _vector, float_type, on_device, rows_of, stream_of
+from ._lib import lib
+from .int8 import device_of, float_type, launch, rows_of, vector
 
 
 def _mask(mask, n):
@@ -25,7 +25,7 @@ def _mask(mask, n):
         return None
     if mask.dtype not in (torch.bool, torch.uint8):
         raise ValueError(f"mask: bool or uint8 is wanted, not {mask.dtype}")
-    return _vector(mask, n, "mask", mask.dtype)
+    return vector(mask, n, "mask", mask.dtype)
 
 
 def balance_loss(logits, ids, mask=None):
@@ -33,20 +33,19 @@ def balance_loss(logits, ids, mask=None):
     (loss float32 [1], counts int32 [E], probs float32 [E], tokens int32 [1]):
     counts = pairs per expert, probs = mean of softmax(logits), loss = E sum counts / (tokens K) probs."""
     n, e, ld = rows_of(logits, "logits")
-    if ids.dim() != 2 or ids.shape[0] != n:
-        raise ValueError(f"ids: [{n}, top_k] is wanted, not {tuple(ids.shape)}")
-    dev = logits.device
-    loss, probs = torch.empty(1, device=dev), torch.empty(e, device=dev)
-    counts = torch.empty(e, dtype=torch.int32, device=dev)
-    tokens = torch.empty(1, dtype=torch.int32, device=dev)
-    with on_device(logits, ids, mask):
-        need = lib().chimere_balance_loss_workspace_size(e, n)
-        ws = torch.empty(need, dtype=torch.uint8, device=dev)
-        lib().chimere_balance_loss(float_type(logits), logits.data_ptr(), ld,
-                                   _vector(ids, ids.numel(), "ids", torch.int32), ids.shape[1], _mask(mask, n),
-                                   loss.data_ptr(), probs.data_ptr(), counts.data_ptr(), tokens.data_ptr(), e, n,
-                                   ws.data_ptr(), need, stream_of(logits))
-    check()
+    ni, k, _ = rows_of(ids, "ids")
+    if ni != n:
+        raise ValueError(f"ids: {n} rows are wanted, not {ni}")
+    device, dev = logits.device, device_of(logits, ids, mask)
+    loss = torch.empty(1, dtype=torch.float32, device=device)
+    probs = torch.empty(e, dtype=torch.float32, device=device)
+    counts = torch.empty(e, dtype=torch.int32, device=device)
+    tokens = torch.empty(1, dtype=torch.int32, device=device)
+    need = lib().chimere_balance_loss_workspace_size(e, n)
+    ws = torch.empty(need, dtype=torch.uint8, device=device) if need else None
+    launch(dev, lib().chimere_balance_loss, float_type(logits), logits.data_ptr(), ld,
+           vector(ids, n * k, "ids", torch.int32), k, _mask(mask, n), loss.data_ptr(), probs.data_ptr(),
+           counts.data_ptr(), tokens.data_ptr(), e, n, ws.data_ptr() if need else None, need)
     return loss, counts, probs, tokens
 
 
@@ -55,15 +54,12 @@ def balance_loss_grad(logits, counts, tokens, grad_loss, top_k, mask=None, out=N
     n, e, ld = rows_of(logits, "logits")
     if out is None:
         out = torch.empty(n, e, dtype=logits.dtype, device=logits.device)
-    if out.shape != logits.shape or out.dtype != logits.dtype:
-        raise ValueError(f"out: {tuple(logits.shape)} {logits.dtype} is wanted, not {tuple(out.shape)} {out.dtype}")
-    _, _, ldo = rows_of(out, "out")
-    with on_device(logits, counts, tokens, grad_loss, mask, out):
-        lib().chimere_balance_loss_grad(float_type(logits), logits.data_ptr(), ld, _mask(mask, n),
-                                        _vector(counts, e, "counts", torch.int32),
-                                        _vector(tokens, 1, "tokens", torch.int32), _vector(grad_loss, 1, "grad_loss"),
-                                        top_k, out.data_ptr(), ldo, e, n, stream_of(logits))
-    check()
+    on, oe, ldo = rows_of(out, "out")
+    if on != n or oe != e or out.dtype != logits.dtype:
+        raise ValueError(f"out: {(n, e)} {logits.dtype} is wanted, not {(on, oe)} {out.dtype}")
+    launch(device_of(logits, counts, tokens, grad_loss, mask, out), lib().chimere_balance_loss_grad, float_type(logits),
+           logits.data_ptr(), ld, _mask(mask, n), vector(counts, e, "counts", torch.int32),
+           vector(tokens, 1, "tokens", torch.int32), vector(grad_loss, 1, "grad_loss"), top_k, out.data_ptr(), ldo, e, n)
     return out
 
 

@@ -307,8 +307,8 @@ void chimere_gemm_i8(const int8_t *a, int64_t a_stride, const float *a_scale, co
                      void *out, int64_t out_stride, int ntok, int nrows, int ncols,
                      hipStream_t stream);
 /* The same for float tokens, quantized as above within the call.  Workspace:
- * chimere_linear_i8_workspace_size(>= ntok, ncols) bytes, 256-byte aligned,
- * needs no initialisation. */
+ * chimere_linear_i8_workspace_size(>= ntok, ncols) bytes (0 where the call
+ * needs none: NULL is taken), 256-byte aligned, needs no initialisation. */
 size_t chimere_linear_i8_workspace_size(int max_ntok, int ncols);
 void chimere_linear_i8(int type, const void *x, int64_t x_stride, const int8_t *w, int64_t w_stride,
                        const float *w_scale, const float *bias, int out_type, void *out,
@@ -348,7 +348,9 @@ void chimere_moe_i8(const chimere_moe_i8_layer *layer, int type, const void *x, 
  * all 0 where N is 0.  A row of logits that are all -inf has probabilities
  * of 0; rows that the mask leaves out are not read.  logits [ntok][E] with
  * logits_stride elements between rows, F32 / F16 / BF16; ids [ntok][top_k];
- * E <= 1024.  Sums have a fixed order: results repeat bit for bit. */
+ * E <= 1024.  Sums have a fixed order: results repeat bit for bit.
+ * Workspace: chimere_balance_loss_workspace_size(E, >= ntok) bytes (0 where
+ * the call needs none: NULL is taken), 256-byte aligned, not initialised. */
 size_t chimere_balance_loss_workspace_size(int n_experts, int max_ntok);
 void chimere_balance_loss(int type, const void *logits, int64_t logits_stride, const int *ids,
                           int top_k, const uint8_t *mask, float *loss, float *probs, int *counts,
