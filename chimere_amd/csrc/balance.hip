@@ -115,16 +115,11 @@ __global__ __launch_bounds__(BAL_THREADS<NV>) void k_balance_sums(Balance b, con
     __syncthreads();
     float sum[4 * NV] = {};
     int rows = 0;
-    // the next round's row is loaded while this one's is summed up
-    BalRow<NV> row, next;
-    auto fetch = [&](int t, BalRow<NV>& r) {
-        const bool on = t < b.T && (!b.mask || b.mask[t]);
-        if (on) r.load(logits + t * b.ld, b.E, b.wide);
-        return on;
-    };
-    bool on = fetch(blockIdx.x * ROWS + (tid >> 4), row);
     for (int t0 = blockIdx.x * ROWS; t0 < b.T; t0 += b.groups * ROWS) {
-        const bool more = fetch(t0 + b.groups * ROWS + (tid >> 4), next);
+        const int t = t0 + (tid >> 4);
+        const bool on = t < b.T && (!b.mask || b.mask[t]);
+        BalRow<NV> row;
+        if (on) row.load(logits + t * b.ld, b.E, b.wide);
         const int pairs = min(ROWS, b.T - t0) * b.K;
         const int* ids = b.ids + (int64_t)t0 * b.K;
         for (int p = tid; p < pairs; p += THREADS) {
@@ -137,8 +132,6 @@ __global__ __launch_bounds__(BAL_THREADS<NV>) void k_balance_sums(Balance b, con
             for (int i = 0; i < 4 * NV; i++) sum[i] += row.v[i];
             rows += (tid & 15) == 0;
         }
-        row = next;
-        on = more;
     }
 #pragma unroll
     for (int i = 0; i < 4 * NV; i++) {
@@ -207,7 +200,7 @@ __global__ __launch_bounds__(256) void k_balance_loss(Balance b) {
     }
     ps[tid] = s;
     pc[tid] = c;
-    if (tid < b.groups) atomicAdd(&n, b.pn[tid]);
+    for (int g = tid; g < b.groups; g += 256) atomicAdd(&n, b.pn[g]);
     __syncthreads();
     float l = 0.0f;
     if (tid < BAL_JOIN && e < b.E) {
