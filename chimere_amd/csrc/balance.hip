@@ -358,7 +358,7 @@ size_t chimere_balance_loss_workspace_size(int n_experts, int max_ntok) {
 static bool balance_args(const char* what, int type, const void* logits, int64_t ld, int E, int K, int T) {
     if (!float_type(type))
         set_error(CHIMERE_ERR_ARG, "%s: unsupported type %d", what, type);
-    else if (E < 1 || E > MAX_E || K < 1 || T < 0)
+    else if (E < 1 || E > MAX_E || K < 1 || K > MAX_E || T < 0 || (int64_t)T * K >= (1 << 30))
         set_error(CHIMERE_ERR_ARG, "%s: n_experts=%d top_k=%d ntok=%d out of range", what, E, K, T);
     else if (T > 0 && (!logits || ld < 0))
         set_error(CHIMERE_ERR_ARG, "%s: null pointer or bad stride", what);

@@ -3,53 +3,9 @@
 // token at a time through the block-quantized GEMV.
 #include "api_internal.h"
 #include "int8_gemm.h"
+#include "int8_quant.h"
 
 namespace chimere {
-
-// the integer of x in a row of scale d
-__device__ __forceinline__ int i8_quant(float x, float d) {
-    return d > 0.0f && d < __builtin_huge_valf() ? (int)__builtin_rintf(x / d) : 0;
-}
-
-// N integers packed into bytes
-template <int N>
-__device__ __forceinline__ void i8_pack(const float (&x)[N], float d, uint32_t (&q)[N / 4]) {
-#pragma unroll
-    for (int k = 0; k < N; k += 4)
-        q[k / 4] = (uint32_t)(uint8_t)i8_quant(x[k], d) | (uint32_t)(uint8_t)i8_quant(x[k + 1], d) << 8 |
-                   (uint32_t)(uint8_t)i8_quant(x[k + 2], d) << 16 | (uint32_t)(uint8_t)i8_quant(x[k + 3], d) << 24;
-}
-
-// Elements c .. c + V - 1 of a row as f32, one 16-byte load where `wide`; those
-// from ncols on are 0
-template <int V, typename T>
-__device__ __forceinline__ void i8_load(const T* row, int c, int ncols, bool wide, float (&x)[V]) {
-    typedef T vec __attribute__((ext_vector_type(V)));
-    if (wide && c + V <= ncols) {
-        const vec v = *(const vec*)(row + c);
-#pragma unroll
-        for (int k = 0; k < V; k++) x[k] = (float)v[k];
-    } else {
-#pragma unroll
-        for (int k = 0; k < V; k++) x[k] = c + k < ncols ? load_f(row + c + k) : 0.0f;
-    }
-}
-
-// max |x| as bits: a NaN is larger than an infinity, and both than any number
-template <int V>
-__device__ __forceinline__ uint32_t i8_amax(uint32_t m, const float (&x)[V]) {
-#pragma unroll
-    for (int k = 0; k < V; k++) m = max(m, __builtin_bit_cast(uint32_t, x[k]) & 0x7FFFFFFFu);
-    return m;
-}
-__device__ __forceinline__ uint32_t wave_amax(uint32_t m) {
-    m = max(m, (uint32_t)xlane<32>((int)m));
-    m = max(m, (uint32_t)xlane<16>((int)m));
-    m = max(m, (uint32_t)xlane<8>((int)m));
-    m = max(m, (uint32_t)xlane<4>((int)m));
-    m = max(m, (uint32_t)xlane<2>((int)m));
-    return max(m, (uint32_t)xlane<1>((int)m));
-}
 
 // Row quantizer: scale = max |x| / 127, q = x / scale rounded to the nearest
 // integer, ties to even (IEEE divisions).  A row that holds an infinity or a
@@ -73,12 +29,12 @@ __global__ __launch_bounds__(256) void k_i8_quantize(const T* __restrict__ x, in
     uint32_t m = 0;
 #pragma unroll
     for (int i = 0; i < KEEP; i++) {
-        i8_load<V>(row, c0 + i * STEP, ncols, wide, v[i]);
+        i8_load(row, c0 + i * STEP, ncols, wide, v[i]);
         m = i8_amax(m, v[i]);
     }
     for (int c = c0 + KEEP * STEP; c < ncols; c += STEP) {
         float u[V];
-        i8_load<V>(row, c, ncols, wide, u);
+        i8_load(row, c, ncols, wide, u);
         m = i8_amax(m, u);
     }
     m = wave_amax(m);
@@ -110,7 +66,7 @@ __global__ __launch_bounds__(256) void k_i8_quantize(const T* __restrict__ x, in
         if (c0 + i * STEP < ncols) put(c0 + i * STEP, v[i]);
     for (int c = c0 + KEEP * STEP; c < ncols; c += STEP) {
         float u[V];
-        i8_load<V>(row, c, ncols, wide, u);
+        i8_load(row, c, ncols, wide, u);
         put(c, u);
     }
 }
@@ -220,44 +176,10 @@ __global__ __launch_bounds__(64 * FEW_WAVES) void k_i8_few(I8Gemm g) {
     float* as = (float*)lds;   // [16 MB]
     uint8_t* aq = lds + 16 * MB * 4;
     if constexpr (QUANT) {
-        // pieces of V elements, row by row, over all threads; each row's maximum
-        // through an LDS atomic (any order gives the same)
-        constexpr int V = 16 / sizeof(X), KEEP = FEW_KEEP / V;
-        uint32_t* bits = (uint32_t*)lds;
-        const bool wide = (((uintptr_t)g.x | (uintptr_t)(g.ldx * sizeof(X))) & 15) == 0;
-        const int per = (S * I8_BK) / V, n = M * per;
-        if (tid < 16 * MB) bits[tid] = 0;
-        __syncthreads();
-        float v[KEEP][V];
-#pragma unroll
-        for (int i = 0; i < KEEP; i++) {
-            const int at = tid + i * 64 * FEW_WAVES, m = min(at / per, M - 1);
-            uint32_t top = 0;
-            if (at < n) {
-                i8_load<V>((const X*)g.x + m * g.ldx, (at - m * per) * V, g.C, wide, v[i]);
-                top = i8_amax(0u, v[i]);
-            }
-            if (M == 1) {
-                top = wave_amax(top);
-                if (lane == 0) atomicMax(&bits[0], top);
-            } else if (at < n) {
-                atomicMax(&bits[m], top);
-            }
-        }
-        __syncthreads();
-        if (tid < M) as[tid] = __builtin_bit_cast(float, bits[tid]) / 127.0f;
-        __syncthreads();
-#pragma unroll
-        for (int i = 0; i < KEEP; i++) {
-            const int at = tid + i * 64 * FEW_WAVES, m = min(at / per, M - 1);
-            if (at < n) {
-                uint32_t p[V / 4];
-                i8_pack<V>(v[i], as[m], p);
-#pragma unroll
-                for (int k = 0; k < V / 4; k++) *(uint32_t*)(aq + m * lda + (at - m * per) * V + 4 * k) = p[k];
-            }
-        }
-        __syncthreads();
+        i8_rows_to_lds<64 * FEW_WAVES, FEW_KEEP>(M, S * I8_BK, lda, as, aq, [&](int m, int c, auto& v) {
+            const bool wide = (((uintptr_t)g.x | (uintptr_t)(g.ldx * sizeof(X))) & 15) == 0;
+            i8_load((const X*)g.x + (m0 + m) * g.ldx, c, g.C, wide, v);
+        }, std::integral_constant<int, 16 / sizeof(X)>{});
     } else {
         if (tid < 16 * MB) as[tid] = g.as[m0 + min(tid, M - 1)];
     }

@@ -59,7 +59,7 @@ struct I8Tile {
 
     // aoff[p] / woff[p]: this lane's row of piece p, as a byte offset from a / w
     // (row (wave * P + p) * 8 + lane / 8 of the tile).  Weight rows come in
-    // blocks of 32 in turn from w and from w2 (the same matrix, or two).
+    // blocks of 16 in turn from w and from w2 (the same matrix, or two).
     static __device__ __forceinline__ void run(const int8_t* a, const int8_t* w, const int8_t* w2,
                                                const uint32_t (&aoff)[PM], const uint32_t (&woff)[PN], int C,
                                                uint8_t* lds, v16i (&acc)[MT][NT]) {
@@ -77,7 +77,7 @@ struct I8Tile {
                 copy16_lds_base(a, aoff[p] + ((wave * PM + p) & 1 ? k1 : k0), at + (wave * PM + p) * 1024);
 #pragma unroll
             for (int p = 0; p < PN; p++)
-                copy16_lds_base((wave * PN + p) & 4 ? w2 : w, woff[p] + ((wave * PN + p) & 1 ? k1 : k0),
+                copy16_lds_base((wave * PN + p) & 2 ? w2 : w, woff[p] + ((wave * PN + p) & 1 ? k1 : k0),
                                 at + BM * I8_BK + (wave * PN + p) * 1024);
         };
 #pragma unroll
@@ -136,7 +136,7 @@ struct I8Tile {
     // value that thread `row` handed in (a scale that is loaded once, ahead of
     // the loop: loaded where it is used, each load's latency was paid 16 times
     // per tile, 17 us of a 256 x 256 tile).  PAIR (w and w2): columns are
-    // counted over w's blocks 0, 2, .. and emit gets the sums of both,
+    // those of w's rows and emit gets the sums of both,
     // emit(row, sums, sums2, of_row).
     static constexpr int PAD = NT * 32 + 8;   // dwords per row: the two half-waves write 4 rows apart, 32 banks apart
     static_assert(NW * 16 * PAD * 4 + BM * 8 <= LDS && 64 * NW >= BM, "the layout fits the stages, a thread per row");
@@ -169,11 +169,11 @@ struct I8Tile {
             for (int q = 0; q < 16 / ROWS; q++) {
                 const int r = q * ROWS + lane / LANES, c = lane % LANES * VEC, m = wm * MT * 32 + h * 16 + r;
                 int x[VEC], y[VEC];
-                const int* p = at + r * PAD + (PAIR ? (c >> 5) * 64 + (c & 31) : c);
+                const int* p = at + r * PAD + (PAIR ? (c >> 4) * 32 + (c & 15) : c);
 #pragma unroll
                 for (int k = 0; k < VEC; k += 4) {
                     *(v4i*)(x + k) = *(const v4i*)(p + k);
-                    if constexpr (PAIR) *(v4i*)(y + k) = *(const v4i*)(p + 32 + k);
+                    if constexpr (PAIR) *(v4i*)(y + k) = *(const v4i*)(p + 16 + k);
                 }
                 if constexpr (PAIR) emit(m, x, y, each[m]);
                 else emit(m, x, each[m]);

@@ -343,4 +343,33 @@ __device__ __forceinline__ void quantize_blocks(int nblk, Src src, Emit emit) {
     }
 }
 
+// exclusive prefix sum of one int per thread over a 1024-thread group
+__device__ __forceinline__ int excl_scan1024(int v, int* wsum, int* total) {
+    const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
+    int x = v;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+        const int y = __shfl_up(x, d);
+        if (lane >= d) x += y;
+    }
+    if (lane == 63) wsum[w] = x;
+    __syncthreads();
+    if (w == 0) {
+        const int t = lane < 16 ? wsum[lane] : 0;
+        int sc = t;
+#pragma unroll
+        for (int d = 1; d < 16; d <<= 1) {
+            const int y = __shfl_up(sc, d);
+            if (lane >= d) sc += y;
+        }
+        __syncthreads();   // pairs with the barrier below for the other waves
+        if (lane < 16) wsum[lane] = sc - t;
+        if (lane == 15) *total = sc;
+    } else {
+        __syncthreads();
+    }
+    __syncthreads();
+    return x - v + wsum[w];
+}
+
 }  // namespace chimere

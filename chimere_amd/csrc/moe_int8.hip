@@ -3,11 +3,17 @@
 // The counterpart over block-quantized weights is chimere_moe_prefill
 // (cs/src/qwen35_model/moe_ffn.rs:1081-1768 per token).
 //
-// Launches: rows of x to 8 bits; the pairs of each expert together, with the
-// list of tiles; gate and up product with h = silu(g) u; rows of h to 8 bits;
-// down product; each token's weighted sum.
+// Bound by the selected experts' weights: each byte of them is read from
+// memory once.  A few pairs of (token, expert), two launches: gate and up of
+// each pair (every work-group quantizes its token), then per token h to 8 bits,
+// down and the weighted sum.  More: rows of x to 8 bits; the pairs of each
+// expert together, with the list of tiles; gate and up product with
+// h = silu(g) u; rows of h to 8 bits; down product; each token's weighted sum.
+#include <type_traits>
+
 #include "api_internal.h"
 #include "int8_gemm.h"
+#include "int8_quant.h"
 #include "moe_common.h"
 
 namespace chimere {
@@ -18,61 +24,194 @@ struct MoeI8 {
     const float *gate_s, *up_s, *down_s;
     const int* ids;
     const float* wts;
-    const int8_t* xq;      // [T][H]
-    const float* xs;       // [T]
-    int *order, *total;    // pairs by expert; {pairs, tiles}
+    const void* x;
+    int64_t ldx;
+    int8_t* xq;            // [T][H]
+    float* xs;             // [T]
+    int *order, *pos;      // sorted position -> pair, pair -> sorted position (-1: left out)
+    int* total;            // {pairs, tiles}
     int4* tiles;           // {expert, first sorted pair, pairs, 0}
-    float* h;              // [pairs][F], in sorted order
+    float* h;              // [pairs][F], in sorted order (few pairs: by pair)
     int8_t* hq;
     float* hs;
-    float* y;              // [T * K][H], by pair
+    void* y;               // [pairs][H], in sorted order: f32, or f16 of sum * 2^-shift
+    int shift;
     void* out;
     int64_t ldo;
     int tile_pairs;
 };
 
+// ------------------------------------------------------------ few pairs
+
+constexpr int FP_WAVES = 8, FP_KEEP = 16, FP_AHEAD = 4;   // FP_AHEAD: a wave's pieces of work whose weights are loaded ahead
+
+// Grid (F / 16, pairs): 16 columns of F of one pair, gate and up.  Steps of 128
+// columns of H dealt to the eight waves; the one token is row 0 of the matrix
+// instruction (the other rows repeat it: the weights' bytes are what counts),
+// sums joined in LDS.
+template <typename X>
+__global__ __launch_bounds__(64 * FP_WAVES) void k_i8_pair_gate_up(MoeI8 a) {
+    extern __shared__ __align__(16) uint8_t lds[];   // scale, integers of the token
+    __shared__ int part[FP_WAVES][2][16];
+    const int p = blockIdx.y, e = a.ids[p], t = p / a.K, f0 = blockIdx.x * 16;
+    if ((unsigned)e >= (unsigned)a.E) return;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int S = (a.H + I8_BK - 1) / I8_BK, last = a.H / 16 - 1, r = lane & 15, pc = (lane >> 4) * 2;
+    const int64_t row = ((int64_t)e * a.F + f0 + r) * a.H;   // F is a multiple of 16
+    v4i w[2][2];
+    auto load_w = [&](int s) {
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+            const int at = min(8 * s + pc + h, last) * 16;
+            w[0][h] = *(const v4i*)(a.gate + row + at);
+            w[1][h] = *(const v4i*)(a.up + row + at);
+        }
+    };
+    if (wave < S) load_w(wave);
+    const float sg = tid < 16 ? a.gate_s[(int64_t)e * a.F + f0 + tid] : 0.0f;
+    const float su = tid < 16 ? a.up_s[(int64_t)e * a.F + f0 + tid] : 0.0f;
+    float* xs = (float*)lds;
+    uint8_t* xq = lds + 16;
+    const X* x = (const X*)a.x + t * a.ldx;
+    const bool wide = ((uintptr_t)x & 15) == 0;
+    i8_rows_to_lds<64 * FP_WAVES, FP_KEEP>(1, S * I8_BK, 0, xs, xq,
+                                           [&](int, int c, auto& v) { i8_load(x, c, a.H, wide, v); },
+                                           std::integral_constant<int, 16 / sizeof(X)>{});
+    v4i g = {}, u = {};
+    for (int s = wave; s < S; s += FP_WAVES) {
+        v4i now[2][2];
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+            now[0][h] = w[0][h];
+            now[1][h] = w[1][h];
+        }
+        if (s + FP_WAVES < S) load_w(s + FP_WAVES);
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+            const v4i f = *(const v4i*)(xq + (8 * s + pc + h) * 16);   // 0 behind H
+            g = __builtin_amdgcn_mfma_i32_16x16x64_i8(f, now[0][h], g, 0, 0, 0);
+            u = __builtin_amdgcn_mfma_i32_16x16x64_i8(f, now[1][h], u, 0, 0, 0);
+        }
+    }
+    if (lane < 16) {   // row 0, column lane
+        part[wave][0][lane] = g[0];
+        part[wave][1][lane] = u[0];
+    }
+    __syncthreads();
+    if (tid < 16) {
+        int gs = 0, us = 0;
+#pragma unroll
+        for (int i = 0; i < FP_WAVES; i++) {
+            gs += part[i][0][tid];
+            us += part[i][1][tid];
+        }
+        a.h[(int64_t)p * a.F + f0 + tid] = det_silu((float)gs * *xs * sg) * ((float)us * *xs * su);
+    }
+}
+
+// Grid (H / 16, T): 16 columns of H of one token.  The token's rows of h to 8
+// bits in LDS; the (k, step of 128 columns of F) pieces dealt to the eight
+// waves, whose sums meet in LDS integers; the weighted sum in ascending k.
+template <typename T>
+__global__ __launch_bounds__(64 * FP_WAVES) void k_i8_pair_down(MoeI8 a) {
+    extern __shared__ __align__(16) uint8_t lds[];   // integers of h
+    __shared__ float hs[MAX_K];
+    __shared__ int sum[MAX_K][16], es[MAX_K];
+    const int t = blockIdx.y, n0 = blockIdx.x * 16;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int S = (a.F + I8_BK - 1) / I8_BK, last = a.F / 16 - 1, r = lane & 15, pc = (lane >> 4) * 2;
+    const int* ids = a.ids + (int64_t)t * a.K;
+    v4i w[FP_AHEAD][2];
+    auto load_w = [&](int u, v4i(&to)[2]) {
+        const int k = u / S, s = u - k * S, e = ids[k];
+        const int8_t* row = a.down + ((int64_t)((unsigned)e < (unsigned)a.E ? e : 0) * a.H + n0 + r) * a.F;
+#pragma unroll
+        for (int h = 0; h < 2; h++) to[h] = *(const v4i*)(row + min(8 * s + pc + h, last) * 16);
+    };
+#pragma unroll
+    for (int i = 0; i < FP_AHEAD; i++)
+        if (wave + i * FP_WAVES < a.K * S) load_w(wave + i * FP_WAVES, w[i]);
+    if (tid < MAX_K * 16) (&sum[0][0])[tid] = 0;
+    if (tid < a.K) es[tid] = (unsigned)ids[tid] < (unsigned)a.E ? ids[tid] : -1;
+    __syncthreads();
+    const int lda = S * I8_BK;
+    i8_rows_to_lds<64 * FP_WAVES, FP_KEEP>(a.K, S * I8_BK, lda, hs, lds,
+                                           [&](int k, int c, auto& v) {
+                                               if (es[k] >= 0) {
+                                                   i8_load(a.h + ((int64_t)t * a.K + k) * a.F, c, a.F, true, v);
+                                               } else {
+#pragma unroll
+                                                   for (int i = 0; i < 4; i++) v[i] = 0.0f;
+                                               }
+                                           },
+                                           std::integral_constant<int, 4>{});
+    auto piece = [&](int u, const v4i(&now)[2]) {
+        const int k = u / S, s = u - k * S;
+        v4i acc = {};
+#pragma unroll
+        for (int h = 0; h < 2; h++)
+            acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(*(const v4i*)(lds + k * lda + (8 * s + pc + h) * 16), now[h],
+                                                        acc, 0, 0, 0);
+        if (lane < 16) atomicAdd(&sum[k][lane], acc[0]);   // integers: any order
+    };
+#pragma unroll
+    for (int i = 0; i < FP_AHEAD; i++)
+        if (wave + i * FP_WAVES < a.K * S) piece(wave + i * FP_WAVES, w[i]);
+    for (int u = wave + FP_AHEAD * FP_WAVES; u < a.K * S; u += FP_WAVES) {
+        load_w(u, w[0]);
+        piece(u, w[0]);
+    }
+    __syncthreads();
+    if (tid < 16) {
+        float acc = 0.0f;
+        for (int k = 0; k < a.K; k++)
+            if (es[k] >= 0)
+                acc = __builtin_fmaf(a.wts[(int64_t)t * a.K + k],
+                                     (float)sum[k][tid] * hs[k] * a.down_s[(int64_t)es[k] * a.H + n0 + tid], acc);
+        store_f((T*)a.out + t * a.ldo + n0 + tid, acc);
+    }
+}
+
+// ------------------------------------------------------------ many pairs
+
 // Counting sort of the pairs by expert; a pair whose id is no expert is left
 // out.  Pairs of one expert come in any order: each pair's row is computed on
 // its own.
 __global__ __launch_bounds__(1024) void k_i8_plan(MoeI8 a) {
-    __shared__ int cnt[MAX_E], first[MAX_E], tile0[MAX_E];
+    __shared__ int first[MAX_E], wsum[16], tot[2];
     const int tid = threadIdx.x, P = a.T * a.K, TP = a.tile_pairs;
-    cnt[tid] = 0;
+    first[tid] = 0;
     __syncthreads();
+#pragma unroll 4
     for (int p = tid; p < P; p += 1024) {
         const int e = a.ids[p];
-        if ((unsigned)e < (unsigned)a.E) atomicAdd(&cnt[e], 1);
+        if ((unsigned)e < (unsigned)a.E) atomicAdd(&first[e], 1);
     }
     __syncthreads();
-    if (tid == 0) {
-        int n = 0, t = 0;
-        for (int e = 0; e < a.E; e++) {
-            first[e] = n;
-            tile0[e] = t;
-            n += cnt[e];
-            t += (cnt[e] + TP - 1) / TP;
+    const int c = first[tid], nt = (c + TP - 1) / TP;
+    const int at = excl_scan1024(c, wsum, &tot[0]);
+    __syncthreads();
+    const int tile = excl_scan1024(nt, wsum, &tot[1]);
+    first[tid] = at;
+    for (int s = 0; s < nt; s++) a.tiles[tile + s] = make_int4(tid, at + s * TP, min(TP, c - s * TP), 0);
+    __syncthreads();
+    if (tid < 2) a.total[tid] = tot[tid];
+#pragma unroll 4
+    for (int p = tid; p < P; p += 1024) {
+        const int e = a.ids[p];
+        int q = -1;
+        if ((unsigned)e < (unsigned)a.E) {
+            q = atomicAdd(&first[e], 1);
+            a.order[q] = p;
         }
-        a.total[0] = n;
-        a.total[1] = t;
-    }
-    __syncthreads();
-    if (tid < a.E)
-        for (int s = 0; s * TP < cnt[tid]; s++)
-            a.tiles[tile0[tid] + s] = make_int4(tid, first[tid] + s * TP, min(TP, cnt[tid] - s * TP), 0);
-    __syncthreads();
-    for (int p = tid; p < P; p += 1024) {
-        const int e = a.ids[p];
-        if ((unsigned)e < (unsigned)a.E) a.order[atomicAdd(&first[e], 1)] = p;
+        a.pos[p] = q;
     }
 }
 
-typedef I8Tile<2, 2, 2, 2> GuTile;    // 128 pairs x 64 columns of F, gate and up
-typedef I8Tile<2, 2, 2, 2> DnTile;    // 128 pairs x 128 columns of H
-
-// Gate and up: the weight rows of a tile alternate in blocks of 32 between
+// Gate and up of a tile: its weight rows alternate in blocks of 16 between
 // gate and up, so g and u of the same (pair, column) meet in a lane.
-__global__ __launch_bounds__(64 * GuTile::NW) void k_i8_gate_up(MoeI8 a) {
-    typedef GuTile Tile;
+template <typename Tile, int WAVES_PER_SIMD>
+__global__ __launch_bounds__(64 * Tile::NW, WAVES_PER_SIMD) void k_i8_gate_up(MoeI8 a) {
     __shared__ __align__(16) uint8_t lds[Tile::LDS];
     const int fb = (a.F + Tile::BN / 2 - 1) / (Tile::BN / 2), tile = blockIdx.x / fb;
     if (tile >= a.total[1]) return;
@@ -87,19 +226,19 @@ __global__ __launch_bounds__(64 * GuTile::NW) void k_i8_gate_up(MoeI8 a) {
 #pragma unroll
     for (int p = 0; p < Tile::PN; p++) {
         const int r = (wave * Tile::PN + p) * 8 + (lane >> 3);
-        woff[p] = (uint32_t)(min(f0 + (r >> 6) * 32 + (r & 31), a.F - 1)) * (uint32_t)a.H;
+        woff[p] = (uint32_t)min(f0 + (r >> 5) * 16 + (r & 15), a.F - 1) * (uint32_t)a.H;
     }
     const int64_t e = t.x;
     const float xs = threadIdx.x < Tile::BM ? a.xs[a.order[t.y + min((int)threadIdx.x, t.z - 1)] / a.K] : 0.0f;
     v16i acc[Tile::MTILES][Tile::NTILES];
     Tile::run(a.xq, a.gate + e * a.F * a.H, a.up + e * a.F * a.H, aoff, woff, a.H, lds, acc);
     constexpr int VEC = 4;
-    const int f = f0 + Tile::first_col<VEC, true>();
+    const int f = f0 + Tile::template first_col<VEC, true>();
     const bool in = f < a.F;   // F is a multiple of 16: all four columns or none
     const float4 sg = in ? *(const float4*)(a.gate_s + e * a.F + f) : float4{};
     const float4 su = in ? *(const float4*)(a.up_s + e * a.F + f) : float4{};
-    Tile::rows<VEC, true>(lds, acc, make_float2(xs, 0.0f),
-                          [&](int r, const int(&g)[VEC], const int(&u)[VEC], float2 of_row) {
+    Tile::template rows<VEC, true>(lds, acc, make_float2(xs, 0.0f),
+                                   [&](int r, const int(&g)[VEC], const int(&u)[VEC], float2 of_row) {
         if (r >= t.z || !in) return;
         const float s = of_row.x;
         float4 h;
@@ -111,8 +250,13 @@ __global__ __launch_bounds__(64 * GuTile::NW) void k_i8_gate_up(MoeI8 a) {
     });
 }
 
-__global__ __launch_bounds__(64 * DnTile::NW) void k_i8_down(MoeI8 a) {
-    typedef DnTile Tile;
+// Down of a tile.  Y = float: the scaled products.  Y = _Float16 (16-bit
+// outputs): the integer sums times 2^-shift, so that none exceeds f16's range
+// and each is off by 2^-11 of itself at most, whatever the scales, which the
+// weighted sum applies (16-bit rows halve what 32768 pairs of 2048 columns
+// write and read again, 268 MB each way).
+template <typename Tile, int WAVES_PER_SIMD, typename Y>
+__global__ __launch_bounds__(64 * Tile::NW, WAVES_PER_SIMD) void k_i8_down(MoeI8 a) {
     __shared__ __align__(16) uint8_t lds[Tile::LDS];
     const int hb = (a.H + Tile::BN - 1) / Tile::BN, tile = blockIdx.x / hb;
     if (tile >= a.total[1]) return;
@@ -126,58 +270,157 @@ __global__ __launch_bounds__(64 * DnTile::NW) void k_i8_down(MoeI8 a) {
     for (int p = 0; p < Tile::PN; p++)
         woff[p] = (uint32_t)min(n0 + (wave * Tile::PN + p) * 8 + (lane >> 3), a.H - 1) * (uint32_t)a.F;
     const int64_t e = t.x;
-    const int row = t.y + min((int)threadIdx.x, t.z - 1);
-    const float2 mine = threadIdx.x < Tile::BM ? make_float2(a.hs[row], __builtin_bit_cast(float, a.order[row]))
-                                               : float2{};
+    const float hs = threadIdx.x < Tile::BM ? a.hs[t.y + min((int)threadIdx.x, t.z - 1)] : 0.0f;
     v16i acc[Tile::MTILES][Tile::NTILES];
     const int8_t* w = a.down + e * a.H * a.F;
     Tile::run(a.hq + (int64_t)t.y * a.F, w, w, aoff, woff, a.F, lds, acc);
-    constexpr int VEC = 4;
-    const int n = n0 + Tile::first_col<VEC>();
-    const bool in = n < a.H;   // H is a multiple of 16: all four columns or none
-    const float4 sd = in ? *(const float4*)(a.down_s + e * a.H + n) : float4{};
-    Tile::rows<VEC>(lds, acc, mine, [&](int r, const int(&x)[VEC], float2 of_row) {
+    constexpr int VEC = 16 / sizeof(Y);
+    const int n = n0 + Tile::template first_col<VEC>();
+    const bool in = n < a.H;   // H is a multiple of 16: all columns or none
+    float sd[VEC];
+#pragma unroll
+    for (int k = 0; k < VEC; k++) sd[k] = sizeof(Y) == 4 && in ? a.down_s[e * a.H + n + k] : 0.0f;
+    const float unit = __builtin_ldexpf(1.0f, -a.shift);
+    Tile::template rows<VEC>(lds, acc, make_float2(hs, 0.0f), [&](int r, const int(&x)[VEC], float2 of_row) {
         if (r >= t.z || !in) return;
-        const float s = of_row.x;
-        *(float4*)(a.y + (int64_t)__builtin_bit_cast(int, of_row.y) * a.H + n) =
-            make_float4((float)x[0] * s * sd.x, (float)x[1] * s * sd.y, (float)x[2] * s * sd.z, (float)x[3] * s * sd.w);
+        float v[VEC];
+#pragma unroll
+        for (int k = 0; k < VEC; k++)
+            v[k] = sizeof(Y) == 4 ? (float)x[k] * of_row.x * sd[k] : (float)x[k] * unit;
+        store_row((Y*)a.y + (int64_t)(t.y + r) * a.H + n, v, VEC, true);
     });
 }
 
-// out[t] = sum over k, ascending, of w[t][k] y[t][k]; a pair whose id is no
-// expert adds nothing.
-template <typename T>
+// out[t] = sum over k, ascending, of w[t][k] y[t][k]; a pair that was left out
+// adds nothing.  A thread takes VEC neighbouring columns, four pairs' loads
+// at a time.
+template <typename Y, typename T>
 __global__ __launch_bounds__(256) void k_i8_combine(MoeI8 a) {
-    const int hb = (a.H + 255) / 256, t = blockIdx.x / hb, h = (blockIdx.x - t * hb) * 256 + threadIdx.x;
-    if (h >= a.H) return;
-    float acc = 0.0f;
-    for (int k = 0; k < a.K; k++) {
-        const int64_t p = (int64_t)t * a.K + k;
-        if ((unsigned)a.ids[p] < (unsigned)a.E) acc = __builtin_fmaf(a.wts[p], a.y[p * a.H + h], acc);
+    constexpr int VEC = 16 / sizeof(Y), AT = 4;
+    typedef Y vec __attribute__((ext_vector_type(VEC)));
+    __shared__ float w[MAX_K], hs[MAX_K];
+    __shared__ int pos[MAX_K], es[MAX_K];
+    const int hb = (a.H / VEC + 255) / 256, t = blockIdx.x / hb, n = ((blockIdx.x - t * hb) * 256 + threadIdx.x) * VEC;
+    if ((int)threadIdx.x < a.K) {
+        const int64_t p = (int64_t)t * a.K + threadIdx.x;
+        const int q = a.pos[p];
+        pos[threadIdx.x] = q;
+        es[threadIdx.x] = a.ids[p];
+        w[threadIdx.x] = a.wts[p];
+        hs[threadIdx.x] = sizeof(Y) == 2 && q >= 0 ? a.hs[q] : 0.0f;
     }
-    store_f((T*)a.out + t * a.ldo + h, acc);
+    __syncthreads();
+    if (n >= a.H) return;   // H is a multiple of 16
+    const float unit = __builtin_ldexpf(1.0f, a.shift);
+    float acc[VEC] = {};
+    for (int k0 = 0; k0 < a.K; k0 += AT) {
+        vec y[AT];
+        float sd[AT][VEC];
+#pragma unroll
+        for (int i = 0; i < AT; i++) {
+            if (k0 + i < a.K && pos[k0 + i] >= 0) {
+                y[i] = *(const vec*)((const Y*)a.y + (int64_t)pos[k0 + i] * a.H + n);
+                if constexpr (sizeof(Y) == 2) {
+#pragma unroll
+                    for (int c = 0; c < VEC; c += 4)
+                        *(float4*)(sd[i] + c) = *(const float4*)(a.down_s + (int64_t)es[k0 + i] * a.H + n + c);
+                }
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < AT; i++) {
+            if (k0 + i < a.K && pos[k0 + i] >= 0) {
+#pragma unroll
+                for (int c = 0; c < VEC; c++) {
+                    const float v = sizeof(Y) == 2 ? (float)y[i][c] * unit * hs[k0 + i] * sd[i][c] : (float)y[i][c];
+                    acc[c] = __builtin_fmaf(w[k0 + i], v, acc[c]);
+                }
+            }
+        }
+    }
+    T* to = (T*)a.out + t * a.ldo + n;
+    if constexpr (sizeof(T) * VEC <= 16) {
+        store_row(to, acc, VEC, (((uintptr_t)a.out | (uintptr_t)(a.ldo * sizeof(T))) & 15) == 0);
+    } else {
+#pragma unroll
+        for (int c = 0; c < VEC; c++) store_f(to + c, acc[c]);
+    }
 }
 
+// ------------------------------------------------------------ host
+
+constexpr int MOE_FEW = 64;
+static int moe_tile_pairs(double avg) {
+    return avg <= 24 ? 32 : avg <= 64 ? 64 : 128;
+}
 struct MoeI8Plan {
-    size_t xq, xs, order, total, tiles, h, hq, hs, y, bytes;
-    int max_tiles;
+    size_t xq, xs, order, pos, total, tiles, h, hq, hs, y, bytes;
+    int max_tiles, tile_pairs;
+    bool few;
 };
 
 static MoeI8Plan plan_moe_i8(int H, int F, int E, int K, int T) {
     MoeI8Plan p{};
     const size_t P = (size_t)T * K;
-    p.max_tiles = (int)(P / GuTile::BM + (P < (size_t)E ? P : (size_t)E));
+    // a few pairs, whose rows fit the work-groups' registers
+    p.few = P <= MOE_FEW && pad_to(H, I8_BK) <= 64 * FP_WAVES * FP_KEEP &&
+            K * pad_to(F, I8_BK) <= 64 * FP_WAVES * FP_KEEP;
     auto take = [&](size_t& at, size_t n) { at = p.bytes; p.bytes += al256(n); };
+    take(p.h, P * F * 4);
+    if (p.few) return p;
+    p.tile_pairs = moe_tile_pairs((double)P / E);
+    p.max_tiles = (int)(P / p.tile_pairs + (P < (size_t)E ? P : (size_t)E));
     take(p.xq, (size_t)T * H);
     take(p.xs, (size_t)T * 4);
     take(p.order, P * 4);
+    take(p.pos, P * 4);
     take(p.total, 8);
-    take(p.tiles, (size_t)p.max_tiles * sizeof(int4));
-    take(p.h, P * F * 4);
+    // the list for the smallest tile, so that more tokens never need less
+    take(p.tiles, (P / 32 + (P < (size_t)E ? P : (size_t)E)) * sizeof(int4));
     take(p.hq, P * F);
     take(p.hs, P * 4);
     take(p.y, P * H * 4);
     return p;
+}
+
+template <typename Tile, int WAVES_PER_SIMD>
+static void launch_gate_up(const MoeI8& a, int max_tiles, hipStream_t s) {
+    const int fb = (a.F + Tile::BN / 2 - 1) / (Tile::BN / 2);
+    hipLaunchKernelGGL((k_i8_gate_up<Tile, WAVES_PER_SIMD>), dim3((unsigned)(max_tiles * fb)), dim3(64 * Tile::NW), 0, s, a);
+}
+template <typename Tile, int WAVES_PER_SIMD>
+static void launch_down(const MoeI8& a, int max_tiles, bool half, hipStream_t s) {
+    const dim3 grid((unsigned)(max_tiles * ((a.H + Tile::BN - 1) / Tile::BN)));
+    if (half) hipLaunchKernelGGL((k_i8_down<Tile, WAVES_PER_SIMD, _Float16>), grid, dim3(64 * Tile::NW), 0, s, a);
+    else hipLaunchKernelGGL((k_i8_down<Tile, WAVES_PER_SIMD, float>), grid, dim3(64 * Tile::NW), 0, s, a);
+}
+
+static void launch_few_pairs(const MoeI8& a, int type, int out_type, hipStream_t s) {
+    const dim3 gu(a.F / 16, a.T * a.K), dn(a.H / 16, a.T), block(64 * FP_WAVES);
+    const size_t lx = 16 + pad_to(a.H, I8_BK), lh = a.K * pad_to(a.F, I8_BK);
+    if (type == T_F32) hipLaunchKernelGGL(k_i8_pair_gate_up<float>, gu, block, lx, s, a);
+    else if (type == T_F16) hipLaunchKernelGGL(k_i8_pair_gate_up<_Float16>, gu, block, lx, s, a);
+    else hipLaunchKernelGGL(k_i8_pair_gate_up<__bf16>, gu, block, lx, s, a);
+    if (out_type == T_F32) hipLaunchKernelGGL(k_i8_pair_down<float>, dn, block, lh, s, a);
+    else if (out_type == T_F16) hipLaunchKernelGGL(k_i8_pair_down<_Float16>, dn, block, lh, s, a);
+    else hipLaunchKernelGGL(k_i8_pair_down<__bf16>, dn, block, lh, s, a);
+}
+
+static void launch_many_pairs(const MoeI8& a, const MoeI8Plan& p, int type, int out_type, hipStream_t s) {
+    launch_i8_quantize(type, a.x, a.ldx, a.xq, a.H, a.xs, a.T, a.H, s);
+    hipLaunchKernelGGL(k_i8_plan, dim3(1), dim3(1024), 0, s, a);
+    if (p.tile_pairs == 32) launch_gate_up<I8Tile<1, 4, 1, 1, 4>, 1>(a, p.max_tiles, s);
+    else if (p.tile_pairs == 64) launch_gate_up<I8Tile<2, 4, 1, 1, 3>, 2>(a, p.max_tiles, s);
+    else launch_gate_up<I8Tile<2, 4, 2, 1, 2>, 2>(a, p.max_tiles, s);
+    launch_i8_quantize(T_F32, a.h, a.F, a.hq, a.F, a.hs, (int64_t)a.T * a.K, a.F, s);
+    const bool half = out_type != T_F32;
+    if (p.tile_pairs == 32) launch_down<I8Tile<1, 4, 1, 1, 4>, 1>(a, p.max_tiles, half, s);
+    else if (p.tile_pairs == 64) launch_down<I8Tile<2, 4, 1, 1, 3>, 2>(a, p.max_tiles, half, s);
+    else launch_down<I8Tile<2, 4, 2, 1, 2>, 2>(a, p.max_tiles, half, s);
+    const dim3 grid((unsigned)((a.H / (half ? 8 : 4) + 255) / 256) * a.T);
+    if (out_type == T_F32) hipLaunchKernelGGL((k_i8_combine<float, float>), grid, dim3(256), 0, s, a);
+    else if (out_type == T_F16) hipLaunchKernelGGL((k_i8_combine<_Float16, _Float16>), grid, dim3(256), 0, s, a);
+    else hipLaunchKernelGGL((k_i8_combine<_Float16, __bf16>), grid, dim3(256), 0, s, a);
 }
 
 static bool moe_i8_shape(const chimere_moe_i8_layer* L, int K, int T) {
@@ -225,21 +468,19 @@ void chimere_moe_i8(const chimere_moe_i8_layer* L, int type, const void* x, int6
     a.H = H; a.F = F; a.E = L->n_experts; a.K = top_k; a.T = ntok;
     a.gate = L->gate; a.up = L->up; a.down = L->down;
     a.gate_s = L->gate_scale; a.up_s = L->up_scale; a.down_s = L->down_scale;
-    a.ids = ids; a.wts = weights; a.out = out; a.ldo = out_stride;
-    a.xq = (int8_t*)(w + p.xq); a.xs = (float*)(w + p.xs);
-    a.order = (int*)(w + p.order); a.total = (int*)(w + p.total); a.tiles = (int4*)(w + p.tiles);
-    a.h = (float*)(w + p.h); a.hq = (int8_t*)(w + p.hq); a.hs = (float*)(w + p.hs); a.y = (float*)(w + p.y);
-    a.tile_pairs = GuTile::BM;
-    launch_i8_quantize(type, x, x_stride, (int8_t*)a.xq, H, (float*)a.xs, ntok, H, stream);
-    hipLaunchKernelGGL(k_i8_plan, dim3(1), dim3(1024), 0, stream, a);
-    const int fb = (F + GuTile::BN / 2 - 1) / (GuTile::BN / 2), hb = (H + DnTile::BN - 1) / DnTile::BN;
-    hipLaunchKernelGGL(k_i8_gate_up, dim3((unsigned)(p.max_tiles * fb)), dim3(64 * GuTile::NW), 0, stream, a);
-    launch_i8_quantize(T_F32, a.h, F, a.hq, F, a.hs, (int64_t)ntok * top_k, F, stream);
-    hipLaunchKernelGGL(k_i8_down, dim3((unsigned)(p.max_tiles * hb)), dim3(64 * DnTile::NW), 0, stream, a);
-    const dim3 grid((unsigned)((H + 255) / 256) * ntok);
-    if (out_type == T_F32) hipLaunchKernelGGL(k_i8_combine<float>, grid, dim3(256), 0, stream, a);
-    else if (out_type == T_F16) hipLaunchKernelGGL(k_i8_combine<_Float16>, grid, dim3(256), 0, stream, a);
-    else hipLaunchKernelGGL(k_i8_combine<__bf16>, grid, dim3(256), 0, stream, a);
+    a.ids = ids; a.wts = weights; a.x = x; a.ldx = x_stride; a.out = out; a.ldo = out_stride;
+    a.h = (float*)(w + p.h);
+    if (p.few) {
+        launch_few_pairs(a, type, out_type, stream);
+    } else {
+        a.xq = (int8_t*)(w + p.xq); a.xs = (float*)(w + p.xs);
+        a.order = (int*)(w + p.order); a.pos = (int*)(w + p.pos);
+        a.total = (int*)(w + p.total); a.tiles = (int4*)(w + p.tiles);
+        a.hq = (int8_t*)(w + p.hq); a.hs = (float*)(w + p.hs); a.y = w + p.y;
+        a.tile_pairs = p.tile_pairs;
+        while ((16256.0 * F) / (double)((int64_t)1 << a.shift) > 65504.0) a.shift++;
+        launch_many_pairs(a, p, type, out_type, stream);
+    }
     check_launch("moe_i8");
 }
 

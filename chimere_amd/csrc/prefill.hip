@@ -196,35 +196,6 @@ __global__ __launch_bounds__(64 * PF_TKT) void k_pf_topk(PfArgs a) {
     for (int i = tid; i < a.E; i += 64 * PF_TKT) a.cnt[(int64_t)blockIdx.x * a.E + i] = cnt[i];
 }
 
-// exclusive prefix sum of one int per thread over a 1024-thread group
-__device__ __forceinline__ int excl_scan1024(int v, int* wsum, int* total) {
-    const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
-    int x = v;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-        const int y = __shfl_up(x, d);
-        if (lane >= d) x += y;
-    }
-    if (lane == 63) wsum[w] = x;
-    __syncthreads();
-    if (w == 0) {
-        const int t = lane < 16 ? wsum[lane] : 0;
-        int sc = t;
-#pragma unroll
-        for (int d = 1; d < 16; d <<= 1) {
-            const int y = __shfl_up(sc, d);
-            if (lane >= d) sc += y;
-        }
-        __syncthreads();   // pairs with the barrier below for the other waves
-        if (lane < 16) wsum[lane] = sc - t;
-        if (lane == 15) *total = sc;
-    } else {
-        __syncthreads();
-    }
-    __syncthreads();
-    return x - v + wsum[w];
-}
-
 // P3: counting sort of the T*K pairs by expert (inside an expert by 16-token top-k
 // work-group, otherwise in any order, which may differ between runs: every
 // pair's output row is computed on its own, so no result depends on it), the shared expert as expert E with all T

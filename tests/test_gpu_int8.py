@@ -238,7 +238,9 @@ def experts_ref(layer, x, ids, wts, dtype):
         ey = y.abs() * (srel + 4 * U) + near @ down[e].abs().T * s * ds[e]
         w = wts[t, k, None]
         out.index_add_(0, t, w * y)
-        tol.index_add_(0, t, w.abs() * (ey + y.abs() * (K + 2) * U))
+        # for 16-bit outputs a pair's sum is held as f16: half a step, 2^-11 of it
+        half = 0.0 if dtype == torch.float32 else 2.0 ** -11
+        tol.index_add_(0, t, w.abs() * (ey + (y.abs() + ey) * ((K + 2) * U + half)))
     return out, tol * (1 + STEP[dtype]) + STEP[dtype] * out.abs() + TINY[dtype]
 
 
