@@ -7,80 +7,22 @@
 
 namespace chimere {
 
-// Row quantizer: scale = max |x| / 127, q = x / scale rounded to the nearest
-// integer, ties to even (IEEE divisions).  A row that holds an infinity or a
-// NaN keeps it in the scale and 0 in its integers, so its products are NaN.
-// Bound by the row's bytes.  W waves per row (rows of up to 1024 columns one,
-// longer ones four: 4 W rows' worth of latency is hidden by the other
-// work-groups), 16 elements of each lane stay in registers between the
-// maximum and the integers; columns past 1024 W are read twice.
+// Row quantizer.  A row that holds an infinity or a NaN keeps it in the scale
+// and 0 in its integers, so its products are NaN.  Bound by the rows' bytes.
 template <typename T, int W>
-__global__ __launch_bounds__(256) void k_i8_quantize(const T* __restrict__ x, int64_t xs, int8_t* __restrict__ q,
-                                                     int64_t qs, float* __restrict__ scale, int64_t nrows, int ncols,
-                                                     bool wide) {
-    constexpr int V = 16 / sizeof(T), KEEP = 16 / V, STEP = 64 * W * V;
-    __shared__ uint32_t part[4];
-    const int wave = threadIdx.x >> 6;
-    const int64_t r = (int64_t)blockIdx.x * (4 / W) + wave / W;
-    if (r >= nrows) return;   // W = 1 only: no barrier follows
-    const T* row = x + r * xs;
-    const int c0 = (threadIdx.x & (64 * W - 1)) * V;
-    float v[KEEP][V];
-    uint32_t m = 0;
-#pragma unroll
-    for (int i = 0; i < KEEP; i++) {
-        i8_load(row, c0 + i * STEP, ncols, wide, v[i]);
-        m = i8_amax(m, v[i]);
-    }
-    for (int c = c0 + KEEP * STEP; c < ncols; c += STEP) {
-        float u[V];
-        i8_load(row, c, ncols, wide, u);
-        m = i8_amax(m, u);
-    }
-    m = wave_amax(m);
-    if constexpr (W == 4) {
-        if ((threadIdx.x & 63) == 0) part[wave] = m;
-        __syncthreads();
-        m = max(max(part[0], part[1]), max(part[2], part[3]));
-    }
-    const float d = __builtin_bit_cast(float, m) / 127.0f;
-    if (c0 == 0) scale[r] = d;
-    int8_t* to = q + r * qs;
-    auto put = [&](int c, const float(&u)[V]) {
-        uint32_t p[V / 4];
-        i8_pack<V>(u, d, p);
-        if (c + V <= ncols) {
-            typedef uint32_t words __attribute__((ext_vector_type(V / 4)));
-            words o;
-#pragma unroll
-            for (int k = 0; k < V / 4; k++) o[k] = p[k];
-            *(words*)(to + c) = o;
-        } else {
-#pragma unroll
-            for (int k = 0; k < V; k++)
-                if (c + k < ncols) to[c + k] = (int8_t)(p[k / 4] >> (8 * (k & 3)));
-        }
-    };
-#pragma unroll
-    for (int i = 0; i < KEEP; i++)
-        if (c0 + i * STEP < ncols) put(c0 + i * STEP, v[i]);
-    for (int c = c0 + KEEP * STEP; c < ncols; c += STEP) {
-        float u[V];
-        i8_load(row, c, ncols, wide, u);
-        put(c, u);
-    }
+__global__ __launch_bounds__(256) void k_i8_quantize(I8Rows<T> q) {
+    i8_quantize_rows<T, W, 256>(q, blockIdx.x);
 }
 
 template <typename T>
 static void launch_i8_quantize(const T* x, int64_t xs, int8_t* q, int64_t qs, float* scale, int64_t nrows, int ncols,
                                hipStream_t s) {
     const bool wide = (((uintptr_t)x | (uintptr_t)(xs * sizeof(T))) & 15) == 0;
-    if (ncols <= 1024)
-        hipLaunchKernelGGL((k_i8_quantize<T, 1>), dim3((unsigned)((nrows + 3) / 4)), dim3(256), 0, s, x, xs, q, qs, scale,
-                           nrows, ncols, wide);
-    else
-        hipLaunchKernelGGL((k_i8_quantize<T, 4>), dim3((unsigned)nrows), dim3(256), 0, s, x, xs, q, qs, scale, nrows,
-                           ncols, wide);
+    const I8Rows<T> r{x, xs, q, qs, scale, nullptr, nullptr, nrows, ncols, wide};
+    const int per = i8_rows_per_group<256>(ncols);
+    const dim3 grid((unsigned)((nrows + per - 1) / per));
+    if (ncols <= I8_WAVE_ROW) hipLaunchKernelGGL((k_i8_quantize<T, 1>), grid, dim3(256), 0, s, r);
+    else hipLaunchKernelGGL((k_i8_quantize<T, 4>), grid, dim3(256), 0, s, r);
 }
 
 void launch_i8_quantize(int type, const void* x, int64_t xs, int8_t* q, int64_t qs, float* scale, int64_t nrows,
@@ -122,9 +64,6 @@ __global__ __launch_bounds__(64 * Tile::NW, WAVES_PER_SIMD) void k_i8_gemm(I8Gem
     for (int p = 0; p < Tile::PN; p++)
         woff[p] = (uint32_t)(min((wave * Tile::PN + p) * 8 + (lane >> 3), g.N - 1 - n0) * g.ldw);
     const float as = threadIdx.x < Tile::BM ? g.as[min(m0 + (int)threadIdx.x, g.M - 1)] : 0.0f;
-    v16i acc[Tile::MTILES][Tile::NTILES];
-    const int8_t* w = g.w + n0 * g.ldw;
-    Tile::run(g.a + m0 * g.lda, w, w, aoff, woff, g.C, lds, acc);
     const int n = n0 + Tile::template first_col<VEC>();
     float ws[VEC], b[VEC];
 #pragma unroll
@@ -133,6 +72,9 @@ __global__ __launch_bounds__(64 * Tile::NW, WAVES_PER_SIMD) void k_i8_gemm(I8Gem
         ws[k] = g.ws[nk];
         b[k] = g.bias ? g.bias[nk] : 0.0f;
     }
+    v16i acc[Tile::MTILES][Tile::NTILES];
+    const int8_t* w = g.w + n0 * g.ldw;
+    Tile::run(g.a + m0 * g.lda, w, w, aoff, woff, g.C, lds, acc);
     const bool wide = (((uintptr_t)g.out | (uintptr_t)(g.ldo * sizeof(T))) & 15) == 0;
     Tile::template rows<VEC>(lds, acc, make_float2(as, 0.0f), [&](int r, const int(&x)[VEC], float2 of_row) {
         if (m0 + r >= g.M || n >= g.N) return;
@@ -173,6 +115,24 @@ __global__ __launch_bounds__(64 * FEW_WAVES) void k_i8_few(I8Gemm g) {
             for (int h = 0; h < 2; h++) fw[j][h] = *(const v4i*)(wrow[j] + min(8 * s + pc + h, last) * 16);
     };
     if (wave < S) load_w(wave);
+    // the scales of this thread's outputs (`at`), ahead of all that is waited for
+    constexpr int OUTS = (MB * NB * 256 + 64 * FEW_WAVES - 1) / (64 * FEW_WAVES);
+    float ws[OUTS], bias[OUTS];
+    // register v of lane l in a block (i, j): token 4 (l / 16) + v, weight row l % 16
+    auto at = [&](int q, int& m, int& n, int& from) {
+        const int o = tid + q * 64 * FEW_WAVES, i = o / (NB * 256), v = o >> 6 & 3, l = o & 63, j = o / 256 % NB;
+        m = i * 16 + 4 * (l >> 4) + v;
+        n = n0 + j * 16 + (l & 15);
+        from = (i * NB + j) * 256 + l * 4 + v;
+        return o < MB * NB * 256 && m < M && n < g.N;
+    };
+#pragma unroll
+    for (int q = 0; q < OUTS; q++) {
+        int m, n, from;
+        const bool in = at(q, m, n, from);
+        ws[q] = in ? g.ws[n] : 0.0f;
+        bias[q] = in && g.bias ? g.bias[n] : 0.0f;
+    }
     float* as = (float*)lds;   // [16 MB]
     uint8_t* aq = lds + 16 * MB * 4;
     if constexpr (QUANT) {
@@ -222,15 +182,13 @@ __global__ __launch_bounds__(64 * FEW_WAVES) void k_i8_few(I8Gemm g) {
 #pragma unroll
         for (int j = 0; j < NB; j++) *(v4i*)(part + ((wave * MB + i) * NB + j) * 256 + lane * 4) = acc[i][j];
     __syncthreads();
-    for (int o = tid; o < MB * NB * 256; o += 64 * FEW_WAVES) {
-        // register v of lane l in a block: token 4 (l / 16) + v, weight row l % 16
-        const int i = o / (NB * 256), v = o >> 6 & 3, l = o & 63, j = o / 256 % NB;
-        const int m = i * 16 + 4 * (l >> 4) + v, n = n0 + j * 16 + (l & 15);
-        if (m >= M || n >= g.N) continue;
-        int sum = 0;
 #pragma unroll
-        for (int w = 0; w < FEW_WAVES; w++) sum += part[((w * MB + i) * NB + j) * 256 + l * 4 + v];
-        store_f((T*)g.out + (m0 + m) * g.ldo + n, (float)sum * as[m] * g.ws[n] + (g.bias ? g.bias[n] : 0.0f));
+    for (int q = 0; q < OUTS; q++) {
+        int m, n, from, sum = 0;
+        if (!at(q, m, n, from)) continue;
+#pragma unroll
+        for (int w = 0; w < FEW_WAVES; w++) sum += part[w * MB * NB * 256 + from];
+        store_f((T*)g.out + (m0 + m) * g.ldo + n, (float)sum * as[m] * ws[q] + bias[q]);
     }
 }
 

@@ -38,6 +38,14 @@ __device__ __forceinline__ void copy16_lds_base(const void* base, uint32_t off, 
                      : "memory");
 }
 
+// a pointer that is the same for the whole wave, in scalar registers
+__device__ __forceinline__ const int8_t* wave_uniform(const int8_t* p) {
+    const uint64_t v = (uint64_t)(uintptr_t)p;
+    const uint64_t lo = (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)v);
+    const uint64_t hi = (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)(v >> 32));
+    return (const int8_t*)(uintptr_t)(hi << 32 | lo);
+}
+
 // `v` (columns k0 .. k0 + 15 of a row) with the columns from C on cleared
 __device__ __forceinline__ v4i clear_tail(v4i v, int k0, int C) {
 #pragma unroll
@@ -48,12 +56,15 @@ __device__ __forceinline__ v4i clear_tail(v4i v, int k0, int C) {
     return v;
 }
 
-// WM x WN waves, each MT x NT blocks of 32 x 32; NS stages
-template <int WM, int WN, int MT, int NT, int NS = 2>
+// WM x WN waves, each MT x NT blocks of 32 x 32; NS stages of weight rows and NA
+// of token rows (these come from L2, the weights often from HBM: more of them
+// in flight is what hides the longer way)
+template <int WM, int WN, int MT, int NT, int NS = 2, int NA = NS>
 struct I8Tile {
     static constexpr int BM = WM * MT * 32, BN = WN * NT * 32, NW = WM * WN;
     static constexpr int WAVES_N = WN, MTILES = MT, NTILES = NT;
-    static constexpr int STAGE = (BM + BN) * I8_BK, LDS = NS * STAGE;
+    static constexpr int SA = BM * I8_BK, SW = BN * I8_BK, LDS = NA * SA + NS * SW;
+    static_assert(NA >= 2 && NA <= NS, "stages");
     static constexpr int PM = BM / 8 / NW, PN = BN / 8 / NW;   // pieces of 8 rows that a wave copies
     static_assert(PM * 8 * NW == BM && PN * 8 * NW == BN, "tile rows over waves");
 
@@ -65,36 +76,50 @@ struct I8Tile {
                                                uint8_t* lds, v16i (&acc)[MT][NT]) {
         const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
         const int wm = wave / WN, wn = wave % WN;
+        a = wave_uniform(a);
+        w = wave_uniform(w);
+        w2 = wave_uniform(w2);
         const int S = (C + I8_BK - 1) / I8_BK, last = (C + 15) / 16 - 1, pc = (lane & 7) ^ (lane >> 4);
         const uint32_t lds0 = (uint32_t)(uintptr_t)(lds_void_t*)lds;
         // copies of step s into stage `to`; past the last step the same columns
         // again, so that the count of copies in flight stays the same
-        auto stage = [&](int s, int to) {
-            const uint32_t at = lds0 + to * STAGE;
+        auto stage_a = [&](int s, int to) {
             const uint32_t k0 = (uint32_t)min(8 * s + pc, last) * 16u, k1 = (uint32_t)min(8 * s + (pc ^ 4), last) * 16u;
 #pragma unroll
             for (int p = 0; p < PM; p++)
-                copy16_lds_base(a, aoff[p] + ((wave * PM + p) & 1 ? k1 : k0), at + (wave * PM + p) * 1024);
+                copy16_lds_base(a, aoff[p] + ((wave * PM + p) & 1 ? k1 : k0), lds0 + to * SA + (wave * PM + p) * 1024);
+        };
+        auto stage_w = [&](int s, int to) {
+            const uint32_t k0 = (uint32_t)min(8 * s + pc, last) * 16u, k1 = (uint32_t)min(8 * s + (pc ^ 4), last) * 16u;
 #pragma unroll
             for (int p = 0; p < PN; p++)
                 copy16_lds_base((wave * PN + p) & 2 ? w2 : w, woff[p] + ((wave * PN + p) & 1 ? k1 : k0),
-                                at + BM * I8_BK + (wave * PN + p) * 1024);
+                                lds0 + NA * SA + to * SW + (wave * PN + p) * 1024);
         };
 #pragma unroll
         for (int i = 0; i < MT; i++)
 #pragma unroll
             for (int j = 0; j < NT; j++) acc[i][j] = v16i{};
+        // in the order of the steps below, which issue token rows first
 #pragma unroll
-        for (int s = 0; s < NS - 1; s++) stage(s, s);
+        for (int s = 0; s < NS - 1; s++) {
+            if (s >= NS - NA) stage_a(s - (NS - NA), s - (NS - NA));
+            stage_w(s, s);
+        }
         const int r = lane & 31, g = lane >> 5;
-        int cur = 0, nxt = NS - 1;
+        int ca = 0, na = NA - 1, cw = 0, nw = NS - 1;
         auto step = [&](int s, auto tail) {
-            wait_vm<(NS - 2) * (PM + PN)>();   // this wave's copies of step s have landed,
-            lds_barrier();                     // every wave's; and step s - 1 has been read by all
-            stage(s + NS - 1, nxt);
-            const uint8_t* at = lds + cur * STAGE;
-            cur = cur + 1 == NS ? 0 : cur + 1;
-            nxt = nxt + 1 == NS ? 0 : nxt + 1;
+            // this wave's copies of step s have landed (issued later: the weights
+            // of NS - NA steps more, and NA - 2 whole steps),
+            wait_vm<(NA < NS ? PN : 0) + (NA - 2) * (PM + PN)>();
+            lds_barrier();   // every wave's; and step s - 1 has been read by all
+            stage_a(s + NA - 1, na);
+            stage_w(s + NS - 1, nw);
+            const uint8_t *at = lds + ca * SA, *wt = lds + NA * SA + cw * SW;
+            ca = ca + 1 == NA ? 0 : ca + 1;
+            na = na + 1 == NA ? 0 : na + 1;
+            cw = cw + 1 == NS ? 0 : cw + 1;
+            nw = nw + 1 == NS ? 0 : nw + 1;
             // the fragments of columns 32 (q + 1) are read while those of 32 q multiply
             v4i fa[2][MT], fw[2][NT];
             auto read = [&](int q) {
@@ -104,7 +129,7 @@ struct I8Tile {
                     fa[q & 1][i] = *(const v4i*)(at + ((wm * MT + i) * 32 + r) * I8_BK + piece);
 #pragma unroll
                 for (int j = 0; j < NT; j++)
-                    fw[q & 1][j] = *(const v4i*)(at + (BM + (wn * NT + j) * 32 + r) * I8_BK + piece);
+                    fw[q & 1][j] = *(const v4i*)(wt + ((wn * NT + j) * 32 + r) * I8_BK + piece);
                 if (tail) {
 #pragma unroll
                     for (int i = 0; i < MT; i++) fa[q & 1][i] = clear_tail(fa[q & 1][i], s * I8_BK + c * 16, C);
@@ -198,9 +223,5 @@ __device__ __forceinline__ void store_row(T* p, const float (&v)[N], int count, 
             if (k < count) p[k] = (T)v[k];
     }
 }
-
-// row quantizer (int8.hip), for float rows of a type on the device
-void launch_i8_quantize(int type, const void* x, int64_t xs, int8_t* q, int64_t qs, float* scale, int64_t nrows,
-                        int ncols, hipStream_t s);
 
 }  // namespace chimere

@@ -73,9 +73,9 @@ __device__ __forceinline__ void i8_rows_to_lds(int M, int cols, int lda, float* 
             load(m, (at - m * per) * V, v[i]);
             top = i8_amax(0u, v[i]);
         }
-        if (M == 1) {
+        if (__all(m == __builtin_amdgcn_readfirstlane(m))) {   // a wave within one row: one atomic
             top = wave_amax(top);
-            if ((tid & 63) == 0) atomicMax(&bits[0], top);
+            if ((tid & 63) == 0) atomicMax(&bits[m], top);
         } else if (at < n) {
             atomicMax(&bits[m], top);
         }
@@ -95,5 +95,89 @@ __device__ __forceinline__ void i8_rows_to_lds(int M, int cols, int lda, float* 
     }
     __syncthreads();
 }
+
+template <typename T>
+struct I8Rows {
+    const T* x;
+    int64_t xs;
+    int8_t* q;
+    int64_t qs;
+    float* scale;
+    const int* to;      // scale of row r at scale[to[r]], or null: scale[r]
+    const int* count;   // rows, where the device has counted them, or null: nrows
+    int64_t nrows;
+    int ncols;
+    bool wide;
+};
+
+// A row goes to one wave up to 1024 columns, to four above: 16 elements of
+// each lane stay in registers between the maximum and the integers; columns
+// past 4096 are read twice.
+constexpr int I8_WAVE_ROW = 1024;
+template <int THREADS>
+constexpr int i8_rows_per_group(int ncols) { return THREADS / 64 / (ncols <= I8_WAVE_ROW ? 1 : 4); }
+
+// The rows of work-group `group` of THREADS threads, W waves each.
+template <typename T, int W, int THREADS>
+__device__ __forceinline__ void i8_quantize_rows(const I8Rows<T>& g, int64_t group) {
+    constexpr int V = 16 / sizeof(T), KEEP = 16 / V, STEP = 64 * W * V;
+    __shared__ uint32_t part[THREADS / 64];
+    const int wave = threadIdx.x >> 6;
+    const int64_t r = group * (THREADS / 64 / W) + wave / W;
+    const bool on = r < (g.count ? *g.count : g.nrows);
+    if (W == 1 && !on) return;   // no barrier follows
+    const T* row = g.x + (on ? r : 0) * g.xs;
+    const int c0 = (threadIdx.x & (64 * W - 1)) * V, ncols = g.ncols;
+    float v[KEEP][V];
+    uint32_t m = 0;
+#pragma unroll
+    for (int i = 0; i < KEEP; i++) {
+        i8_load(row, c0 + i * STEP, ncols, g.wide, v[i]);
+        m = i8_amax(m, v[i]);
+    }
+    for (int c = c0 + KEEP * STEP; c < ncols; c += STEP) {
+        float u[V];
+        i8_load(row, c, ncols, g.wide, u);
+        m = i8_amax(m, u);
+    }
+    m = wave_amax(m);
+    if constexpr (W == 4) {
+        if ((threadIdx.x & 63) == 0) part[wave] = m;
+        __syncthreads();
+        const uint32_t* p = part + wave / 4 * 4;
+        m = max(max(p[0], p[1]), max(p[2], p[3]));
+        if (!on) return;
+    }
+    const float d = __builtin_bit_cast(float, m) / 127.0f;
+    if (c0 == 0) g.scale[g.to ? g.to[r] : r] = d;
+    int8_t* to = g.q + r * g.qs;
+    auto put = [&](int c, const float(&u)[V]) {
+        uint32_t p[V / 4];
+        i8_pack(u, d, p);
+        if (c + V <= ncols) {
+            typedef uint32_t words __attribute__((ext_vector_type(V / 4)));
+            words o;
+#pragma unroll
+            for (int k = 0; k < V / 4; k++) o[k] = p[k];
+            *(words*)(to + c) = o;
+        } else {
+#pragma unroll
+            for (int k = 0; k < V; k++)
+                if (c + k < ncols) to[c + k] = (int8_t)(p[k / 4] >> (8 * (k & 3)));
+        }
+    };
+#pragma unroll
+    for (int i = 0; i < KEEP; i++)
+        if (c0 + i * STEP < ncols) put(c0 + i * STEP, v[i]);
+    for (int c = c0 + KEEP * STEP; c < ncols; c += STEP) {
+        float u[V];
+        i8_load(row, c, ncols, g.wide, u);
+        put(c, u);
+    }
+}
+
+// rows of a float type (int8.hip)
+void launch_i8_quantize(int type, const void* x, int64_t xs, int8_t* q, int64_t qs, float* scale, int64_t nrows,
+                        int ncols, hipStream_t s);
 
 }  // namespace chimere

@@ -28,13 +28,14 @@ struct MoeI8 {
     int64_t ldx;
     int8_t* xq;            // [T][H]
     float* xs;             // [T]
-    int *order, *pos;      // sorted position -> pair, pair -> sorted position (-1: left out)
+    int *order, *rank;     // sorted position -> pair; pair -> rank among 1024 pairs' of its expert
     int* total;            // {pairs, tiles}
+    int* cnt;              // pairs per expert of every 1024 pairs
     int4* tiles;           // {expert, first sorted pair, pairs, 0}
     float* h;              // [pairs][F], in sorted order (few pairs: by pair)
     int8_t* hq;
-    float* hs;
-    void* y;               // [pairs][H], in sorted order: f32, or f16 of sum * 2^-shift
+    float* hs;             // by pair
+    void* y;               // [pairs][H], by pair: f32, or f16 of sum * 2^-shift
     int shift;
     void* out;
     int64_t ldo;
@@ -115,8 +116,8 @@ __global__ __launch_bounds__(64 * FP_WAVES) void k_i8_pair_gate_up(MoeI8 a) {
 template <typename T>
 __global__ __launch_bounds__(64 * FP_WAVES) void k_i8_pair_down(MoeI8 a) {
     extern __shared__ __align__(16) uint8_t lds[];   // integers of h
-    __shared__ float hs[MAX_K];
-    __shared__ int sum[MAX_K][16], es[MAX_K];
+    __shared__ float hs[MAX_K], y[MAX_K][16];
+    __shared__ int sum[MAX_K][16];
     const int t = blockIdx.y, n0 = blockIdx.x * 16;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int S = (a.F + I8_BK - 1) / I8_BK, last = a.F / 16 - 1, r = lane & 15, pc = (lane >> 4) * 2;
@@ -131,20 +132,18 @@ __global__ __launch_bounds__(64 * FP_WAVES) void k_i8_pair_down(MoeI8 a) {
 #pragma unroll
     for (int i = 0; i < FP_AHEAD; i++)
         if (wave + i * FP_WAVES < a.K * S) load_w(wave + i * FP_WAVES, w[i]);
+    // thread -> (k, column): its scale and weight, ahead of all that is waited for
+    const int mk = tid >> 4, mc = tid & 15, me = mk < a.K ? ids[mk] : -1;
+    const bool mine = (unsigned)me < (unsigned)a.E;
+    const float sd = mine ? a.down_s[(int64_t)me * a.H + n0 + mc] : 0.0f;
+    const float wk = mine ? a.wts[(int64_t)t * a.K + mk] : 0.0f;
     if (tid < MAX_K * 16) (&sum[0][0])[tid] = 0;
-    if (tid < a.K) es[tid] = (unsigned)ids[tid] < (unsigned)a.E ? ids[tid] : -1;
-    __syncthreads();
+    // (a pair that was left out: whatever its row holds, its sums are not used)
     const int lda = S * I8_BK;
-    i8_rows_to_lds<64 * FP_WAVES, FP_KEEP>(a.K, S * I8_BK, lda, hs, lds,
-                                           [&](int k, int c, auto& v) {
-                                               if (es[k] >= 0) {
-                                                   i8_load(a.h + ((int64_t)t * a.K + k) * a.F, c, a.F, true, v);
-                                               } else {
-#pragma unroll
-                                                   for (int i = 0; i < 4; i++) v[i] = 0.0f;
-                                               }
-                                           },
-                                           std::integral_constant<int, 4>{});
+    i8_rows_to_lds<64 * FP_WAVES, FP_KEEP>(
+        a.K, S * I8_BK, lda, hs, lds,
+        [&](int k, int c, auto& v) { i8_load(a.h + ((int64_t)t * a.K + k) * a.F, c, a.F, true, v); },
+        std::integral_constant<int, 4>{});
     auto piece = [&](int u, const v4i(&now)[2]) {
         const int k = u / S, s = u - k * S;
         v4i acc = {};
@@ -162,12 +161,13 @@ __global__ __launch_bounds__(64 * FP_WAVES) void k_i8_pair_down(MoeI8 a) {
         piece(u, w[0]);
     }
     __syncthreads();
+    // a pair that was left out: 0 times 0
+    if (mk < a.K) y[mk][mc] = mine ? (float)sum[mk][mc] * hs[mk] * sd : 0.0f;
+    if (mk < MAX_K && mc == 0) hs[mk] = wk;
+    __syncthreads();
     if (tid < 16) {
         float acc = 0.0f;
-        for (int k = 0; k < a.K; k++)
-            if (es[k] >= 0)
-                acc = __builtin_fmaf(a.wts[(int64_t)t * a.K + k],
-                                     (float)sum[k][tid] * hs[k] * a.down_s[(int64_t)es[k] * a.H + n0 + tid], acc);
+        for (int k = 0; k < a.K; k++) acc = __builtin_fmaf(hs[k], y[k][tid], acc);
         store_f((T*)a.out + t * a.ldo + n0 + tid, acc);
     }
 }
@@ -176,47 +176,72 @@ __global__ __launch_bounds__(64 * FP_WAVES) void k_i8_pair_down(MoeI8 a) {
 
 // Counting sort of the pairs by expert; a pair whose id is no expert is left
 // out.  Pairs of one expert come in any order: each pair's row is computed on
-// its own.
-__global__ __launch_bounds__(1024) void k_i8_plan(MoeI8 a) {
+// its own.  A work-group takes 1024 pairs: counts per expert and each pair's
+// rank among them (PLAN 0); then every work-group adds up all counts, scans
+// them and places its own pairs, the first one lists the tiles (PLAN 1).  Up to
+// 1024 pairs: one work-group does both (PLAN 2).  (One work-group for 32768
+// pairs, its atomics one after another: 31 us.)
+template <int PLAN>
+__device__ __forceinline__ void i8_plan(const MoeI8& a, int groups) {
     __shared__ int first[MAX_E], wsum[16], tot[2];
-    const int tid = threadIdx.x, P = a.T * a.K, TP = a.tile_pairs;
-    first[tid] = 0;
-    __syncthreads();
-#pragma unroll 4
-    for (int p = tid; p < P; p += 1024) {
-        const int e = a.ids[p];
-        if ((unsigned)e < (unsigned)a.E) atomicAdd(&first[e], 1);
+    const int tid = threadIdx.x, p = blockIdx.x * 1024 + tid, P = a.T * a.K, TP = a.tile_pairs;
+    const int id = p < P ? a.ids[p] : -1, e = (unsigned)id < (unsigned)a.E ? id : -1;
+    int rank = 0;
+    if constexpr (PLAN != 1) {
+        first[tid] = 0;
+        __syncthreads();
+        if (e >= 0) rank = atomicAdd(&first[e], 1);
+        __syncthreads();
+        if constexpr (PLAN == 0) {
+            if (tid < a.E) a.cnt[blockIdx.x * a.E + tid] = first[tid];
+            if (e >= 0) a.rank[p] = rank;
+            return;
+        }
     }
-    __syncthreads();
-    const int c = first[tid], nt = (c + TP - 1) / TP;
+    int c = 0, before = 0;
+    if constexpr (PLAN == 1) {
+        if (e >= 0) rank = a.rank[p];
+        if (tid < a.E) {
+#pragma unroll 8
+            for (int g = 0; g < groups; g++) {
+                const int n = a.cnt[g * a.E + tid];
+                c += n;
+                before += g < (int)blockIdx.x ? n : 0;
+            }
+        }
+    } else {
+        c = first[tid];
+    }
+    const int nt = (c + TP - 1) / TP;
     const int at = excl_scan1024(c, wsum, &tot[0]);
     __syncthreads();
     const int tile = excl_scan1024(nt, wsum, &tot[1]);
-    first[tid] = at;
-    for (int s = 0; s < nt; s++) a.tiles[tile + s] = make_int4(tid, at + s * TP, min(TP, c - s * TP), 0);
+    first[tid] = at + before;
     __syncthreads();
+    if (e >= 0) a.order[first[e] + rank] = p;
+    if (blockIdx.x != 0) return;
+    for (int s = 0; s < nt; s++) a.tiles[tile + s] = make_int4(tid, at + s * TP, min(TP, c - s * TP), 0);
     if (tid < 2) a.total[tid] = tot[tid];
-#pragma unroll 4
-    for (int p = tid; p < P; p += 1024) {
-        const int e = a.ids[p];
-        int q = -1;
-        if ((unsigned)e < (unsigned)a.E) {
-            q = atomicAdd(&first[e], 1);
-            a.order[q] = p;
-        }
-        a.pos[p] = q;
-    }
 }
+
+// The first launch: `groups` work-groups plan, the others take rows of x to 8 bits.
+template <int PLAN, typename X>
+__global__ __launch_bounds__(1024) void k_i8_prepare(MoeI8 a, I8Rows<X> x, int groups) {
+    if ((int)blockIdx.x < groups) i8_plan<PLAN>(a, groups);
+    else if (a.H <= I8_WAVE_ROW) i8_quantize_rows<X, 1, 1024>(x, blockIdx.x - groups);
+    else i8_quantize_rows<X, 4, 1024>(x, blockIdx.x - groups);
+}
+__global__ __launch_bounds__(1024) void k_i8_plan(MoeI8 a, int groups) { i8_plan<1>(a, groups); }
+
+// rows of h, in sorted order, to 8 bits; their scales by pair
+template <int W>
+__global__ __launch_bounds__(256) void k_i8_hidden(I8Rows<float> h) { i8_quantize_rows<float, W, 256>(h, blockIdx.x); }
 
 // Gate and up of a tile: its weight rows alternate in blocks of 16 between
 // gate and up, so g and u of the same (pair, column) meet in a lane.
-template <typename Tile, int WAVES_PER_SIMD>
-__global__ __launch_bounds__(64 * Tile::NW, WAVES_PER_SIMD) void k_i8_gate_up(MoeI8 a) {
-    __shared__ __align__(16) uint8_t lds[Tile::LDS];
-    const int fb = (a.F + Tile::BN / 2 - 1) / (Tile::BN / 2), tile = blockIdx.x / fb;
-    if (tile >= a.total[1]) return;
-    const int4 t = a.tiles[tile];
-    const int f0 = (blockIdx.x - tile * fb) * (Tile::BN / 2), lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+template <typename Tile>
+__device__ __forceinline__ void i8_gate_up(const MoeI8& a, const int4& t, int f0, uint8_t* lds) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     uint32_t aoff[Tile::PM], woff[Tile::PN];
 #pragma unroll
     for (int p = 0; p < Tile::PM; p++) {
@@ -230,13 +255,13 @@ __global__ __launch_bounds__(64 * Tile::NW, WAVES_PER_SIMD) void k_i8_gate_up(Mo
     }
     const int64_t e = t.x;
     const float xs = threadIdx.x < Tile::BM ? a.xs[a.order[t.y + min((int)threadIdx.x, t.z - 1)] / a.K] : 0.0f;
-    v16i acc[Tile::MTILES][Tile::NTILES];
-    Tile::run(a.xq, a.gate + e * a.F * a.H, a.up + e * a.F * a.H, aoff, woff, a.H, lds, acc);
     constexpr int VEC = 4;
     const int f = f0 + Tile::template first_col<VEC, true>();
     const bool in = f < a.F;   // F is a multiple of 16: all four columns or none
     const float4 sg = in ? *(const float4*)(a.gate_s + e * a.F + f) : float4{};
     const float4 su = in ? *(const float4*)(a.up_s + e * a.F + f) : float4{};
+    v16i acc[Tile::MTILES][Tile::NTILES];
+    Tile::run(a.xq, a.gate + e * a.F * a.H, a.up + e * a.F * a.H, aoff, woff, a.H, lds, acc);
     Tile::template rows<VEC, true>(lds, acc, make_float2(xs, 0.0f),
                                    [&](int r, const int(&g)[VEC], const int(&u)[VEC], float2 of_row) {
         if (r >= t.z || !in) return;
@@ -255,13 +280,9 @@ __global__ __launch_bounds__(64 * Tile::NW, WAVES_PER_SIMD) void k_i8_gate_up(Mo
 // and each is off by 2^-11 of itself at most, whatever the scales, which the
 // weighted sum applies (16-bit rows halve what 32768 pairs of 2048 columns
 // write and read again, 268 MB each way).
-template <typename Tile, int WAVES_PER_SIMD, typename Y>
-__global__ __launch_bounds__(64 * Tile::NW, WAVES_PER_SIMD) void k_i8_down(MoeI8 a) {
-    __shared__ __align__(16) uint8_t lds[Tile::LDS];
-    const int hb = (a.H + Tile::BN - 1) / Tile::BN, tile = blockIdx.x / hb;
-    if (tile >= a.total[1]) return;
-    const int4 t = a.tiles[tile];
-    const int n0 = (blockIdx.x - tile * hb) * Tile::BN, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+template <typename Tile, typename Y>
+__device__ __forceinline__ void i8_down(const MoeI8& a, const int4& t, int n0, uint8_t* lds) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     uint32_t aoff[Tile::PM], woff[Tile::PN];
 #pragma unroll
     for (int p = 0; p < Tile::PM; p++)
@@ -270,70 +291,109 @@ __global__ __launch_bounds__(64 * Tile::NW, WAVES_PER_SIMD) void k_i8_down(MoeI8
     for (int p = 0; p < Tile::PN; p++)
         woff[p] = (uint32_t)min(n0 + (wave * Tile::PN + p) * 8 + (lane >> 3), a.H - 1) * (uint32_t)a.F;
     const int64_t e = t.x;
-    const float hs = threadIdx.x < Tile::BM ? a.hs[t.y + min((int)threadIdx.x, t.z - 1)] : 0.0f;
-    v16i acc[Tile::MTILES][Tile::NTILES];
-    const int8_t* w = a.down + e * a.H * a.F;
-    Tile::run(a.hq + (int64_t)t.y * a.F, w, w, aoff, woff, a.F, lds, acc);
+    const int pair = threadIdx.x < Tile::BM ? a.order[t.y + min((int)threadIdx.x, t.z - 1)] : 0;
+    const float2 mine = make_float2(sizeof(Y) == 4 ? a.hs[pair] : 0.0f, __builtin_bit_cast(float, pair));
     constexpr int VEC = 16 / sizeof(Y);
     const int n = n0 + Tile::template first_col<VEC>();
     const bool in = n < a.H;   // H is a multiple of 16: all columns or none
     float sd[VEC];
 #pragma unroll
     for (int k = 0; k < VEC; k++) sd[k] = sizeof(Y) == 4 && in ? a.down_s[e * a.H + n + k] : 0.0f;
+    v16i acc[Tile::MTILES][Tile::NTILES];
+    const int8_t* w = a.down + e * a.H * a.F;
+    Tile::run(a.hq + (int64_t)t.y * a.F, w, w, aoff, woff, a.F, lds, acc);
     const float unit = __builtin_ldexpf(1.0f, -a.shift);
-    Tile::template rows<VEC>(lds, acc, make_float2(hs, 0.0f), [&](int r, const int(&x)[VEC], float2 of_row) {
+    Tile::template rows<VEC>(lds, acc, mine, [&](int r, const int(&x)[VEC], float2 of_row) {
         if (r >= t.z || !in) return;
         float v[VEC];
 #pragma unroll
         for (int k = 0; k < VEC; k++)
             v[k] = sizeof(Y) == 4 ? (float)x[k] * of_row.x * sd[k] : (float)x[k] * unit;
-        store_row((Y*)a.y + (int64_t)(t.y + r) * a.H + n, v, VEC, true);
+        store_row((Y*)a.y + (int64_t)__builtin_bit_cast(int, of_row.y) * a.H + n, v, VEC, true);
     });
 }
 
+// Tiles of up to 32 pairs (four waves, four stages), or of up to 128 (eight
+// waves), whose last tile of an expert takes the code for 64 rows where that
+// holds its pairs: as many copies and matrix instructions less.
+typedef I8Tile<1, 4, 1, 1, 4> Tile32;
+typedef I8Tile<2, 4, 1, 1, 4, 2> Tile64;
+typedef I8Tile<2, 4, 2, 1, 3, 2> Tile128;
+static_assert(Tile32::BN == 128 && Tile64::BN == 128 && Tile128::BN == 128, "one grid for all");
+static_assert(Tile32::LDS == 80 << 10 && Tile64::LDS == 80 << 10 && Tile128::LDS == 80 << 10, "two work-groups per CU");
+
+// Work-group -> (tile, column block), in contiguous eighths for the XCDs, that
+// work-groups are dealt to round-robin, so that the tiles of an expert and the
+// column blocks of a tile share an L2; false: none.
+__device__ __forceinline__ bool i8_tile_of(const MoeI8& a, int blocks, int4& t, int& block) {
+    const int n = a.total[1] * blocks, per = (n + 7) / 8, at = blockIdx.x >> 3, id = (blockIdx.x & 7) * per + at;
+    if (at >= per || id >= n) return false;
+    t = a.tiles[id / blocks];
+    block = id % blocks;
+    return true;
+}
+
+template <int ROWS>
+__global__ __launch_bounds__(ROWS == 32 ? 256 : 512, ROWS == 32 ? 2 : 4) void k_i8_gate_up(MoeI8 a) {
+    __shared__ __align__(16) uint8_t lds[ROWS == 32 ? Tile32::LDS : Tile128::LDS];
+    int4 t;
+    int block;
+    if (!i8_tile_of(a, (a.F + 63) / 64, t, block)) return;
+    if constexpr (ROWS == 32) i8_gate_up<Tile32>(a, t, block * 64, lds);
+    else if (t.z <= 64) i8_gate_up<Tile64>(a, t, block * 64, lds);
+    else i8_gate_up<Tile128>(a, t, block * 64, lds);
+}
+
+template <int ROWS, typename Y>
+__global__ __launch_bounds__(ROWS == 32 ? 256 : 512, ROWS == 32 ? 2 : 4) void k_i8_down(MoeI8 a) {
+    __shared__ __align__(16) uint8_t lds[ROWS == 32 ? Tile32::LDS : Tile128::LDS];
+    int4 t;
+    int block;
+    if (!i8_tile_of(a, (a.H + 127) / 128, t, block)) return;
+    if constexpr (ROWS == 32) i8_down<Tile32, Y>(a, t, block * 128, lds);
+    else if (t.z <= 64) i8_down<Tile64, Y>(a, t, block * 128, lds);
+    else i8_down<Tile128, Y>(a, t, block * 128, lds);
+}
+
 // out[t] = sum over k, ascending, of w[t][k] y[t][k]; a pair that was left out
-// adds nothing.  A thread takes VEC neighbouring columns, four pairs' loads
-// at a time.
+// adds nothing (its row of y, not written by this call, is read but not used).
+// A thread takes VEC neighbouring columns, eight pairs' loads at a time.
 template <typename Y, typename T>
 __global__ __launch_bounds__(256) void k_i8_combine(MoeI8 a) {
-    constexpr int VEC = 16 / sizeof(Y), AT = 4;
+    constexpr int VEC = 16 / sizeof(Y), AT = 8;
     typedef Y vec __attribute__((ext_vector_type(VEC)));
-    __shared__ float w[MAX_K], hs[MAX_K];
-    __shared__ int pos[MAX_K], es[MAX_K];
     const int hb = (a.H / VEC + 255) / 256, t = blockIdx.x / hb, n = ((blockIdx.x - t * hb) * 256 + threadIdx.x) * VEC;
-    if ((int)threadIdx.x < a.K) {
-        const int64_t p = (int64_t)t * a.K + threadIdx.x;
-        const int q = a.pos[p];
-        pos[threadIdx.x] = q;
-        es[threadIdx.x] = a.ids[p];
-        w[threadIdx.x] = a.wts[p];
-        hs[threadIdx.x] = sizeof(Y) == 2 && q >= 0 ? a.hs[q] : 0.0f;
-    }
-    __syncthreads();
     if (n >= a.H) return;   // H is a multiple of 16
+    const int64_t p0 = (int64_t)t * a.K;
     const float unit = __builtin_ldexpf(1.0f, a.shift);
     float acc[VEC] = {};
     for (int k0 = 0; k0 < a.K; k0 += AT) {
         vec y[AT];
-        float sd[AT][VEC];
+        float sd[AT][VEC], w[AT], hs[AT];
+        int e[AT];
 #pragma unroll
         for (int i = 0; i < AT; i++) {
-            if (k0 + i < a.K && pos[k0 + i] >= 0) {
-                y[i] = *(const vec*)((const Y*)a.y + (int64_t)pos[k0 + i] * a.H + n);
-                if constexpr (sizeof(Y) == 2) {
+            const int64_t p = p0 + min(k0 + i, a.K - 1);
+            y[i] = *(const vec*)((const Y*)a.y + p * a.H + n);
+            e[i] = k0 + i < a.K ? a.ids[p] : -1;
+            w[i] = a.wts[p];
+            hs[i] = sizeof(Y) == 2 ? a.hs[p] : 0.0f;
+        }
 #pragma unroll
-                    for (int c = 0; c < VEC; c += 4)
-                        *(float4*)(sd[i] + c) = *(const float4*)(a.down_s + (int64_t)es[k0 + i] * a.H + n + c);
-                }
+        for (int i = 0; i < AT; i++) {
+            if (sizeof(Y) == 2 && (unsigned)e[i] < (unsigned)a.E) {
+#pragma unroll
+                for (int c = 0; c < VEC; c += 4)
+                    *(float4*)(sd[i] + c) = *(const float4*)(a.down_s + (int64_t)e[i] * a.H + n + c);
             }
         }
 #pragma unroll
         for (int i = 0; i < AT; i++) {
-            if (k0 + i < a.K && pos[k0 + i] >= 0) {
+            if ((unsigned)e[i] < (unsigned)a.E) {
 #pragma unroll
                 for (int c = 0; c < VEC; c++) {
-                    const float v = sizeof(Y) == 2 ? (float)y[i][c] * unit * hs[k0 + i] * sd[i][c] : (float)y[i][c];
-                    acc[c] = __builtin_fmaf(w[k0 + i], v, acc[c]);
+                    const float v = sizeof(Y) == 2 ? (float)y[i][c] * unit * hs[i] * sd[i][c] : (float)y[i][c];
+                    acc[c] = __builtin_fmaf(w[i], v, acc[c]);
                 }
             }
         }
@@ -349,12 +409,15 @@ __global__ __launch_bounds__(256) void k_i8_combine(MoeI8 a) {
 
 // ------------------------------------------------------------ host
 
+// Pairs up to which each is computed on its own, and pairs per expert on
+// average from which tiles hold 128 of them instead of 32 (H = 2048, F = 512,
+// 256 experts, top-8, us, tiles of 32 / 128: average 16 185 / 193, 32 215 / 211, 64
+// 283 / 250, 128 439 / 334).
 constexpr int MOE_FEW = 64;
-static int moe_tile_pairs(double avg) {
-    return avg <= 24 ? 32 : avg <= 64 ? 64 : 128;
-}
+static int moe_tile_pairs(double avg) { return avg <= 24 ? 32 : 128; }
+
 struct MoeI8Plan {
-    size_t xq, xs, order, pos, total, tiles, h, hq, hs, y, bytes;
+    size_t xq, xs, order, rank, total, cnt, tiles, h, hq, hs, y, bytes;
     int max_tiles, tile_pairs;
     bool few;
 };
@@ -373,26 +436,15 @@ static MoeI8Plan plan_moe_i8(int H, int F, int E, int K, int T) {
     take(p.xq, (size_t)T * H);
     take(p.xs, (size_t)T * 4);
     take(p.order, P * 4);
-    take(p.pos, P * 4);
+    take(p.rank, P * 4);
     take(p.total, 8);
+    take(p.cnt, (P + 1023) / 1024 * E * 4);
     // the list for the smallest tile, so that more tokens never need less
     take(p.tiles, (P / 32 + (P < (size_t)E ? P : (size_t)E)) * sizeof(int4));
     take(p.hq, P * F);
     take(p.hs, P * 4);
     take(p.y, P * H * 4);
     return p;
-}
-
-template <typename Tile, int WAVES_PER_SIMD>
-static void launch_gate_up(const MoeI8& a, int max_tiles, hipStream_t s) {
-    const int fb = (a.F + Tile::BN / 2 - 1) / (Tile::BN / 2);
-    hipLaunchKernelGGL((k_i8_gate_up<Tile, WAVES_PER_SIMD>), dim3((unsigned)(max_tiles * fb)), dim3(64 * Tile::NW), 0, s, a);
-}
-template <typename Tile, int WAVES_PER_SIMD>
-static void launch_down(const MoeI8& a, int max_tiles, bool half, hipStream_t s) {
-    const dim3 grid((unsigned)(max_tiles * ((a.H + Tile::BN - 1) / Tile::BN)));
-    if (half) hipLaunchKernelGGL((k_i8_down<Tile, WAVES_PER_SIMD, _Float16>), grid, dim3(64 * Tile::NW), 0, s, a);
-    else hipLaunchKernelGGL((k_i8_down<Tile, WAVES_PER_SIMD, float>), grid, dim3(64 * Tile::NW), 0, s, a);
 }
 
 static void launch_few_pairs(const MoeI8& a, int type, int out_type, hipStream_t s) {
@@ -406,17 +458,46 @@ static void launch_few_pairs(const MoeI8& a, int type, int out_type, hipStream_t
     else hipLaunchKernelGGL(k_i8_pair_down<__bf16>, dn, block, lh, s, a);
 }
 
+template <typename X>
+static void launch_prepare(const MoeI8& a, hipStream_t s) {
+    const int groups = (a.T * a.K + 1023) / 1024, per = i8_rows_per_group<1024>(a.H);
+    const bool wide = (((uintptr_t)a.x | (uintptr_t)(a.ldx * sizeof(X))) & 15) == 0;
+    const I8Rows<X> x{(const X*)a.x, a.ldx, a.xq, a.H, a.xs, nullptr, nullptr, a.T, a.H, wide};
+    const dim3 grid(groups + (a.T + per - 1) / per);
+    if (groups == 1) {
+        hipLaunchKernelGGL((k_i8_prepare<2, X>), grid, dim3(1024), 0, s, a, x, groups);
+    } else {
+        hipLaunchKernelGGL((k_i8_prepare<0, X>), grid, dim3(1024), 0, s, a, x, groups);
+        hipLaunchKernelGGL(k_i8_plan, dim3(groups), dim3(1024), 0, s, a, groups);
+    }
+}
+
+static void launch_hidden(const MoeI8& a, hipStream_t s) {
+    const I8Rows<float> h{a.h, a.F, a.hq, a.F, a.hs, a.order, a.total, 0, a.F, true};
+    const int per = i8_rows_per_group<256>(a.F);
+    const dim3 grid((a.T * a.K + per - 1) / per);
+    if (a.F <= I8_WAVE_ROW) hipLaunchKernelGGL(k_i8_hidden<1>, grid, dim3(256), 0, s, h);
+    else hipLaunchKernelGGL(k_i8_hidden<4>, grid, dim3(256), 0, s, h);
+}
+
 static void launch_many_pairs(const MoeI8& a, const MoeI8Plan& p, int type, int out_type, hipStream_t s) {
-    launch_i8_quantize(type, a.x, a.ldx, a.xq, a.H, a.xs, a.T, a.H, s);
-    hipLaunchKernelGGL(k_i8_plan, dim3(1), dim3(1024), 0, s, a);
-    if (p.tile_pairs == 32) launch_gate_up<I8Tile<1, 4, 1, 1, 4>, 1>(a, p.max_tiles, s);
-    else if (p.tile_pairs == 64) launch_gate_up<I8Tile<2, 4, 1, 1, 3>, 2>(a, p.max_tiles, s);
-    else launch_gate_up<I8Tile<2, 4, 2, 1, 2>, 2>(a, p.max_tiles, s);
-    launch_i8_quantize(T_F32, a.h, a.F, a.hq, a.F, a.hs, (int64_t)a.T * a.K, a.F, s);
+    if (type == T_F32) launch_prepare<float>(a, s);
+    else if (type == T_F16) launch_prepare<_Float16>(a, s);
+    else launch_prepare<__bf16>(a, s);
+    const dim3 gu((unsigned)((p.max_tiles * ((a.F + 63) / 64) + 7) / 8 * 8));
+    const dim3 dn((unsigned)((p.max_tiles * ((a.H + 127) / 128) + 7) / 8 * 8));
     const bool half = out_type != T_F32;
-    if (p.tile_pairs == 32) launch_down<I8Tile<1, 4, 1, 1, 4>, 1>(a, p.max_tiles, half, s);
-    else if (p.tile_pairs == 64) launch_down<I8Tile<2, 4, 1, 1, 3>, 2>(a, p.max_tiles, half, s);
-    else launch_down<I8Tile<2, 4, 2, 1, 2>, 2>(a, p.max_tiles, half, s);
+    if (p.tile_pairs == 32) {
+        hipLaunchKernelGGL(k_i8_gate_up<32>, gu, dim3(256), 0, s, a);
+        launch_hidden(a, s);
+        if (half) hipLaunchKernelGGL((k_i8_down<32, _Float16>), dn, dim3(256), 0, s, a);
+        else hipLaunchKernelGGL((k_i8_down<32, float>), dn, dim3(256), 0, s, a);
+    } else {
+        hipLaunchKernelGGL(k_i8_gate_up<128>, gu, dim3(512), 0, s, a);
+        launch_hidden(a, s);
+        if (half) hipLaunchKernelGGL((k_i8_down<128, _Float16>), dn, dim3(512), 0, s, a);
+        else hipLaunchKernelGGL((k_i8_down<128, float>), dn, dim3(512), 0, s, a);
+    }
     const dim3 grid((unsigned)((a.H / (half ? 8 : 4) + 255) / 256) * a.T);
     if (out_type == T_F32) hipLaunchKernelGGL((k_i8_combine<float, float>), grid, dim3(256), 0, s, a);
     else if (out_type == T_F16) hipLaunchKernelGGL((k_i8_combine<_Float16, _Float16>), grid, dim3(256), 0, s, a);
@@ -474,8 +555,8 @@ void chimere_moe_i8(const chimere_moe_i8_layer* L, int type, const void* x, int6
         launch_few_pairs(a, type, out_type, stream);
     } else {
         a.xq = (int8_t*)(w + p.xq); a.xs = (float*)(w + p.xs);
-        a.order = (int*)(w + p.order); a.pos = (int*)(w + p.pos);
-        a.total = (int*)(w + p.total); a.tiles = (int4*)(w + p.tiles);
+        a.order = (int*)(w + p.order); a.rank = (int*)(w + p.rank);
+        a.total = (int*)(w + p.total); a.cnt = (int*)(w + p.cnt); a.tiles = (int4*)(w + p.tiles);
         a.hq = (int8_t*)(w + p.hq); a.hs = (float*)(w + p.hs); a.y = w + p.y;
         a.tile_pairs = p.tile_pairs;
         while ((16256.0 * F) / (double)((int64_t)1 << a.shift) > 65504.0) a.shift++;
