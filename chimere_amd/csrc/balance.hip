@@ -360,8 +360,8 @@ static bool balance_args(const char* what, int type, const void* logits, int64_t
         set_error(CHIMERE_ERR_ARG, "%s: unsupported type %d", what, type);
     else if (E < 1 || E > MAX_E || K < 1 || K > MAX_E || T < 0 || (int64_t)T * K >= (1 << 30))
         set_error(CHIMERE_ERR_ARG, "%s: n_experts=%d top_k=%d ntok=%d out of range", what, E, K, T);
-    else if (T > 0 && (!logits || ld < 0))
-        set_error(CHIMERE_ERR_ARG, "%s: null pointer or bad stride", what);
+    else if (T > 0 && (!logits || ld < 0 || !float_aligned(type, logits)))
+        set_error(CHIMERE_ERR_ARG, "%s: null or misaligned pointer, or bad stride", what);
     else
         return true;
     return false;
@@ -396,8 +396,8 @@ void chimere_balance_loss_grad(int type, const void* logits, int64_t logits_stri
                                const int* counts, const int* tokens, const float* grad_loss, int top_k, void* grad,
                                int64_t grad_stride, int n_experts, int ntok, hipStream_t stream) {
     if (!balance_args("balance_loss_grad", type, logits, logits_stride, n_experts, top_k, ntok) || ntok == 0) return;
-    CHIMERE_REQUIRE(counts && tokens && grad_loss && grad && grad_stride >= n_experts, CHIMERE_ERR_ARG,
-                    "balance_loss_grad: null pointer or bad stride");
+    CHIMERE_REQUIRE(counts && tokens && grad_loss && grad && grad_stride >= n_experts && float_aligned(type, grad),
+                    CHIMERE_ERR_ARG, "balance_loss_grad: null or misaligned pointer, or bad stride");
     Balance b{};
     b.mask = mask; b.counts = counts; b.tokens = tokens; b.grad_loss = grad_loss;
     b.ld = logits_stride; b.ldg = grad_stride; b.E = n_experts; b.K = top_k; b.T = ntok;

@@ -100,7 +100,7 @@ __global__ __launch_bounds__(64 * FEW_WAVES) void k_i8_few(I8Gemm g) {
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int m0 = blockIdx.y * 16 * MB, n0 = blockIdx.x * 16 * NB;
     const int S = (g.C + I8_BK - 1) / I8_BK, last = (g.C + 15) / 16 - 1;
-    const int r = lane & 15, pc = (lane >> 4) * 2;
+    const int r = lane & 15, pc = lane >> 4;
     const int lda = S * I8_BK + 16;   // of the integers in LDS: rows 4 banks apart
     const int M = min(g.M - m0, 16 * MB);
     const int8_t* arow[MB];
@@ -112,7 +112,7 @@ __global__ __launch_bounds__(64 * FEW_WAVES) void k_i8_few(I8Gemm g) {
 #pragma unroll
         for (int j = 0; j < NB; j++)
 #pragma unroll
-            for (int h = 0; h < 2; h++) fw[j][h] = *(const v4i*)(wrow[j] + min(8 * s + pc + h, last) * 16);
+            for (int h = 0; h < 2; h++) fw[j][h] = *(const v4i*)(wrow[j] + min(8 * s + 4 * h + pc, last) * 16);
     };
     if (wave < S) load_w(wave);
     // the scales of this thread's outputs (`at`), ahead of all that is waited for
@@ -156,10 +156,10 @@ __global__ __launch_bounds__(64 * FEW_WAVES) void k_i8_few(I8Gemm g) {
 #pragma unroll
             for (int h = 0; h < 2; h++) {
                 if constexpr (QUANT) {
-                    fa[i][h] = *(const v4i*)(arow[i] + (8 * s + pc + h) * 16);
+                    fa[i][h] = *(const v4i*)(arow[i] + (8 * s + 4 * h + pc) * 16);
                 } else {
-                    fa[i][h] = *(const v4i*)(arow[i] + min(8 * s + pc + h, last) * 16);
-                    if ((s + 1) * I8_BK > g.C) fa[i][h] = clear_tail(fa[i][h], (8 * s + pc + h) * 16, g.C);
+                    fa[i][h] = *(const v4i*)(arow[i] + min(8 * s + 4 * h + pc, last) * 16);
+                    if ((s + 1) * I8_BK > g.C) fa[i][h] = clear_tail(fa[i][h], (8 * s + 4 * h + pc) * 16, g.C);
                 }
             }
 #pragma unroll
@@ -246,11 +246,17 @@ static void launch_gemm(const I8Gemm& g, hipStream_t s) {
     }
 }
 
-// One or two float tokens: quantized by every work-group (1x4096x2048 5.7 us
-// against 6.6 in two launches, 2x4096x2048 5.9 / 6.7, 4x4096x2048 7.3 / 6.8),
-// as long as they fit its threads' registers.
-static bool quantizes_itself(int ntok, int ncols) {
+// A few float tokens: quantized by every work-group, one launch instead of two,
+// as long as they fit its threads' registers: one or two tokens (GPU time in
+// one / two launches: 1x4096x2048 5.7 / 6.6 us, 2x4096x2048 5.9 / 6.7,
+// 1x151936x2048 51 / 55), and up to four where the work-groups are few
+// (4x4096x2048 7.3 / 6.8, but the second launch and its workspace cost the
+// calling thread another 3.8 us, of 7.1; 4x16384x2048 12.6 / 11.3).
+static bool needs_no_workspace(int ntok, int ncols) {
     return ntok <= 2 && ntok * pad_to(ncols, I8_BK) <= 64 * FEW_WAVES * FEW_KEEP;
+}
+static bool quantizes_itself(int ntok, int nrows, int ncols) {
+    return ntok <= (nrows <= FEW_N ? 4 : 2) && ntok * pad_to(ncols, I8_BK) <= 64 * FEW_WAVES * FEW_KEEP;
 }
 template <typename T, typename X>
 static void launch_few_quantizing(const I8Gemm& g, hipStream_t s) {
@@ -285,8 +291,9 @@ void chimere_quantize_i8(int type, const void* x, int64_t x_stride, int8_t* q, i
     CHIMERE_REQUIRE(x && q && scale, CHIMERE_ERR_ARG, "quantize_i8: null pointer");
     CHIMERE_REQUIRE(x_stride >= 0 && q_stride >= ncols, CHIMERE_ERR_ARG, "quantize_i8: bad strides %lld %lld",
                     (long long)x_stride, (long long)q_stride);
-    CHIMERE_REQUIRE((((uintptr_t)q | (uintptr_t)q_stride) & 15) == 0 && ((uintptr_t)scale & 3) == 0, CHIMERE_ERR_ARG,
-                    "quantize_i8: rows of q must be 16-byte aligned");
+    CHIMERE_REQUIRE((((uintptr_t)q | (uintptr_t)q_stride) & 15) == 0 && ((uintptr_t)scale & 3) == 0 &&
+                        float_aligned(type, x),
+                    CHIMERE_ERR_ARG, "quantize_i8: rows of q must be 16-byte aligned, x and scale to their elements");
     launch_i8_quantize(type, x, x_stride, q, q_stride, scale, nrows, ncols, stream);
     check_launch("quantize_i8");
 }
@@ -302,8 +309,8 @@ static bool gemm_args(const char* what, const int8_t* w, int64_t ldw, const floa
         set_error(CHIMERE_ERR_ARG, "%s: null pointer", what);
     } else if (ldw < ncols || ldw > I8_MAX_STRIDE || ldo < nrows) {
         set_error(CHIMERE_ERR_ARG, "%s: bad strides w %lld out %lld", what, (long long)ldw, (long long)ldo);
-    } else if (((uintptr_t)w | (uintptr_t)ldw) & 15) {
-        set_error(CHIMERE_ERR_ARG, "%s: rows of 8-bit integers must be 16-byte aligned", what);
+    } else if ((((uintptr_t)w | (uintptr_t)ldw) & 15) || !float_aligned(out_type, out)) {
+        set_error(CHIMERE_ERR_ARG, "%s: rows of 8-bit integers must be 16-byte aligned, out to its elements", what);
     } else if (((int64_t)ntok + 31) / 32 * (((int64_t)nrows + 15) / 16) > 0x7FFFFFFF) {
         set_error(CHIMERE_ERR_ARG, "%s: too many outputs (%d x %d)", what, ntok, nrows);
     } else {
@@ -327,7 +334,7 @@ void chimere_gemm_i8(const int8_t* a, int64_t a_stride, const float* a_scale, co
 }
 
 size_t chimere_linear_i8_workspace_size(int max_ntok, int ncols) {
-    if (max_ntok < 1 || ncols < 1 || ncols > I8_MAX_C || quantizes_itself(max_ntok, ncols)) return 0;
+    if (max_ntok < 1 || ncols < 1 || ncols > I8_MAX_C || needs_no_workspace(max_ntok, ncols)) return 0;
     return al256((size_t)max_ntok * pad_to(ncols, 16)) + al256((size_t)max_ntok * 4);
 }
 
@@ -338,14 +345,15 @@ void chimere_linear_i8(int type, const void* x, int64_t x_stride, const int8_t* 
     if (!gemm_args("linear_i8", w, w_stride, w_scale, out_type, out, out_stride, ntok, nrows, ncols) || ntok == 0) return;
     const size_t need = chimere_linear_i8_workspace_size(ntok, ncols);
     CHIMERE_REQUIRE(x && (workspace || !need), CHIMERE_ERR_ARG, "linear_i8: null pointer");
-    CHIMERE_REQUIRE(x_stride >= 0, CHIMERE_ERR_ARG, "linear_i8: bad stride %lld", (long long)x_stride);
+    CHIMERE_REQUIRE(x_stride >= 0 && float_aligned(type, x), CHIMERE_ERR_ARG,
+                    "linear_i8: bad stride %lld, or x not aligned to its elements", (long long)x_stride);
     CHIMERE_REQUIRE(workspace_bytes >= need && ((uintptr_t)workspace & 255) == 0, CHIMERE_ERR_WORKSPACE,
                     "linear_i8: workspace %zu bytes < %zu (or not 256-byte aligned)", workspace_bytes, need);
     const int64_t lda = pad_to(ncols, 16);
     int8_t* q = (int8_t*)workspace;
     float* as = (float*)((uint8_t*)workspace + al256((size_t)ntok * lda));
     const I8Gemm g{q, w, as, w_scale, bias, out, lda, w_stride, out_stride, ntok, nrows, ncols, x, x_stride};
-    if (quantizes_itself(ntok, ncols)) {
+    if (quantizes_itself(ntok, nrows, ncols)) {
         if (out_type == T_F32) launch_few_quantizing<float>(type, g, stream);
         else if (out_type == T_F16) launch_few_quantizing<_Float16>(type, g, stream);
         else launch_few_quantizing<__bf16>(type, g, stream);

@@ -1,14 +1,21 @@
 // int8_quant.h -- rows of floats as 8-bit integers with one scale: scale =
-// max |x| / 127, q = x / scale rounded to the nearest integer, ties to even
-// (IEEE divisions).
+// max |x| times 1/127 (its f32 value: what torch computes for a division by
+// the number 127, so that rows quantized there have the same scales), q =
+// x / scale (IEEE) rounded to the nearest integer, ties to even.
 #pragma once
 #include "float_rows.h"
 
 namespace chimere {
 
-// the integer of x in a row of scale d
+// a row's scale from its max |x| as bits
+__device__ __forceinline__ float i8_scale(uint32_t amax) {
+    return __builtin_bit_cast(float, amax) * (1.0f / 127.0f);
+}
+// the integer of x in a row of scale d (held to +-127: a subnormal scale can be
+// rounded down by up to a third)
 __device__ __forceinline__ int i8_quant(float x, float d) {
-    return d > 0.0f && d < __builtin_huge_valf() ? (int)__builtin_rintf(x / d) : 0;
+    const float q = __builtin_fminf(__builtin_fmaxf(__builtin_rintf(x / d), -127.0f), 127.0f);
+    return d > 0.0f && d < __builtin_huge_valf() ? (int)q : 0;
 }
 
 // N integers packed into bytes
@@ -81,7 +88,7 @@ __device__ __forceinline__ void i8_rows_to_lds(int M, int cols, int lda, float* 
         }
     }
     __syncthreads();
-    for (int m = tid; m < M; m += THREADS) as[m] = __builtin_bit_cast(float, bits[m]) / 127.0f;
+    for (int m = tid; m < M; m += THREADS) as[m] = i8_scale(bits[m]);
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < KEEP / V; i++) {
@@ -148,7 +155,7 @@ __device__ __forceinline__ void i8_quantize_rows(const I8Rows<T>& g, int64_t gro
         m = max(max(p[0], p[1]), max(p[2], p[3]));
         if (!on) return;
     }
-    const float d = __builtin_bit_cast(float, m) / 127.0f;
+    const float d = i8_scale(m);
     if (c0 == 0) g.scale[g.to ? g.to[r] : r] = d;
     int8_t* to = g.q + r * g.qs;
     auto put = [&](int c, const float(&u)[V]) {

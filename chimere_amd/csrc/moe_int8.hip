@@ -57,13 +57,13 @@ __global__ __launch_bounds__(64 * FP_WAVES) void k_i8_pair_gate_up(MoeI8 a) {
     const int p = blockIdx.y, e = a.ids[p], t = p / a.K, f0 = blockIdx.x * 16;
     if ((unsigned)e >= (unsigned)a.E) return;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int S = (a.H + I8_BK - 1) / I8_BK, last = a.H / 16 - 1, r = lane & 15, pc = (lane >> 4) * 2;
+    const int S = (a.H + I8_BK - 1) / I8_BK, last = a.H / 16 - 1, r = lane & 15, pc = lane >> 4;
     const int64_t row = ((int64_t)e * a.F + f0 + r) * a.H;   // F is a multiple of 16
     v4i w[2][2];
     auto load_w = [&](int s) {
 #pragma unroll
         for (int h = 0; h < 2; h++) {
-            const int at = min(8 * s + pc + h, last) * 16;
+            const int at = min(8 * s + 4 * h + pc, last) * 16;
             w[0][h] = *(const v4i*)(a.gate + row + at);
             w[1][h] = *(const v4i*)(a.up + row + at);
         }
@@ -89,7 +89,7 @@ __global__ __launch_bounds__(64 * FP_WAVES) void k_i8_pair_gate_up(MoeI8 a) {
         if (s + FP_WAVES < S) load_w(s + FP_WAVES);
 #pragma unroll
         for (int h = 0; h < 2; h++) {
-            const v4i f = *(const v4i*)(xq + (8 * s + pc + h) * 16);   // 0 behind H
+            const v4i f = *(const v4i*)(xq + (8 * s + 4 * h + pc) * 16);   // 0 behind H
             g = __builtin_amdgcn_mfma_i32_16x16x64_i8(f, now[0][h], g, 0, 0, 0);
             u = __builtin_amdgcn_mfma_i32_16x16x64_i8(f, now[1][h], u, 0, 0, 0);
         }
@@ -120,14 +120,14 @@ __global__ __launch_bounds__(64 * FP_WAVES) void k_i8_pair_down(MoeI8 a) {
     __shared__ int sum[MAX_K][16];
     const int t = blockIdx.y, n0 = blockIdx.x * 16;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int S = (a.F + I8_BK - 1) / I8_BK, last = a.F / 16 - 1, r = lane & 15, pc = (lane >> 4) * 2;
+    const int S = (a.F + I8_BK - 1) / I8_BK, last = a.F / 16 - 1, r = lane & 15, pc = lane >> 4;
     const int* ids = a.ids + (int64_t)t * a.K;
     v4i w[FP_AHEAD][2];
     auto load_w = [&](int u, v4i(&to)[2]) {
         const int k = u / S, s = u - k * S, e = ids[k];
         const int8_t* row = a.down + ((int64_t)((unsigned)e < (unsigned)a.E ? e : 0) * a.H + n0 + r) * a.F;
 #pragma unroll
-        for (int h = 0; h < 2; h++) to[h] = *(const v4i*)(row + min(8 * s + pc + h, last) * 16);
+        for (int h = 0; h < 2; h++) to[h] = *(const v4i*)(row + min(8 * s + 4 * h + pc, last) * 16);
     };
 #pragma unroll
     for (int i = 0; i < FP_AHEAD; i++)
@@ -149,7 +149,7 @@ __global__ __launch_bounds__(64 * FP_WAVES) void k_i8_pair_down(MoeI8 a) {
         v4i acc = {};
 #pragma unroll
         for (int h = 0; h < 2; h++)
-            acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(*(const v4i*)(lds + k * lda + (8 * s + pc + h) * 16), now[h],
+            acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(*(const v4i*)(lds + k * lda + (8 * s + 4 * h + pc) * 16), now[h],
                                                         acc, 0, 0, 0);
         if (lane < 16) atomicAdd(&sum[k][lane], acc[0]);   // integers: any order
     };
@@ -538,7 +538,8 @@ void chimere_moe_i8(const chimere_moe_i8_layer* L, int type, const void* x, int6
                     "moe_i8: weights and scales must be 16-byte aligned");
     if (ntok == 0) return;
     CHIMERE_REQUIRE(x && ids && weights && out && workspace, CHIMERE_ERR_ARG, "moe_i8: null pointer");
-    CHIMERE_REQUIRE(x_stride >= 0 && out_stride >= L->hidden, CHIMERE_ERR_ARG, "moe_i8: bad strides %lld %lld",
+    CHIMERE_REQUIRE(x_stride >= 0 && out_stride >= L->hidden && float_aligned(type, x) && float_aligned(out_type, out),
+                    CHIMERE_ERR_ARG, "moe_i8: bad strides %lld %lld, or rows not aligned to their elements",
                     (long long)x_stride, (long long)out_stride);
     const int H = L->hidden, F = L->ffn;
     const MoeI8Plan p = plan_moe_i8(H, F, L->n_experts, top_k, ntok);

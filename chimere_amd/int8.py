@@ -12,7 +12,8 @@ holds one layer's routed experts in this format.
 Tensors lie on one ROCm device; launches go to that device's current torch
 stream, scratch comes from torch's allocator on it.  Rows of 8-bit integers
 start 16-byte aligned: ``quantize_i8`` makes them so (a view of padded rows
-where ncols is no multiple of 16).  A rejected call raises ``ChimereError``
+where ncols is no multiple of 16).  Nothing is recorded for autograd: these
+are the products of a server.  A rejected call raises ``ChimereError``
 (the library's checks) or ``ValueError`` (types, shapes, devices).
 """
 import ctypes as C
@@ -94,7 +95,7 @@ def _bias(bias, n):
 
 def quantize_i8(x, q=None, scale=None):
     """x [rows, ncols] -> (q int8 [rows, ncols], scale float32 [rows]), x ~ q * scale: scale = max |x| / 127 of the
-    row, ties to even.  For tokens and for weights (rows = output channels)."""
+    row (as torch divides by a number: times 1/127), ties to even.  For tokens and for weights (rows = output channels)."""
     n, c, ld = rows_of(x, "x")
     if q is None:
         q = torch.empty(n, (c + 15) // 16 * 16, dtype=torch.int8, device=x.device)[:, :c]

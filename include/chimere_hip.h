@@ -292,10 +292,11 @@ void chimere_fused_moe_iq3s(const float *hidden, const void *gate_exps, const vo
  * stride, in bytes), and what lies between their ncols integers and the next
  * multiple of 16 is read but does not matter.  Outputs may not overlap
  * inputs.  ntok = 0 launches nothing.  Sums of products are exact (int32), so
- * results repeat bit for bit and do not depend on ntok. */
+ * results repeat bit for bit; a token's f32 results do not depend on ntok. */
 
-/* scale[r] = max |x[r]| / 127, q[r][c] = x[r][c] / scale[r] rounded to the
- * nearest integer, ties to even (0 where the scale is 0).  A row that holds
+/* scale[r] = max |x[r]| * (1 / 127 as f32; torch's max / 127), q[r][c] =
+ * x[r][c] / scale[r] rounded to the nearest integer, ties to even, and held
+ * to +-127 (0 where the scale is 0).  A row that holds
  * an infinity or a NaN gets it as scale, and zeros.  Only the ncols integers
  * of a row are written.  For tokens and for weights (rows = channels). */
 void chimere_quantize_i8(int type, const void *x, int64_t x_stride, int8_t *q, int64_t q_stride,

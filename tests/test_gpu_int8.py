@@ -35,8 +35,8 @@ def q_ref(x):
     x = x.detach().float().cpu().numpy()
     bits = (x.view(np.uint32) & 0x7FFFFFFF).max(1)
     with np.errstate(all="ignore"):
-        scale = bits.view(np.float32) / np.float32(127)
-        q = np.rint(x / scale[:, None])
+        scale = bits.view(np.float32) * (np.float32(1) / np.float32(127))
+        q = np.rint(x / scale[:, None]).clip(-127, 127)
     q[~((scale > 0) & np.isfinite(scale))] = 0
     return torch.from_numpy(q.astype(np.float64)), torch.from_numpy(scale.astype(np.float64))
 
@@ -85,7 +85,7 @@ def test_quantize_borders(dev, c):
     half[0, 0] = 127.0
     rows = [half, half * 3, half / 7, half * 2.0 ** -149, half * 2.0 ** -140, half * 2.0 ** -120, half * 2.0 ** 120,
             torch.nextafter(half, torch.zeros_like(half)), torch.nextafter(half * 0.37, half * 1e3),
-            torch.zeros(1, c, device=dev), -torch.zeros(1, c, device=dev)]
+            half * 1.5 * 2.0 ** -149, half * 2.3 * 2.0 ** -149, torch.zeros(1, c, device=dev), -torch.zeros(1, c, device=dev)]
     x = torch.cat(rows)
     for bad in (float("inf"), -float("inf"), float("nan")):
         r = torch.randn(1, c, generator=g, device=dev)
@@ -95,6 +95,19 @@ def test_quantize_borders(dev, c):
     rq, rs = q_ref(x)
     assert ((s.double().cpu() == rs) | (s.double().cpu().isnan() & rs.isnan())).all()
     assert (q.double().cpu() == rq).all()
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+def test_quantize_many_ties(dev, dtype):
+    """Rows whose largest value is a multiple of 127 in its last places, so that every other one is a tie; scales as torch's."""
+    g = gen(1)
+    x = torch.randint(-254, 255, (200, 300), generator=g, device=dev)
+    x[:, 0] = 254
+    x = (x.float() * 2.0 ** torch.randint(-8, 5, (200, 1), generator=g, device=dev)).to(TYPES[dtype])
+    q, s = int8.quantize_i8(x)
+    rq, rs = q_ref(x)
+    assert (s.double().cpu() == rs).all() and (q.double().cpu() == rq).all()
+    assert (s == x.float().abs().amax(1) / 127).all()
 
 
 def test_quantize_strides_and_what_is_left(dev):
@@ -162,7 +175,7 @@ def test_gemm_strides_and_what_is_left(dev, m, n, c):
 
 
 @pytest.mark.parametrize("xt", TYPES)
-@pytest.mark.parametrize("m,n,c", [(1, 4096, 2048), (1, 5, 1), (1, 1000, 4097), (2, 70, 300), (3, 1000, 2048), (8, 513, 1024), (12, 100, 9000),
+@pytest.mark.parametrize("m,n,c", [(1, 4096, 2048), (1, 5, 1), (1, 1000, 4097), (2, 70, 300), (3, 1000, 2048), (8, 513, 1024), (12, 100, 9000), (4, 8192, 2048), (4, 500, 2049), (3, 8200, 512), (2, 9001, 4000), (1, 8193, 8192), (1, 40, 8193),
                                    (40, 300, 500), (300, 500, 129)])
 def test_linear(dev, m, n, c, xt):
     print(f"linear {m}x{n}x{c} {xt}", flush=True)

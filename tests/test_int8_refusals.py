@@ -30,7 +30,7 @@ def test_quantize():
     good = [0, P, 64, P, 64, P, 4, 64, None]
     refuses("chimere_quantize_i8", good, type=(0, 2, 1), x=(1, None, 1), q=(3, None, 1), scale=(5, None, 1), rows=(6, -1, 1),
             cols=(7, 0, 1), x_stride=(2, -1, 1), q_short=(4, 48, 1), q_stride=(4, 72, 1), q_ptr=(3, ODD, 1),
-            too_many=(6, 1 << 31, 1))
+            too_many=(6, 1 << 31, 1), x_align=(1, C.c_void_p(0x1002), 1))
     good[6] = 0
     _lib.lib().chimere_quantize_i8(*good)           # no rows: nothing to do
     assert err()[0] == 0
@@ -40,7 +40,8 @@ def test_gemm():
     good = [P, 64, P, P, 64, P, None, 0, P, 32, 4, 32, 64, None]
     refuses("chimere_gemm_i8", good, a=(0, None, 1), lda=(1, 48, 1), lda_align=(1, 72, 1), a_align=(0, ODD, 1), a_scale=(2, None, 1),
             w=(3, None, 1), w_align=(3, ODD, 1), ldw=(4, 63, 1), ldw_far=(4, 1 << 24, 1), w_scale=(5, None, 1), type=(7, 8, 1),
-            out=(8, None, 1), ldo=(9, 31, 1), ntok=(10, -1, 1), nrows=(11, 0, 1), ncols=(12, 0, 1), long=(12, 131072, 1))
+            out=(8, None, 1), ldo=(9, 31, 1), ntok=(10, -1, 1), nrows=(11, 0, 1), ncols=(12, 0, 1), long=(12, 131072, 1),
+            out_align=(8, C.c_void_p(0x1002), 1))
     good[10] = 0
     _lib.lib().chimere_gemm_i8(*good)
     assert err()[0] == 0
@@ -87,10 +88,10 @@ def test_balance():
     assert need > 0 == L.chimere_balance_loss_workspace_size(1025, 10)
     good = [0, P, 256, P, 8, None, P, P, P, P, 256, 1000, P, need, None]
     refuses("chimere_balance_loss", good, type=(0, 8, 1), logits=(1, None, 1), stride=(2, -1, 1), ids=(3, None, 1), k=(4, 0, 1),
-            loss=(6, None, 1), probs=(7, None, 1), counts=(8, None, 1), tokens=(9, None, 1), many=(10, 1025, 1), none=(10, 0, 1),
+            loss=(6, None, 1), probs=(7, None, 1), counts=(8, None, 1), tokens=(9, None, 1), many=(10, 1025, 1), none=(10, 0, 1), far=(11, 1 << 30, 1), wide=(4, 1025, 1),
             ntok=(11, -1, 1), ws=(12, None, 1), ws_align=(12, ODD, 3), ws_small=(13, need - 1, 3))
     good = [0, P, 256, None, P, P, P, 8, P, 256, 256, 1000, None]
-    refuses("chimere_balance_loss_grad", good, type=(0, 2, 1), logits=(1, None, 1), counts=(4, None, 1), tokens=(5, None, 1),
+    refuses("chimere_balance_loss_grad", good, align=(1, C.c_void_p(0x1002), 1), grad_align=(8, C.c_void_p(0x1001), 1), type=(0, 2, 1), logits=(1, None, 1), counts=(4, None, 1), tokens=(5, None, 1),
             grad_loss=(6, None, 1), k=(7, 0, 1), grad=(8, None, 1), ldg=(9, 255, 1), many=(10, 2000, 1), ntok=(11, -1, 1))
     good[11] = 0
     L.chimere_balance_loss_grad(*good)
