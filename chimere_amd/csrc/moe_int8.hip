@@ -9,6 +9,8 @@
 // down and the weighted sum.  More: rows of x to 8 bits; the pairs of each
 // expert together, with the list of tiles; gate and up product with
 // h = silu(g) u; rows of h to 8 bits; down product; each token's weighted sum.
+#include <math.h>
+
 #include <type_traits>
 
 #include "api_internal.h"
@@ -110,34 +112,40 @@ __global__ __launch_bounds__(64 * FP_WAVES) void k_i8_pair_gate_up(MoeI8 a) {
     }
 }
 
-// Grid (H / 16, T): 16 columns of H of one token.  The token's rows of h to 8
-// bits in LDS; the (k, step of 128 columns of F) pieces dealt to the eight
+// Grid (H / COLS, T): 16 or 8 columns of H of one token.  The token's rows of h
+// to 8 bits in LDS; the (k, step of 128 columns of F) pieces dealt to the eight
 // waves, whose sums meet in LDS integers; the weighted sum in ascending k.
-template <typename T>
+// With 8 columns a matrix instruction takes two pieces, one in rows 0 .. 7 of
+// the weights and row 0 of h, one in rows 8 .. 15 and row 1: twice the
+// work-groups, where 16 columns would leave half of the CUs idle (one token
+// of H = 2048: 7.3 us with 16, 6.6 with 8).
+template <typename T, int COLS>
 __global__ __launch_bounds__(64 * FP_WAVES) void k_i8_pair_down(MoeI8 a) {
+    constexpr int PER = 16 / COLS;                   // pieces per instruction
     extern __shared__ __align__(16) uint8_t lds[];   // integers of h
-    __shared__ float hs[MAX_K], y[MAX_K][16];
-    __shared__ int sum[MAX_K][16];
-    const int t = blockIdx.y, n0 = blockIdx.x * 16;
+    __shared__ float hs[MAX_K], wk[MAX_K], y[MAX_K][COLS];
+    __shared__ int sum[MAX_K][COLS];
+    const int t = blockIdx.y, n0 = blockIdx.x * COLS;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int S = (a.F + I8_BK - 1) / I8_BK, last = a.F / 16 - 1, r = lane & 15, pc = lane >> 4;
+    const int pieces = a.K * S, n = (pieces + PER - 1) / PER;
     const int* ids = a.ids + (int64_t)t * a.K;
     v4i w[FP_AHEAD][2];
     auto load_w = [&](int u, v4i(&to)[2]) {
-        const int k = u / S, s = u - k * S, e = ids[k];
-        const int8_t* row = a.down + ((int64_t)((unsigned)e < (unsigned)a.E ? e : 0) * a.H + n0 + r) * a.F;
+        const int at = min(u * PER + r / COLS, pieces - 1), k = at / S, s = at - k * S, e = ids[k];
+        const int8_t* row = a.down + ((int64_t)((unsigned)e < (unsigned)a.E ? e : 0) * a.H + n0 + r % COLS) * a.F;
 #pragma unroll
         for (int h = 0; h < 2; h++) to[h] = *(const v4i*)(row + min(8 * s + 4 * h + pc, last) * 16);
     };
 #pragma unroll
     for (int i = 0; i < FP_AHEAD; i++)
-        if (wave + i * FP_WAVES < a.K * S) load_w(wave + i * FP_WAVES, w[i]);
+        if (wave + i * FP_WAVES < n) load_w(wave + i * FP_WAVES, w[i]);
     // thread -> (k, column): its scale and weight, ahead of all that is waited for
-    const int mk = tid >> 4, mc = tid & 15, me = mk < a.K ? ids[mk] : -1;
+    const int mk = tid / COLS, mc = tid % COLS, me = mk < a.K ? ids[mk] : -1;
     const bool mine = (unsigned)me < (unsigned)a.E;
     const float sd = mine ? a.down_s[(int64_t)me * a.H + n0 + mc] : 0.0f;
-    const float wk = mine ? a.wts[(int64_t)t * a.K + mk] : 0.0f;
-    if (tid < MAX_K * 16) (&sum[0][0])[tid] = 0;
+    const float wt = mine ? a.wts[(int64_t)t * a.K + mk] : 0.0f;
+    if (tid < MAX_K * COLS) (&sum[0][0])[tid] = 0;
     // (a pair that was left out: whatever its row holds, its sums are not used)
     const int lda = S * I8_BK;
     i8_rows_to_lds<64 * FP_WAVES, FP_KEEP>(
@@ -145,29 +153,32 @@ __global__ __launch_bounds__(64 * FP_WAVES) void k_i8_pair_down(MoeI8 a) {
         [&](int k, int c, auto& v) { i8_load(a.h + ((int64_t)t * a.K + k) * a.F, c, a.F, true, v); },
         std::integral_constant<int, 4>{});
     auto piece = [&](int u, const v4i(&now)[2]) {
-        const int k = u / S, s = u - k * S;
+        const int mine_at = min(u * PER + (r & (PER - 1)), pieces - 1), mk_ = mine_at / S, ms = mine_at - mk_ * S;
         v4i acc = {};
 #pragma unroll
         for (int h = 0; h < 2; h++)
-            acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(*(const v4i*)(lds + k * lda + (8 * s + 4 * h + pc) * 16), now[h],
-                                                        acc, 0, 0, 0);
-        if (lane < 16) atomicAdd(&sum[k][lane], acc[0]);   // integers: any order
+            acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(*(const v4i*)(lds + mk_ * lda + (8 * ms + 4 * h + pc) * 16),
+                                                        now[h], acc, 0, 0, 0);
+        // lane r < 16 holds column r of every row; its weights' piece is row r / COLS
+        const int at = u * PER + r / COLS;
+        if (lane < 16 && at < pieces) atomicAdd(&sum[at / S][r % COLS], PER == 2 && r >= COLS ? acc[1] : acc[0]);
     };
 #pragma unroll
     for (int i = 0; i < FP_AHEAD; i++)
-        if (wave + i * FP_WAVES < a.K * S) piece(wave + i * FP_WAVES, w[i]);
-    for (int u = wave + FP_AHEAD * FP_WAVES; u < a.K * S; u += FP_WAVES) {
+        if (wave + i * FP_WAVES < n) piece(wave + i * FP_WAVES, w[i]);
+    for (int u = wave + FP_AHEAD * FP_WAVES; u < n; u += FP_WAVES) {
         load_w(u, w[0]);
         piece(u, w[0]);
     }
     __syncthreads();
-    // a pair that was left out: 0 times 0
-    if (mk < a.K) y[mk][mc] = mine ? (float)sum[mk][mc] * hs[mk] * sd : 0.0f;
-    if (mk < MAX_K && mc == 0) hs[mk] = wk;
+    if (mk < a.K) {
+        y[mk][mc] = mine ? (float)sum[mk][mc] * hs[mk] * sd : 0.0f;   // a pair that was left out: 0 times 0
+        if (mc == 0) wk[mk] = wt;
+    }
     __syncthreads();
-    if (tid < 16) {
+    if (tid < COLS) {
         float acc = 0.0f;
-        for (int k = 0; k < a.K; k++) acc = __builtin_fmaf(hs[k], y[k][tid], acc);
+        for (int k = 0; k < a.K; k++) acc = __builtin_fmaf(wk[k], y[k][tid], acc);
         store_f((T*)a.out + t * a.ldo + n0 + tid, acc);
     }
 }
@@ -409,11 +420,25 @@ __global__ __launch_bounds__(256) void k_i8_combine(MoeI8 a) {
 
 // ------------------------------------------------------------ host
 
-// Pairs up to which each is computed on its own, and pairs per expert on
-// average from which tiles hold 128 of them instead of 32 (H = 2048, F = 512,
-// 256 experts, top-8, us, tiles of 32 / 128: average 16 185 / 193, 32 215 / 211, 64
-// 283 / 250, 128 439 / 334).
-constexpr int MOE_FEW = 64;
+// Whether each pair is computed on its own: two launches read an expert's
+// weights again for every pair of it, five read them once; the three more are
+// worth about 50 MB.  Pairs that meet an expert again, by even routing, are P -
+// E (1 - (1 - 1/E)^P).  Together / on its own, us (H, F, E, K; tokens):
+//   2048, 512, 256, 8    1 24.5 / 13.1   4 32 / 24   8 42 / 40   16 60 / 73
+//   2048, 512, 8, 2      4 22 / 12.6     8 22 / 16   16 21 / 26  64 23 / 86
+//   1024, 1024, 64, 4    4 25 / 18       8 30 / 24   16 37 / 40
+//   4096, 2048, 8, 1     4 30 / 29       8 35 / 50
+constexpr double MOE_AGAIN = 50e6;
+constexpr int MOE_PAIRS = 512;   // the most that were measured
+static bool moe_few(int H, int F, int E, int K, int64_t P) {
+    const double again = P - E * (1.0 - pow(1.0 - 1.0 / E, (double)P));
+    // rows that fit the work-groups' registers
+    return P <= MOE_PAIRS && again * 3.0 * H * F <= MOE_AGAIN && pad_to(H, I8_BK) <= 64 * FP_WAVES * FP_KEEP &&
+           K * pad_to(F, I8_BK) <= 64 * FP_WAVES * FP_KEEP;
+}
+// Pairs per tile: 128 instead of 32 where an expert meets more than 24 on
+// average (H = 2048, F = 512, 256 experts, top-8, us, tiles of 32 / 128: average
+// 16 185 / 193, 32 215 / 211, 64 283 / 250, 128 439 / 334).
 static int moe_tile_pairs(double avg) { return avg <= 24 ? 32 : 128; }
 
 struct MoeI8Plan {
@@ -425,9 +450,7 @@ struct MoeI8Plan {
 static MoeI8Plan plan_moe_i8(int H, int F, int E, int K, int T) {
     MoeI8Plan p{};
     const size_t P = (size_t)T * K;
-    // a few pairs, whose rows fit the work-groups' registers
-    p.few = P <= MOE_FEW && pad_to(H, I8_BK) <= 64 * FP_WAVES * FP_KEEP &&
-            K * pad_to(F, I8_BK) <= 64 * FP_WAVES * FP_KEEP;
+    p.few = moe_few(H, F, E, K, (int64_t)P);
     auto take = [&](size_t& at, size_t n) { at = p.bytes; p.bytes += al256(n); };
     take(p.h, P * F * 4);
     if (p.few) return p;
@@ -447,15 +470,23 @@ static MoeI8Plan plan_moe_i8(int H, int F, int E, int K, int T) {
     return p;
 }
 
+template <int COLS>
+static void launch_pair_down(const MoeI8& a, int out_type, hipStream_t s) {
+    const dim3 grid(a.H / COLS, a.T), block(64 * FP_WAVES);
+    const size_t lh = a.K * pad_to(a.F, I8_BK);
+    if (out_type == T_F32) hipLaunchKernelGGL((k_i8_pair_down<float, COLS>), grid, block, lh, s, a);
+    else if (out_type == T_F16) hipLaunchKernelGGL((k_i8_pair_down<_Float16, COLS>), grid, block, lh, s, a);
+    else hipLaunchKernelGGL((k_i8_pair_down<__bf16, COLS>), grid, block, lh, s, a);
+}
+
 static void launch_few_pairs(const MoeI8& a, int type, int out_type, hipStream_t s) {
-    const dim3 gu(a.F / 16, a.T * a.K), dn(a.H / 16, a.T), block(64 * FP_WAVES);
-    const size_t lx = 16 + pad_to(a.H, I8_BK), lh = a.K * pad_to(a.F, I8_BK);
+    const dim3 gu(a.F / 16, a.T * a.K), block(64 * FP_WAVES);
+    const size_t lx = 16 + pad_to(a.H, I8_BK);
     if (type == T_F32) hipLaunchKernelGGL(k_i8_pair_gate_up<float>, gu, block, lx, s, a);
     else if (type == T_F16) hipLaunchKernelGGL(k_i8_pair_gate_up<_Float16>, gu, block, lx, s, a);
     else hipLaunchKernelGGL(k_i8_pair_gate_up<__bf16>, gu, block, lx, s, a);
-    if (out_type == T_F32) hipLaunchKernelGGL(k_i8_pair_down<float>, dn, block, lh, s, a);
-    else if (out_type == T_F16) hipLaunchKernelGGL(k_i8_pair_down<_Float16>, dn, block, lh, s, a);
-    else hipLaunchKernelGGL(k_i8_pair_down<__bf16>, dn, block, lh, s, a);
+    if (a.T * (a.H / 16) <= 256) launch_pair_down<8>(a, out_type, s);
+    else launch_pair_down<16>(a, out_type, s);
 }
 
 template <typename X>
