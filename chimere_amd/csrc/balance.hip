@@ -24,19 +24,6 @@ struct Balance {
     bool wide;       // rows of logits (and grad) start on multiples of four elements
 };
 
-// e^x for x <= 0 (x a difference from the maximum): 2^(x log2 e) by the
-// hardware's exponential, with what the product x log2 e is off by (exactly
-// known from the fma, log2 e in two parts) put right to first order: about 2
-// units in the last place, at half of det_exp's instructions, and the sums over
-// rows are bound by these.  Below e^-86 it comes to 0.
-__device__ __forceinline__ float bal_exp(float x) {
-    constexpr float HI = 0x1.715476p+0f, LO = 0x1.4ae0cp-26f, LN2 = 0x1.62e430p-1f;
-    x = x < -120.0f ? -120.0f : x;   // (not a maximum: a NaN stays)
-    const float t = x * HI, off = __builtin_fmaf(x, LO, __builtin_fmaf(x, HI, -t));
-    const float e = __builtin_amdgcn_exp2f(t);
-    return __builtin_fmaf(e, off * LN2, e);
-}
-
 // Sixteen lanes per row, lane l of them the columns 64 i + 4 l .. + 3 for
 // i < NV: a row of E = 256 is four loads of 16 bytes per lane, and the sums
 // over a row are four DPP steps for four rows at once (one wave per row: six
@@ -81,7 +68,7 @@ struct BalRow {
 #pragma unroll
         for (int i = 0; i < NV; i++) {
 #pragma unroll
-            for (int k = 0; k < 4; k++) v[4 * i + k] = bal_exp(v[4 * i + k] - from);
+            for (int k = 0; k < 4; k++) v[4 * i + k] = fast_exp(v[4 * i + k] - from);
             s += (v[4 * i] + v[4 * i + 1]) + (v[4 * i + 2] + v[4 * i + 3]);
         }
         s = slot_reduce16(s);

@@ -19,4 +19,23 @@ __device__ __forceinline__ void store_f(float* p, float v) { *p = v; }
 __device__ __forceinline__ void store_f(_Float16* p, float v) { *p = (_Float16)v; }
 __device__ __forceinline__ void store_f(__bf16* p, float v) { *p = (__bf16)v; }
 
+// e^x for x <= 88: 2^(x log2 e) by the hardware's exponential, with what the
+// product x log2 e is off by (known exactly from the fma, log2 e in two parts)
+// put right to first order: about 2 units in the last place, at half of
+// det_exp's instructions, for sums and tiles that are bound by these.  Below
+// e^-87 it comes to 0; a NaN stays one.
+__device__ __forceinline__ float fast_exp(float x) {
+    constexpr float HI = 0x1.715476p+0f, LO = 0x1.4ae0cp-26f, LN2 = 0x1.62e430p-1f;
+    x = x < -120.0f ? -120.0f : x;   // (not a maximum: a NaN stays)
+    const float t = x * HI, off = __builtin_fmaf(x, LO, __builtin_fmaf(x, HI, -t));
+    const float e = __builtin_amdgcn_exp2f(t);
+    return __builtin_fmaf(e, off * LN2, e);
+}
+// g / (1 + e^-g) with the hardware's reciprocal (1 unit in the last place); 0
+// where e^-g leaves f32's range, as det_silu
+__device__ __forceinline__ float fast_silu(float g) {
+    const float e = -g > 88.0f ? __builtin_huge_valf() : fast_exp(-g);
+    return g * __builtin_amdgcn_rcpf(1.0f + e);
+}
+
 }  // namespace chimere

@@ -108,7 +108,7 @@ __global__ __launch_bounds__(64 * FP_WAVES) void k_i8_pair_gate_up(MoeI8 a) {
             gs += part[i][0][tid];
             us += part[i][1][tid];
         }
-        a.h[(int64_t)p * a.F + f0 + tid] = det_silu((float)gs * *xs * sg) * ((float)us * *xs * su);
+        a.h[(int64_t)p * a.F + f0 + tid] = fast_silu((float)gs * *xs * sg) * ((float)us * *xs * su);
     }
 }
 
@@ -278,10 +278,10 @@ __device__ __forceinline__ void i8_gate_up(const MoeI8& a, const int4& t, int f0
         if (r >= t.z || !in) return;
         const float s = of_row.x;
         float4 h;
-        h.x = det_silu((float)g[0] * s * sg.x) * ((float)u[0] * s * su.x);
-        h.y = det_silu((float)g[1] * s * sg.y) * ((float)u[1] * s * su.y);
-        h.z = det_silu((float)g[2] * s * sg.z) * ((float)u[2] * s * su.z);
-        h.w = det_silu((float)g[3] * s * sg.w) * ((float)u[3] * s * su.w);
+        h.x = fast_silu((float)g[0] * s * sg.x) * ((float)u[0] * s * su.x);
+        h.y = fast_silu((float)g[1] * s * sg.y) * ((float)u[1] * s * su.y);
+        h.z = fast_silu((float)g[2] * s * sg.z) * ((float)u[2] * s * su.z);
+        h.w = fast_silu((float)g[3] * s * sg.w) * ((float)u[3] * s * su.w);
         *(float4*)(a.h + (int64_t)(t.y + r) * a.F + f) = h;
     });
 }
@@ -324,14 +324,32 @@ __device__ __forceinline__ void i8_down(const MoeI8& a, const int4& t, int n0, u
     });
 }
 
-// Tiles of up to 32 pairs (four waves, four stages), or of up to 128 (eight
-// waves), whose last tile of an expert takes the code for 64 rows where that
-// holds its pairs: as many copies and matrix instructions less.
-typedef I8Tile<1, 4, 1, 1, 4> Tile32;
-typedef I8Tile<2, 4, 1, 1, 4, 2> Tile64;
-typedef I8Tile<2, 4, 2, 1, 3, 2> Tile128;
-static_assert(Tile32::BN == 128 && Tile64::BN == 128 && Tile128::BN == 128, "one grid for all");
-static_assert(Tile32::LDS == 80 << 10 && Tile64::LDS == 80 << 10 && Tile128::LDS == 80 << 10, "two work-groups per CU");
+// Tiles of up to 64 pairs (four waves) or of up to 128 (eight waves); one that
+// holds half of that or less, the last of an expert, takes the code for half
+// the rows: as many copies and matrix instructions less.
+template <int ROWS>
+struct MoeTile;
+template <>
+struct MoeTile<64> {
+    typedef I8Tile<2, 2, 1, 2, 2, 2> Whole;
+    typedef I8Tile<1, 4, 1, 1, 2, 2> Half;
+    static constexpr int LDS = 48 << 10, GROUPS = 3;   // work-groups per CU
+};
+template <>
+struct MoeTile<128> {
+    typedef I8Tile<2, 4, 2, 1, 2, 2> Whole;
+    typedef I8Tile<2, 4, 1, 1, 3, 2> Half;
+    static constexpr int LDS = 64 << 10, GROUPS = 2;
+};
+template <int ROWS>
+constexpr bool moe_tile_fits() {
+    typedef typename MoeTile<ROWS>::Whole W;
+    typedef typename MoeTile<ROWS>::Half H;
+    return W::BM == ROWS && H::BM == ROWS / 2 && W::BN == 128 && H::BN == 128 && W::NW == ROWS / 16 && H::NW == W::NW &&
+           W::LDS <= MoeTile<ROWS>::LDS && H::LDS <= MoeTile<ROWS>::LDS &&
+           MoeTile<ROWS>::LDS * MoeTile<ROWS>::GROUPS <= 160 << 10;
+}
+static_assert(moe_tile_fits<64>() && moe_tile_fits<128>(), "one grid and one LDS size for both codes of a kernel");
 
 // Work-group -> (tile, column block), in contiguous eighths for the XCDs, that
 // work-groups are dealt to round-robin, so that the tiles of an expert and the
@@ -345,25 +363,23 @@ __device__ __forceinline__ bool i8_tile_of(const MoeI8& a, int blocks, int4& t, 
 }
 
 template <int ROWS>
-__global__ __launch_bounds__(ROWS == 32 ? 256 : 512, ROWS == 32 ? 2 : 4) void k_i8_gate_up(MoeI8 a) {
-    __shared__ __align__(16) uint8_t lds[ROWS == 32 ? Tile32::LDS : Tile128::LDS];
+__global__ __launch_bounds__(ROWS * 4, ROWS / 64 * MoeTile<ROWS>::GROUPS) void k_i8_gate_up(MoeI8 a) {
+    __shared__ __align__(16) uint8_t lds[MoeTile<ROWS>::LDS];
     int4 t;
     int block;
     if (!i8_tile_of(a, (a.F + 63) / 64, t, block)) return;
-    if constexpr (ROWS == 32) i8_gate_up<Tile32>(a, t, block * 64, lds);
-    else if (t.z <= 64) i8_gate_up<Tile64>(a, t, block * 64, lds);
-    else i8_gate_up<Tile128>(a, t, block * 64, lds);
+    if (t.z <= ROWS / 2) i8_gate_up<typename MoeTile<ROWS>::Half>(a, t, block * 64, lds);
+    else i8_gate_up<typename MoeTile<ROWS>::Whole>(a, t, block * 64, lds);
 }
 
 template <int ROWS, typename Y>
-__global__ __launch_bounds__(ROWS == 32 ? 256 : 512, ROWS == 32 ? 2 : 4) void k_i8_down(MoeI8 a) {
-    __shared__ __align__(16) uint8_t lds[ROWS == 32 ? Tile32::LDS : Tile128::LDS];
+__global__ __launch_bounds__(ROWS * 4, ROWS / 64 * MoeTile<ROWS>::GROUPS) void k_i8_down(MoeI8 a) {
+    __shared__ __align__(16) uint8_t lds[MoeTile<ROWS>::LDS];
     int4 t;
     int block;
     if (!i8_tile_of(a, (a.H + 127) / 128, t, block)) return;
-    if constexpr (ROWS == 32) i8_down<Tile32, Y>(a, t, block * 128, lds);
-    else if (t.z <= 64) i8_down<Tile64, Y>(a, t, block * 128, lds);
-    else i8_down<Tile128, Y>(a, t, block * 128, lds);
+    if (t.z <= ROWS / 2) i8_down<typename MoeTile<ROWS>::Half, Y>(a, t, block * 128, lds);
+    else i8_down<typename MoeTile<ROWS>::Whole, Y>(a, t, block * 128, lds);
 }
 
 // out[t] = sum over k, ascending, of w[t][k] y[t][k]; a pair that was left out
@@ -429,17 +445,17 @@ __global__ __launch_bounds__(256) void k_i8_combine(MoeI8 a) {
 //   1024, 1024, 64, 4    4 25 / 18       8 30 / 24   16 37 / 40
 //   4096, 2048, 8, 1     4 30 / 29       8 35 / 50
 constexpr double MOE_AGAIN = 50e6;
-constexpr int MOE_PAIRS = 512;   // the most that were measured
+constexpr int MOE_PAIRS = 256;   // of small experts too (256, 128, 8, 2; 512 pairs: 23 / 38)
 static bool moe_few(int H, int F, int E, int K, int64_t P) {
     const double again = P - E * (1.0 - pow(1.0 - 1.0 / E, (double)P));
     // rows that fit the work-groups' registers
     return P <= MOE_PAIRS && again * 3.0 * H * F <= MOE_AGAIN && pad_to(H, I8_BK) <= 64 * FP_WAVES * FP_KEEP &&
            K * pad_to(F, I8_BK) <= 64 * FP_WAVES * FP_KEEP;
 }
-// Pairs per tile: 128 instead of 32 where an expert meets more than 24 on
-// average (H = 2048, F = 512, 256 experts, top-8, us, tiles of 32 / 128: average
-// 16 185 / 193, 32 215 / 211, 64 283 / 250, 128 439 / 334).
-static int moe_tile_pairs(double avg) { return avg <= 24 ? 32 : 128; }
+// Pairs per tile: 128 instead of 64 where an expert meets more than 40 on
+// average (H = 2048, F = 512, 256 experts, top-8, us, tiles of 64 / 128: average 16
+// 184 / 191, 32 206 / 208, 48 231 / 230, 64 249 / 245, 128 367 / 331).
+static int moe_tile_pairs(double avg) { return avg <= 40 ? 64 : 128; }
 
 struct MoeI8Plan {
     size_t xq, xs, order, rank, total, cnt, tiles, h, hq, hs, y, bytes;
@@ -463,7 +479,7 @@ static MoeI8Plan plan_moe_i8(int H, int F, int E, int K, int T) {
     take(p.total, 8);
     take(p.cnt, (P + 1023) / 1024 * E * 4);
     // the list for the smallest tile, so that more tokens never need less
-    take(p.tiles, (P / 32 + (P < (size_t)E ? P : (size_t)E)) * sizeof(int4));
+    take(p.tiles, (P / 64 + (P < (size_t)E ? P : (size_t)E)) * sizeof(int4));
     take(p.hq, P * F);
     take(p.hs, P * 4);
     take(p.y, P * H * 4);
@@ -518,11 +534,11 @@ static void launch_many_pairs(const MoeI8& a, const MoeI8Plan& p, int type, int 
     const dim3 gu((unsigned)((p.max_tiles * ((a.F + 63) / 64) + 7) / 8 * 8));
     const dim3 dn((unsigned)((p.max_tiles * ((a.H + 127) / 128) + 7) / 8 * 8));
     const bool half = out_type != T_F32;
-    if (p.tile_pairs == 32) {
-        hipLaunchKernelGGL(k_i8_gate_up<32>, gu, dim3(256), 0, s, a);
+    if (p.tile_pairs == 64) {
+        hipLaunchKernelGGL(k_i8_gate_up<64>, gu, dim3(256), 0, s, a);
         launch_hidden(a, s);
-        if (half) hipLaunchKernelGGL((k_i8_down<32, _Float16>), dn, dim3(256), 0, s, a);
-        else hipLaunchKernelGGL((k_i8_down<32, float>), dn, dim3(256), 0, s, a);
+        if (half) hipLaunchKernelGGL((k_i8_down<64, _Float16>), dn, dim3(256), 0, s, a);
+        else hipLaunchKernelGGL((k_i8_down<64, float>), dn, dim3(256), 0, s, a);
     } else {
         hipLaunchKernelGGL(k_i8_gate_up<128>, gu, dim3(512), 0, s, a);
         launch_hidden(a, s);
