@@ -21,25 +21,33 @@ struct Balance {
     int* done;       // how many of them have ended
     float *loss, *probs;
     int *counts_out, *tokens_out;
-    bool wide;       // rows of logits (and grad) start on multiples of four elements
 };
 
-// Sixteen lanes per row, lane l of them the columns 64 i + 4 l .. + 3 for
-// i < NV: a row of E = 256 is four loads of 16 bytes per lane, and the sums
-// over a row are four DPP steps for four rows at once (one wave per row: six
-// steps each).
-template <int NV>
+// LANES lanes per row, lane l of them the columns 4 LANES i + 4 l .. + 3 for
+// i < NV.  Sixteen up to 512 columns: a row of 256 is four loads of 16 bytes
+// per lane, and the sums over a row are four DPP steps for four rows at once;
+// above, the whole wave, so that a lane keeps 16 values and as many sums.
+template <int LANES, int NV>
 struct BalRow {
     float v[4 * NV];
+    static __device__ __forceinline__ int lane() { return threadIdx.x & (LANES - 1); }
+    static __device__ __forceinline__ int col(int i) { return 4 * LANES * i + 4 * lane(); }
+    static __device__ __forceinline__ float sum(float x) {
+        x = slot_reduce16(x);
+        if constexpr (LANES == 64) {
+            x += xlane<16>(x);
+            x += xlane<32>(x);
+        }
+        return x;
+    }
 
     template <typename T>
-    __device__ __forceinline__ void load(const T* row, int E, bool wide) {
-        typedef T vec __attribute__((ext_vector_type(4)));
-        const int l = threadIdx.x & 15;
+    __device__ __forceinline__ void load(const T* row, int E) {
+        typedef typename VecOf<T, 4>::type vec;
 #pragma unroll
         for (int i = 0; i < NV; i++) {
-            const int c = 64 * i + 4 * l;
-            if (wide && c + 4 <= E) {
+            const int c = col(i);
+            if (c + 4 <= E) {
                 const vec x = *(const vec*)(row + c);
 #pragma unroll
                 for (int k = 0; k < 4; k++) v[4 * i + k] = (float)x[k];
@@ -52,16 +60,16 @@ struct BalRow {
     // softmax of the loaded row; one of -inf alone has no probabilities: zeros
     __device__ __forceinline__ void softmax() {
         float m = v[0];
-        bool nan = false;
 #pragma unroll
-        for (int i = 0; i < 4 * NV; i++) {
-            m = __builtin_fmaxf(m, v[i]);
-            nan |= v[i] != v[i];
-        }
+        for (int i = 1; i < 4 * NV; i++) m = __builtin_fmaxf(m, v[i]);
         m = __builtin_fmaxf(m, xlane<8>(m));
         m = __builtin_fmaxf(m, xlane<4>(m));
         m = __builtin_fmaxf(m, xlane<2>(m));
         m = __builtin_fmaxf(m, xlane<1>(m));
+        if constexpr (LANES == 64) {
+            m = __builtin_fmaxf(m, xlane<16>(m));
+            m = __builtin_fmaxf(m, xlane<32>(m));
+        }
         // where all are -inf: 0 instead, so that every exponential is 0 (a NaN among them stays one)
         const float from = m == -__builtin_huge_valf() ? 0.0f : m;
         float s = 0.0f;
@@ -71,7 +79,7 @@ struct BalRow {
             for (int k = 0; k < 4; k++) v[4 * i + k] = fast_exp(v[4 * i + k] - from);
             s += (v[4 * i] + v[4 * i + 1]) + (v[4 * i + 2] + v[4 * i + 3]);
         }
-        s = slot_reduce16(s);
+        s = sum(s);
         const float r = s == 0.0f ? 0.0f : 1.0f / s;
 #pragma unroll
         for (int i = 0; i < 4 * NV; i++) v[i] *= r;
@@ -80,33 +88,30 @@ struct BalRow {
 
 // Columns past E hold exponentials of -inf: 0.
 
-// threads of a work-group of the sums: 16 waves, for more than 512 experts (64
-// values and as many sums per lane) eight, so that none is spilled
-template <int NV>
-constexpr int BAL_THREADS = NV > 8 ? 512 : 1024;
+constexpr int BAL_THREADS = 1024;   // of a work-group of the sums
 
 // Probabilities and pairs summed over the rows of each work-group (row t of
 // round i: (i * groups + group) * 64 + ..), every sum in a fixed order: a lane
 // over its rows, four rows of a wave, the waves.  Counts are integers: LDS
 // atomics in any order.  With one work-group the results follow at once.
-template <typename T, int NV, bool ONE>
-__global__ __launch_bounds__(BAL_THREADS<NV>) void k_balance_sums(Balance b, const T* __restrict__ logits) {
-    constexpr int THREADS = BAL_THREADS<NV>, ROWS = THREADS / 16;
-    __shared__ float part[THREADS / 64][64 * NV];
+template <typename T, int LANES, int NV, bool ONE>
+__global__ __launch_bounds__(BAL_THREADS) void k_balance_sums(Balance b, const T* __restrict__ logits) {
+    constexpr int THREADS = BAL_THREADS, ROWS = THREADS / LANES, COLS = 4 * LANES * NV;
+    __shared__ float part[THREADS / 64][COLS];
     __shared__ float lpart[THREADS / 64];
-    __shared__ int cnt[64 * NV], n;
+    __shared__ int cnt[COLS], n;
     const int tid = threadIdx.x, wave = tid >> 6;
-    for (int e = tid; e < 64 * NV; e += THREADS) cnt[e] = 0;
+    for (int e = tid; e < COLS; e += THREADS) cnt[e] = 0;
     if (tid == 0) n = 0;
     if (!ONE && blockIdx.x == 0 && tid == 0) *b.done = 0;   // for k_balance_loss, that follows
     __syncthreads();
     float sum[4 * NV] = {};
     int rows = 0;
     for (int t0 = blockIdx.x * ROWS; t0 < b.T; t0 += b.groups * ROWS) {
-        const int t = t0 + (tid >> 4);
+        const int t = t0 + tid / LANES;
         const bool on = t < b.T && (!b.mask || b.mask[t]);
-        BalRow<NV> row;
-        if (on) row.load(logits + t * b.ld, b.E, b.wide);
+        BalRow<LANES, NV> row;
+        if (on) row.load(logits + t * b.ld, b.E);
         const int pairs = min(ROWS, b.T - t0) * b.K;
         const int* ids = b.ids + (int64_t)t0 * b.K;
         for (int p = tid; p < pairs; p += THREADS) {
@@ -117,18 +122,20 @@ __global__ __launch_bounds__(BAL_THREADS<NV>) void k_balance_sums(Balance b, con
             row.softmax();
 #pragma unroll
             for (int i = 0; i < 4 * NV; i++) sum[i] += row.v[i];
-            rows += (tid & 15) == 0;
+            rows += row.lane() == 0;
         }
     }
+    if constexpr (LANES == 16) {
 #pragma unroll
-    for (int i = 0; i < 4 * NV; i++) {
-        sum[i] += xlane<16>(sum[i]);
-        sum[i] += xlane<32>(sum[i]);
+        for (int i = 0; i < 4 * NV; i++) {
+            sum[i] += xlane<16>(sum[i]);
+            sum[i] += xlane<32>(sum[i]);
+        }
     }
-    if ((tid & 63) < 16)
+    if ((tid & 63) < LANES)
 #pragma unroll
         for (int i = 0; i < NV; i++)
-            *(float4*)&part[wave][64 * i + 4 * (tid & 15)] =
+            *(float4*)&part[wave][BalRow<LANES, NV>::col(i)] =
                 make_float4(sum[4 * i], sum[4 * i + 1], sum[4 * i + 2], sum[4 * i + 3]);
     if (rows) atomicAdd(&n, rows);
     __syncthreads();
@@ -220,40 +227,39 @@ __global__ __launch_bounds__(256) void k_balance_loss(Balance b) {
     }
 }
 
-template <typename T, int NV>
+template <typename T, int LANES, int NV>
 __global__ __launch_bounds__(256) void k_balance_grad(Balance b, const T* __restrict__ logits, T* __restrict__ grad) {
-    typedef T vec __attribute__((ext_vector_type(4)));
-    const int l = threadIdx.x & 15, n = *b.tokens;
+    typedef BalRow<LANES, NV> Row;
+    constexpr int ROWS = 256 / LANES;
+    const int n = *b.tokens;
     const float all = n ? 1.0f / ((float)n * (float)b.K) : 0.0f;
     const float c = n ? *b.grad_loss * (float)b.E / (float)n : 0.0f;
     float f[4 * NV];
 #pragma unroll
     for (int i = 0; i < NV; i++) {
-        const int e = 64 * i + 4 * l;
-        int4 x = make_int4(0, 0, 0, 0);
-        if (e + 4 <= b.E && ((uintptr_t)b.counts & 15) == 0) {
-            x = *(const int4*)(b.counts + e);
+        typedef typename VecOf<int, 4>::type vec;
+        const int e = Row::col(i);
+        vec x = {};
+        if (e + 4 <= b.E) {
+            x = *(const vec*)(b.counts + e);
         } else {
-            if (e < b.E) x.x = b.counts[e];
-            if (e + 1 < b.E) x.y = b.counts[e + 1];
-            if (e + 2 < b.E) x.z = b.counts[e + 2];
-            if (e + 3 < b.E) x.w = b.counts[e + 3];
+#pragma unroll
+            for (int k = 0; k < 4; k++) x[k] = e + k < b.E ? b.counts[e + k] : 0;
         }
-        f[4 * i] = (float)x.x * all;
-        f[4 * i + 1] = (float)x.y * all;
-        f[4 * i + 2] = (float)x.z * all;
-        f[4 * i + 3] = (float)x.w * all;
+#pragma unroll
+        for (int k = 0; k < 4; k++) f[4 * i + k] = (float)x[k] * all;
     }
-    BalRow<NV> p, next;
-    auto fetch = [&](int t, BalRow<NV>& r) {
+    // the next round's row is loaded while this one's gradient is formed
+    Row p, next;
+    auto fetch = [&](int t, Row& r) {
         const bool on = t < b.T && (!b.mask || b.mask[t]);
-        if (on) r.load(logits + t * b.ld, b.E, b.wide);
+        if (on) r.load(logits + t * b.ld, b.E);
         return on;
     };
-    const int first = blockIdx.x * 16 + (threadIdx.x >> 4);
+    const int first = blockIdx.x * ROWS + threadIdx.x / LANES;
     bool on = fetch(first, p);
-    for (int t = first; t < b.T; t += gridDim.x * 16) {
-        const bool more = fetch(t + gridDim.x * 16, next);
+    for (int t = first; t < b.T; t += gridDim.x * ROWS) {
+        const bool more = fetch(t + gridDim.x * ROWS, next);
         float d = 0.0f;
         if (on) {
             p.softmax();
@@ -261,72 +267,62 @@ __global__ __launch_bounds__(256) void k_balance_grad(Balance b, const T* __rest
             for (int i = 0; i < 4 * NV; i += 4)
                 d += __builtin_fmaf(f[i], p.v[i], f[i + 1] * p.v[i + 1]) +
                      __builtin_fmaf(f[i + 2], p.v[i + 2], f[i + 3] * p.v[i + 3]);
-            d = slot_reduce16(d);
+            d = Row::sum(d);
         }
         T* to = grad + t * b.ldg;
 #pragma unroll
         for (int i = 0; i < NV; i++) {
-            const int e = 64 * i + 4 * l;
+            const int e = Row::col(i);
             float o[4];
 #pragma unroll
             for (int k = 0; k < 4; k++) o[k] = on ? c * p.v[4 * i + k] * (f[4 * i + k] - d) : 0.0f;
-            if (b.wide && e + 4 <= b.E) {
-                vec x;
-#pragma unroll
-                for (int k = 0; k < 4; k++) x[k] = (T)o[k];
-                *(vec*)(to + e) = x;
-            } else {
-#pragma unroll
-                for (int k = 0; k < 4; k++)
-                    if (e + k < b.E) store_f(to + e + k, o[k]);
-            }
+            store_row(to + e, o, b.E - e);
         }
         p = next;
         on = more;
     }
 }
 
-// Work-groups of the sums of T rows: one, that also finishes, up to BAL_ONE rows.
-constexpr int BAL_ONE = 256, BAL_GROUPS = 256, BAL_GRAD = 1024;
+// Work-groups of the sums of T rows: one, that also finishes, up to BAL_ONE
+// rounds of its rows.
+constexpr int BAL_ONE = 4, BAL_GROUPS = 256, BAL_GRAD = 1024;
 static int balance_groups(int T, int E) {
-    const int n = (T + (E > 512 ? 31 : 63)) / (E > 512 ? 32 : 64);
-    return T <= BAL_ONE ? 1 : n < BAL_GROUPS ? n : BAL_GROUPS;
+    const int rows = E > 512 ? 16 : 64, n = (T + rows - 1) / rows;
+    return n <= BAL_ONE ? 1 : n < BAL_GROUPS ? n : BAL_GROUPS;
 }
 
-template <typename T, int NV>
+template <typename T, int LANES, int NV>
 static void launch_balance(const Balance& b, const void* logits, hipStream_t s) {
+    const dim3 block(BAL_THREADS);
     if (b.groups == 1) {
-        hipLaunchKernelGGL((k_balance_sums<T, NV, true>), dim3(1), dim3(BAL_THREADS<NV>), 0, s, b, (const T*)logits);
+        hipLaunchKernelGGL((k_balance_sums<T, LANES, NV, true>), dim3(1), block, 0, s, b, (const T*)logits);
     } else {
-        hipLaunchKernelGGL((k_balance_sums<T, NV, false>), dim3(b.groups), dim3(BAL_THREADS<NV>), 0, s, b, (const T*)logits);
+        hipLaunchKernelGGL((k_balance_sums<T, LANES, NV, false>), dim3(b.groups), block, 0, s, b, (const T*)logits);
         hipLaunchKernelGGL(k_balance_loss, dim3((b.E + BAL_JOIN - 1) / BAL_JOIN), dim3(256), 0, s, b);
     }
 }
 
-template <typename T, int NV>
+template <typename T, int LANES, int NV>
 static void launch_balance_grad(const Balance& b, const void* logits, void* grad, hipStream_t s) {
-    const int n = (b.T + 15) / 16;
-    hipLaunchKernelGGL((k_balance_grad<T, NV>), dim3(n < BAL_GRAD ? n : BAL_GRAD), dim3(256), 0, s, b, (const T*)logits, (T*)grad);
+    const int rows = 256 / LANES, n = (b.T + rows - 1) / rows;
+    hipLaunchKernelGGL((k_balance_grad<T, LANES, NV>), dim3(n < BAL_GRAD ? n : BAL_GRAD), dim3(256), 0, s, b,
+                       (const T*)logits, (T*)grad);
 }
 
-// f(type of the rows, NV of E columns)
+// f(type of the rows, LANES, NV of E columns)
 template <typename F>
 static void balance_kind(int type, int E, F f) {
     auto width = [&](auto t) {
-        if (E <= 64) f(t, std::integral_constant<int, 1>{});
-        else if (E <= 128) f(t, std::integral_constant<int, 2>{});
-        else if (E <= 256) f(t, std::integral_constant<int, 4>{});
-        else if (E <= 512) f(t, std::integral_constant<int, 8>{});
-        else f(t, std::integral_constant<int, 16>{});
+        std::integral_constant<int, 16> few;
+        if (E <= 64) f(t, few, std::integral_constant<int, 1>{});
+        else if (E <= 128) f(t, few, std::integral_constant<int, 2>{});
+        else if (E <= 256) f(t, few, std::integral_constant<int, 4>{});
+        else if (E <= 512) f(t, few, std::integral_constant<int, 8>{});
+        else f(t, std::integral_constant<int, 64>{}, std::integral_constant<int, 4>{});
     };
     if (type == T_F32) width((float*)nullptr);
     else if (type == T_F16) width((_Float16*)nullptr);
     else width((__bf16*)nullptr);
-}
-
-static bool balance_wide(int type, const void* p, int64_t ld) {
-    const int size = type == T_F32 ? 4 : 2;
-    return (((uintptr_t)p | (uintptr_t)(ld * size)) & (4 * size - 1)) == 0;
 }
 
 }  // namespace chimere
@@ -372,9 +368,8 @@ void chimere_balance_loss(int type, const void* logits, int64_t logits_stride, c
     b.lpart = (float*)(w + 2 * one + al256((size_t)b.groups * 4));
     b.done = (int*)(b.lpart + MAX_E / BAL_JOIN);
     b.loss = loss; b.probs = probs; b.counts_out = counts; b.tokens_out = tokens;
-    b.wide = balance_wide(type, logits, logits_stride);
-    balance_kind(type, n_experts, [&](auto t, auto nv) {
-        launch_balance<std::remove_pointer_t<decltype(t)>, decltype(nv)::value>(b, logits, stream);
+    balance_kind(type, n_experts, [&](auto t, auto lanes, auto nv) {
+        launch_balance<std::remove_pointer_t<decltype(t)>, decltype(lanes)::value, decltype(nv)::value>(b, logits, stream);
     });
     check_launch("balance_loss");
 }
@@ -388,9 +383,8 @@ void chimere_balance_loss_grad(int type, const void* logits, int64_t logits_stri
     Balance b{};
     b.mask = mask; b.counts = counts; b.tokens = tokens; b.grad_loss = grad_loss;
     b.ld = logits_stride; b.ldg = grad_stride; b.E = n_experts; b.K = top_k; b.T = ntok;
-    b.wide = balance_wide(type, logits, logits_stride) && balance_wide(type, grad, grad_stride);
-    balance_kind(type, n_experts, [&](auto t, auto nv) {
-        launch_balance_grad<std::remove_pointer_t<decltype(t)>, decltype(nv)::value>(b, logits, grad, stream);
+    balance_kind(type, n_experts, [&](auto t, auto lanes, auto nv) {
+        launch_balance_grad<std::remove_pointer_t<decltype(t)>, decltype(lanes)::value, decltype(nv)::value>(b, logits, grad, stream);
     });
     check_launch("balance_loss_grad");
 }

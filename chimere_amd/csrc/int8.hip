@@ -17,8 +17,7 @@ __global__ __launch_bounds__(256) void k_i8_quantize(I8Rows<T> q) {
 template <typename T>
 static void launch_i8_quantize(const T* x, int64_t xs, int8_t* q, int64_t qs, float* scale, int64_t nrows, int ncols,
                                hipStream_t s) {
-    const bool wide = (((uintptr_t)x | (uintptr_t)(xs * sizeof(T))) & 15) == 0;
-    const I8Rows<T> r{x, xs, q, qs, scale, nullptr, nullptr, nrows, ncols, wide};
+    const I8Rows<T> r{x, xs, q, qs, scale, nullptr, nullptr, nrows, ncols};
     const int per = i8_rows_per_group<256>(ncols);
     const dim3 grid((unsigned)((nrows + per - 1) / per));
     if (ncols <= I8_WAVE_ROW) hipLaunchKernelGGL((k_i8_quantize<T, 1>), grid, dim3(256), 0, s, r);
@@ -75,13 +74,12 @@ __global__ __launch_bounds__(64 * Tile::NW, WAVES_PER_SIMD) void k_i8_gemm(I8Gem
     v16i acc[Tile::MTILES][Tile::NTILES];
     const int8_t* w = g.w + n0 * g.ldw;
     Tile::run(g.a + m0 * g.lda, w, w, aoff, woff, g.C, lds, acc);
-    const bool wide = (((uintptr_t)g.out | (uintptr_t)(g.ldo * sizeof(T))) & 15) == 0;
     Tile::template rows<VEC>(lds, acc, make_float2(as, 0.0f), [&](int r, const int(&x)[VEC], float2 of_row) {
         if (m0 + r >= g.M || n >= g.N) return;
         float v[VEC];
 #pragma unroll
         for (int k = 0; k < VEC; k++) v[k] = (float)x[k] * of_row.x * ws[k] + b[k];
-        store_row((T*)g.out + (m0 + r) * g.ldo + n, v, g.N - n, wide);
+        store_row((T*)g.out + (m0 + r) * g.ldo + n, v, g.N - n);
     });
 }
 
@@ -137,8 +135,7 @@ __global__ __launch_bounds__(64 * FEW_WAVES) void k_i8_few(I8Gemm g) {
     uint8_t* aq = lds + 16 * MB * 4;
     if constexpr (QUANT) {
         i8_rows_to_lds<64 * FEW_WAVES, FEW_KEEP>(M, S * I8_BK, lda, as, aq, [&](int m, int c, auto& v) {
-            const bool wide = (((uintptr_t)g.x | (uintptr_t)(g.ldx * sizeof(X))) & 15) == 0;
-            i8_load((const X*)g.x + (m0 + m) * g.ldx, c, g.C, wide, v);
+            i8_load((const X*)g.x + (m0 + m) * g.ldx, c, g.C, v);
         }, std::integral_constant<int, 16 / sizeof(X)>{});
     } else {
         if (tid < 16 * MB) as[tid] = g.as[m0 + min(tid, M - 1)];
@@ -231,7 +228,8 @@ static void launch_gemm(const I8Gemm& g, hipStream_t s) {
         if (g.N <= FEW_N) launch_few<T, int8_t, 1, 1>(g, s);
         else launch_few<T, int8_t, 1, 2>(g, s);
     } else if (tiles(64, 64) <= 64) {
-        if (g.M <= 32) launch_few<T, int8_t, 2, 1>(g, s);
+        if (tiles(32, 16) <= 128) launch_few<T, int8_t, 1, 1>(g, s);
+        else if (g.M <= 32) launch_few<T, int8_t, 2, 1>(g, s);
         else launch_few<T, int8_t, 2, 2>(g, s);
     } else if (tiles(64, 64) <= 256) {
         launch_tiles<T, I8Tile<2, 2, 1, 1, 4>, 1>(g, s);

@@ -207,21 +207,4 @@ struct I8Tile {
     }
 };
 
-// n values at p (of which `count` are inside the row) as the type of p, in one
-// store of up to 16 bytes where `wide`
-template <int N, typename T>
-__device__ __forceinline__ void store_row(T* p, const float (&v)[N], int count, bool wide) {
-    typedef T vec __attribute__((ext_vector_type(N)));
-    if (wide && count >= N) {
-        vec o;
-#pragma unroll
-        for (int k = 0; k < N; k++) o[k] = (T)v[k];
-        *(vec*)p = o;
-    } else {
-#pragma unroll
-        for (int k = 0; k < N; k++)
-            if (k < count) p[k] = (T)v[k];
-    }
-}
-
 }  // namespace chimere

@@ -27,12 +27,11 @@ __device__ __forceinline__ void i8_pack(const float (&x)[N], float d, uint32_t (
                    (uint32_t)(uint8_t)i8_quant(x[k + 2], d) << 16 | (uint32_t)(uint8_t)i8_quant(x[k + 3], d) << 24;
 }
 
-// Elements c .. c + V - 1 of a row as f32, one 16-byte load where `wide`; those
-// from ncols on are 0
+// Elements c .. c + V - 1 of a row as f32, those from ncols on 0
 template <typename T, int V>
-__device__ __forceinline__ void i8_load(const T* row, int c, int ncols, bool wide, float (&x)[V]) {
-    typedef T vec __attribute__((ext_vector_type(V)));
-    if (wide && c + V <= ncols) {
+__device__ __forceinline__ void i8_load(const T* row, int c, int ncols, float (&x)[V]) {
+    typedef typename VecOf<T, V>::type vec;
+    if (c + V <= ncols) {
         const vec v = *(const vec*)(row + c);
 #pragma unroll
         for (int k = 0; k < V; k++) x[k] = (float)v[k];
@@ -114,7 +113,6 @@ struct I8Rows {
     const int* count;   // rows, where the device has counted them, or null: nrows
     int64_t nrows;
     int ncols;
-    bool wide;
 };
 
 // A row goes to one wave up to 1024 columns, to four above: 16 elements of
@@ -139,12 +137,12 @@ __device__ __forceinline__ void i8_quantize_rows(const I8Rows<T>& g, int64_t gro
     uint32_t m = 0;
 #pragma unroll
     for (int i = 0; i < KEEP; i++) {
-        i8_load(row, c0 + i * STEP, ncols, g.wide, v[i]);
+        i8_load(row, c0 + i * STEP, ncols, v[i]);
         m = i8_amax(m, v[i]);
     }
     for (int c = c0 + KEEP * STEP; c < ncols; c += STEP) {
         float u[V];
-        i8_load(row, c, ncols, g.wide, u);
+        i8_load(row, c, ncols, u);
         m = i8_amax(m, u);
     }
     m = wave_amax(m);
@@ -178,7 +176,7 @@ __device__ __forceinline__ void i8_quantize_rows(const I8Rows<T>& g, int64_t gro
         if (c0 + i * STEP < ncols) put(c0 + i * STEP, v[i]);
     for (int c = c0 + KEEP * STEP; c < ncols; c += STEP) {
         float u[V];
-        i8_load(row, c, ncols, g.wide, u);
+        i8_load(row, c, ncols, u);
         put(c, u);
     }
 }

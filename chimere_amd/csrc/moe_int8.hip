@@ -76,9 +76,8 @@ __global__ __launch_bounds__(64 * FP_WAVES) void k_i8_pair_gate_up(MoeI8 a) {
     float* xs = (float*)lds;
     uint8_t* xq = lds + 16;
     const X* x = (const X*)a.x + t * a.ldx;
-    const bool wide = ((uintptr_t)x & 15) == 0;
     i8_rows_to_lds<64 * FP_WAVES, FP_KEEP>(1, S * I8_BK, 0, xs, xq,
-                                           [&](int, int c, auto& v) { i8_load(x, c, a.H, wide, v); },
+                                           [&](int, int c, auto& v) { i8_load(x, c, a.H, v); },
                                            std::integral_constant<int, 16 / sizeof(X)>{});
     v4i g = {}, u = {};
     for (int s = wave; s < S; s += FP_WAVES) {
@@ -150,7 +149,7 @@ __global__ __launch_bounds__(64 * FP_WAVES) void k_i8_pair_down(MoeI8 a) {
     const int lda = S * I8_BK;
     i8_rows_to_lds<64 * FP_WAVES, FP_KEEP>(
         a.K, S * I8_BK, lda, hs, lds,
-        [&](int k, int c, auto& v) { i8_load(a.h + ((int64_t)t * a.K + k) * a.F, c, a.F, true, v); },
+        [&](int k, int c, auto& v) { i8_load(a.h + ((int64_t)t * a.K + k) * a.F, c, a.F, v); },
         std::integral_constant<int, 4>{});
     auto piece = [&](int u, const v4i(&now)[2]) {
         const int mine_at = min(u * PER + (r & (PER - 1)), pieces - 1), mk_ = mine_at / S, ms = mine_at - mk_ * S;
@@ -320,7 +319,7 @@ __device__ __forceinline__ void i8_down(const MoeI8& a, const int4& t, int n0, u
 #pragma unroll
         for (int k = 0; k < VEC; k++)
             v[k] = sizeof(Y) == 4 ? (float)x[k] * of_row.x * sd[k] : (float)x[k] * unit;
-        store_row((Y*)a.y + (int64_t)__builtin_bit_cast(int, of_row.y) * a.H + n, v, VEC, true);
+        store_row((Y*)a.y + (int64_t)__builtin_bit_cast(int, of_row.y) * a.H + n, v, VEC);
     });
 }
 
@@ -425,13 +424,7 @@ __global__ __launch_bounds__(256) void k_i8_combine(MoeI8 a) {
             }
         }
     }
-    T* to = (T*)a.out + t * a.ldo + n;
-    if constexpr (sizeof(T) * VEC <= 16) {
-        store_row(to, acc, VEC, (((uintptr_t)a.out | (uintptr_t)(a.ldo * sizeof(T))) & 15) == 0);
-    } else {
-#pragma unroll
-        for (int c = 0; c < VEC; c++) store_f(to + c, acc[c]);
-    }
+    store_row((T*)a.out + t * a.ldo + n, acc, VEC);
 }
 
 // ------------------------------------------------------------ host
@@ -508,8 +501,7 @@ static void launch_few_pairs(const MoeI8& a, int type, int out_type, hipStream_t
 template <typename X>
 static void launch_prepare(const MoeI8& a, hipStream_t s) {
     const int groups = (a.T * a.K + 1023) / 1024, per = i8_rows_per_group<1024>(a.H);
-    const bool wide = (((uintptr_t)a.x | (uintptr_t)(a.ldx * sizeof(X))) & 15) == 0;
-    const I8Rows<X> x{(const X*)a.x, a.ldx, a.xq, a.H, a.xs, nullptr, nullptr, a.T, a.H, wide};
+    const I8Rows<X> x{(const X*)a.x, a.ldx, a.xq, a.H, a.xs, nullptr, nullptr, a.T, a.H};
     const dim3 grid(groups + (a.T + per - 1) / per);
     if (groups == 1) {
         hipLaunchKernelGGL((k_i8_prepare<2, X>), grid, dim3(1024), 0, s, a, x, groups);
@@ -520,7 +512,7 @@ static void launch_prepare(const MoeI8& a, hipStream_t s) {
 }
 
 static void launch_hidden(const MoeI8& a, hipStream_t s) {
-    const I8Rows<float> h{a.h, a.F, a.hq, a.F, a.hs, a.order, a.total, 0, a.F, true};
+    const I8Rows<float> h{a.h, a.F, a.hq, a.F, a.hs, a.order, a.total, 0, a.F};
     const int per = i8_rows_per_group<256>(a.F);
     const dim3 grid((a.T * a.K + per - 1) / per);
     if (a.F <= I8_WAVE_ROW) hipLaunchKernelGGL(k_i8_hidden<1>, grid, dim3(256), 0, s, h);

@@ -77,7 +77,8 @@ def choice(T, E, K, seed, dtype, dev, drop=0.0):
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("T,E,K", [(1, 1, 1), (1, 256, 8), (2, 3, 2), (5, 64, 6), (7, 65, 4), (33, 100, 3), (64, 256, 8), (63, 200, 8),
                                    (257, 256, 8), (300, 1024, 10), (1000, 257, 2), (1023, 8, 2), (1024, 128, 8), (1025, 255, 5),
-                                   (3000, 512, 4), (5000, 60, 6), (9001, 256, 8), (20000, 24, 4)])
+                                   (3000, 512, 4), (5000, 60, 6), (9001, 256, 8), (20000, 24, 4), (64, 1023, 8), (65, 645, 4), (219, 645, 4), (4200, 600, 2),
+                                   (257, 13, 2), (16500, 513, 3)])
 def test_balance(dev, T, E, K, dtype):
     print(f"balance T={T} E={E} K={K} {dtype}", flush=True)
     x, ids, g = choice(T, E, K, T + E, TYPES[dtype], dev, drop=0.1)

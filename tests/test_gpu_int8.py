@@ -380,3 +380,18 @@ def test_refusals(dev):
             f()
     with pytest.raises(ChimereError):
         layer.forward(x, torch.zeros(4, 17, dtype=torch.int32, device=dev), torch.ones(4, 17, device=dev))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_every_address(dev, dtype):
+    """Tokens and outputs that start on every element of a vector, rows of odd length, with and without whole vectors."""
+    g = gen(3)
+    w, ws = weights(301, 515, g)
+    for off in range(9):
+        print(f"address {off} {dtype}", flush=True)
+        for m in (1, 3, 40, 200):
+            x = torch.randn(m * 521 + off, generator=g, device=dev).to(TYPES[dtype])[off:].view(m, 521)[:, :515]
+            room = torch.full((m * 303 + off,), 7.0, dtype=TYPES[dtype], device=dev)
+            int8.linear_i8(x, w, ws, out=room[off:].view(m, 303)[:, :301])
+            close(room[off:].view(m, 303)[:, :301], *product(*q_ref(x), w, ws, None, TYPES[dtype]))
+            assert (room[:off] == 7.0).all() and (room[off:].view(m, 303)[:, 301:] == 7.0).all()
