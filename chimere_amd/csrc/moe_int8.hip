@@ -189,28 +189,37 @@ __global__ __launch_bounds__(64 * FP_WAVES) void k_i8_pair_down(MoeI8 a) {
 // its own.  A work-group takes 1024 pairs: counts per expert and each pair's
 // rank among them (PLAN 0); then every work-group adds up all counts, scans
 // them and places its own pairs, the first one lists the tiles (PLAN 1).  Up to
-// 1024 pairs: one work-group does both (PLAN 2).  (One work-group for 32768
-// pairs, its atomics one after another: 31 us.)
+// PLAN_ONE pairs: one work-group does both (PLAN 2), a launch less.  (One
+// work-group for 32768 pairs, its atomics one after another: 31 us.)
+constexpr int PLAN_ONE = 4096;
 template <int PLAN>
 __device__ __forceinline__ void i8_plan(const MoeI8& a, int groups) {
+    constexpr int AT = PLAN == 2 ? PLAN_ONE / 1024 : 1;   // pairs of a thread
     __shared__ int first[MAX_E], wsum[16], tot[2];
-    const int tid = threadIdx.x, p = blockIdx.x * 1024 + tid, P = a.T * a.K, TP = a.tile_pairs;
-    const int id = p < P ? a.ids[p] : -1, e = (unsigned)id < (unsigned)a.E ? id : -1;
-    int rank = 0;
+    const int tid = threadIdx.x, P = a.T * a.K, TP = a.tile_pairs;
+    int e[AT], rank[AT];
+#pragma unroll
+    for (int i = 0; i < AT; i++) {
+        const int p = (blockIdx.x * AT + i) * 1024 + tid, id = p < P ? a.ids[p] : -1;
+        e[i] = (unsigned)id < (unsigned)a.E ? id : -1;
+        rank[i] = 0;
+    }
     if constexpr (PLAN != 1) {
         first[tid] = 0;
         __syncthreads();
-        if (e >= 0) rank = atomicAdd(&first[e], 1);
+#pragma unroll
+        for (int i = 0; i < AT; i++)
+            if (e[i] >= 0) rank[i] = atomicAdd(&first[e[i]], 1);
         __syncthreads();
         if constexpr (PLAN == 0) {
             if (tid < a.E) a.cnt[blockIdx.x * a.E + tid] = first[tid];
-            if (e >= 0) a.rank[p] = rank;
+            if (e[0] >= 0) a.rank[blockIdx.x * 1024 + tid] = rank[0];
             return;
         }
     }
     int c = 0, before = 0;
     if constexpr (PLAN == 1) {
-        if (e >= 0) rank = a.rank[p];
+        if (e[0] >= 0) rank[0] = a.rank[blockIdx.x * 1024 + tid];
         if (tid < a.E) {
 #pragma unroll 8
             for (int g = 0; g < groups; g++) {
@@ -228,7 +237,9 @@ __device__ __forceinline__ void i8_plan(const MoeI8& a, int groups) {
     const int tile = excl_scan1024(nt, wsum, &tot[1]);
     first[tid] = at + before;
     __syncthreads();
-    if (e >= 0) a.order[first[e] + rank] = p;
+#pragma unroll
+    for (int i = 0; i < AT; i++)
+        if (e[i] >= 0) a.order[first[e[i]] + rank[i]] = (blockIdx.x * AT + i) * 1024 + tid;
     if (blockIdx.x != 0) return;
     for (int s = 0; s < nt; s++) a.tiles[tile + s] = make_int4(tid, at + s * TP, min(TP, c - s * TP), 0);
     if (tid < 2) a.total[tid] = tot[tid];
@@ -323,32 +334,34 @@ __device__ __forceinline__ void i8_down(const MoeI8& a, const int4& t, int n0, u
     });
 }
 
-// Tiles of up to 64 pairs (four waves) or of up to 128 (eight waves); one that
-// holds half of that or less, the last of an expert, takes the code for half
-// the rows: as many copies and matrix instructions less.
+// Tiles of up to 64 pairs (four waves) or 128 (eight waves) against BN weight
+// rows; one that holds half of its pairs or less, the last of an expert,
+// takes the code for half the rows: as many copies and matrix instructions less.
+// (256 x 256 tiles, one work-group per CU: 16 experts, 2811 tokens 109 us
+// against 106, 8192 tokens of 256 experts 486 against 513.)
 template <int ROWS>
 struct MoeTile;
 template <>
 struct MoeTile<64> {
     typedef I8Tile<2, 2, 1, 2, 2, 2> Whole;
     typedef I8Tile<1, 4, 1, 1, 2, 2> Half;
-    static constexpr int LDS = 48 << 10, GROUPS = 3;   // work-groups per CU
+    static constexpr int BN = 128, WAVES = 4, LDS = 48 << 10, GROUPS = 3;   // work-groups per CU
 };
 template <>
 struct MoeTile<128> {
     typedef I8Tile<2, 4, 2, 1, 2, 2> Whole;
     typedef I8Tile<2, 4, 1, 1, 3, 2> Half;
-    static constexpr int LDS = 64 << 10, GROUPS = 2;
+    static constexpr int BN = 128, WAVES = 8, LDS = 64 << 10, GROUPS = 2;
 };
 template <int ROWS>
 constexpr bool moe_tile_fits() {
-    typedef typename MoeTile<ROWS>::Whole W;
-    typedef typename MoeTile<ROWS>::Half H;
-    return W::BM == ROWS && H::BM == ROWS / 2 && W::BN == 128 && H::BN == 128 && W::NW == ROWS / 16 && H::NW == W::NW &&
-           W::LDS <= MoeTile<ROWS>::LDS && H::LDS <= MoeTile<ROWS>::LDS &&
-           MoeTile<ROWS>::LDS * MoeTile<ROWS>::GROUPS <= 160 << 10;
+    typedef MoeTile<ROWS> M;
+    typedef typename M::Whole W;
+    typedef typename M::Half H;
+    return W::BM == ROWS && H::BM == ROWS / 2 && W::BN == M::BN && H::BN == M::BN && W::NW == M::WAVES &&
+           H::NW == M::WAVES && W::LDS <= M::LDS && H::LDS <= M::LDS && M::LDS * M::GROUPS <= 160 << 10;
 }
-static_assert(moe_tile_fits<64>() && moe_tile_fits<128>(), "one grid and one LDS size for both codes of a kernel");
+static_assert(moe_tile_fits<64>() && moe_tile_fits<128>(), "one grid and one LDS size per kernel");
 
 // Work-group -> (tile, column block), in contiguous eighths for the XCDs, that
 // work-groups are dealt to round-robin, so that the tiles of an expert and the
@@ -362,23 +375,27 @@ __device__ __forceinline__ bool i8_tile_of(const MoeI8& a, int blocks, int4& t, 
 }
 
 template <int ROWS>
-__global__ __launch_bounds__(ROWS * 4, ROWS / 64 * MoeTile<ROWS>::GROUPS) void k_i8_gate_up(MoeI8 a) {
-    __shared__ __align__(16) uint8_t lds[MoeTile<ROWS>::LDS];
+__global__ __launch_bounds__(64 * MoeTile<ROWS>::WAVES, MoeTile<ROWS>::WAVES / 4 * MoeTile<ROWS>::GROUPS)
+void k_i8_gate_up(MoeI8 a) {
+    typedef MoeTile<ROWS> M;
+    __shared__ __align__(16) uint8_t lds[M::LDS];
     int4 t;
     int block;
-    if (!i8_tile_of(a, (a.F + 63) / 64, t, block)) return;
-    if (t.z <= ROWS / 2) i8_gate_up<typename MoeTile<ROWS>::Half>(a, t, block * 64, lds);
-    else i8_gate_up<typename MoeTile<ROWS>::Whole>(a, t, block * 64, lds);
+    if (!i8_tile_of(a, (a.F + M::BN / 2 - 1) / (M::BN / 2), t, block)) return;
+    if (t.z <= ROWS / 2) i8_gate_up<typename M::Half>(a, t, block * (M::BN / 2), lds);
+    else i8_gate_up<typename M::Whole>(a, t, block * (M::BN / 2), lds);
 }
 
 template <int ROWS, typename Y>
-__global__ __launch_bounds__(ROWS * 4, ROWS / 64 * MoeTile<ROWS>::GROUPS) void k_i8_down(MoeI8 a) {
-    __shared__ __align__(16) uint8_t lds[MoeTile<ROWS>::LDS];
+__global__ __launch_bounds__(64 * MoeTile<ROWS>::WAVES, MoeTile<ROWS>::WAVES / 4 * MoeTile<ROWS>::GROUPS)
+void k_i8_down(MoeI8 a) {
+    typedef MoeTile<ROWS> M;
+    __shared__ __align__(16) uint8_t lds[M::LDS];
     int4 t;
     int block;
-    if (!i8_tile_of(a, (a.H + 127) / 128, t, block)) return;
-    if (t.z <= ROWS / 2) i8_down<typename MoeTile<ROWS>::Half, Y>(a, t, block * 128, lds);
-    else i8_down<typename MoeTile<ROWS>::Whole, Y>(a, t, block * 128, lds);
+    if (!i8_tile_of(a, (a.H + M::BN - 1) / M::BN, t, block)) return;
+    if (t.z <= ROWS / 2) i8_down<typename M::Half, Y>(a, t, block * M::BN, lds);
+    else i8_down<typename M::Whole, Y>(a, t, block * M::BN, lds);
 }
 
 // out[t] = sum over k, ascending, of w[t][k] y[t][k]; a pair that was left out
@@ -500,7 +517,7 @@ static void launch_few_pairs(const MoeI8& a, int type, int out_type, hipStream_t
 
 template <typename X>
 static void launch_prepare(const MoeI8& a, hipStream_t s) {
-    const int groups = (a.T * a.K + 1023) / 1024, per = i8_rows_per_group<1024>(a.H);
+    const int P = a.T * a.K, groups = P <= PLAN_ONE ? 1 : (P + 1023) / 1024, per = i8_rows_per_group<1024>(a.H);
     const I8Rows<X> x{(const X*)a.x, a.ldx, a.xq, a.H, a.xs, nullptr, nullptr, a.T, a.H};
     const dim3 grid(groups + (a.T + per - 1) / per);
     if (groups == 1) {
@@ -519,24 +536,25 @@ static void launch_hidden(const MoeI8& a, hipStream_t s) {
     else hipLaunchKernelGGL(k_i8_hidden<4>, grid, dim3(256), 0, s, h);
 }
 
+template <int ROWS>
+static void launch_tiles(const MoeI8& a, int max_tiles, bool half, hipStream_t s) {
+    constexpr int BN = MoeTile<ROWS>::BN;
+    const dim3 block(64 * MoeTile<ROWS>::WAVES);
+    const dim3 gu((unsigned)((max_tiles * ((a.F + BN / 2 - 1) / (BN / 2)) + 7) / 8 * 8));
+    const dim3 dn((unsigned)((max_tiles * ((a.H + BN - 1) / BN) + 7) / 8 * 8));
+    hipLaunchKernelGGL(k_i8_gate_up<ROWS>, gu, block, 0, s, a);
+    launch_hidden(a, s);
+    if (half) hipLaunchKernelGGL((k_i8_down<ROWS, _Float16>), dn, block, 0, s, a);
+    else hipLaunchKernelGGL((k_i8_down<ROWS, float>), dn, block, 0, s, a);
+}
+
 static void launch_many_pairs(const MoeI8& a, const MoeI8Plan& p, int type, int out_type, hipStream_t s) {
     if (type == T_F32) launch_prepare<float>(a, s);
     else if (type == T_F16) launch_prepare<_Float16>(a, s);
     else launch_prepare<__bf16>(a, s);
-    const dim3 gu((unsigned)((p.max_tiles * ((a.F + 63) / 64) + 7) / 8 * 8));
-    const dim3 dn((unsigned)((p.max_tiles * ((a.H + 127) / 128) + 7) / 8 * 8));
     const bool half = out_type != T_F32;
-    if (p.tile_pairs == 64) {
-        hipLaunchKernelGGL(k_i8_gate_up<64>, gu, dim3(256), 0, s, a);
-        launch_hidden(a, s);
-        if (half) hipLaunchKernelGGL((k_i8_down<64, _Float16>), dn, dim3(256), 0, s, a);
-        else hipLaunchKernelGGL((k_i8_down<64, float>), dn, dim3(256), 0, s, a);
-    } else {
-        hipLaunchKernelGGL(k_i8_gate_up<128>, gu, dim3(512), 0, s, a);
-        launch_hidden(a, s);
-        if (half) hipLaunchKernelGGL((k_i8_down<128, _Float16>), dn, dim3(512), 0, s, a);
-        else hipLaunchKernelGGL((k_i8_down<128, float>), dn, dim3(512), 0, s, a);
-    }
+    if (p.tile_pairs == 64) launch_tiles<64>(a, p.max_tiles, half, s);
+    else launch_tiles<128>(a, p.max_tiles, half, s);
     const dim3 grid((unsigned)((a.H / (half ? 8 : 4) + 255) / 256) * a.T);
     if (out_type == T_F32) hipLaunchKernelGGL((k_i8_combine<float, float>), grid, dim3(256), 0, s, a);
     else if (out_type == T_F16) hipLaunchKernelGGL((k_i8_combine<_Float16, _Float16>), grid, dim3(256), 0, s, a);
