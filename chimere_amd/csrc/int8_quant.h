@@ -11,20 +11,47 @@ namespace chimere {
 __device__ __forceinline__ float i8_scale(uint32_t amax) {
     return __builtin_bit_cast(float, amax) * (1.0f / 127.0f);
 }
-// the integer of x in a row of scale d (held to +-127: a subnormal scale can be
-// rounded down by up to a third)
-__device__ __forceinline__ int i8_quant(float x, float d) {
-    const float q = __builtin_fminf(__builtin_fmaxf(__builtin_rintf(x / d), -127.0f), 127.0f);
-    return d > 0.0f && d < __builtin_huge_valf() ? (int)q : 0;
-}
+// x / d as IEEE rounds it, with what a row's divisions share worked out once:
+// from y = 1 / d (rounded to nearest) the product x y is off by two units in
+// the last place at most, one correction q + (x - q d) y makes that less than
+// one and a second the nearest (Markstein, "Computation of elementary functions
+// on the IBM RISC System/6000 processor", 1990); the remainders are exact in an
+// fma as long as nothing leaves f32's normal range, so rows of scale under 2^-90
+// divide.  With the packing below 8 operations an element, where a division and
+// conversions take about 20: rows of 512 bf16, 32768 of them, 14.4 -> 11.8 us,
+// 4096 rows of 2048 8.4 -> 7.0.
+struct I8Scale {
+    float d, y;
+    bool ok, near;
+    __device__ __forceinline__ explicit I8Scale(float scale)
+        : d(scale), y(1.0f / scale), ok(scale > 0.0f && scale < __builtin_huge_valf()), near(scale >= 0x1p-90f) {}
+    __device__ __forceinline__ float quotient(float x) const {
+        const float q = x * y, u = __builtin_fmaf(__builtin_fmaf(-q, d, x), y, q);
+        return __builtin_fmaf(__builtin_fmaf(-u, d, x), y, u);
+    }
+    // The integer of a quotient in the low byte: the sum's unit is 1, so the
+    // addition rounds to the nearest integer, ties to even.  Held to +-127: a
+    // subnormal scale can be rounded down by up to a third.
+    __device__ __forceinline__ uint32_t byte(float q) const {
+        return __float_as_uint(__builtin_amdgcn_fmed3f(q, -127.0f, 127.0f) + 12582912.0f);
+    }
+};
 
-// N integers packed into bytes
+// N integers packed into bytes; 0 where the scale is 0, infinite or NaN
 template <int N>
-__device__ __forceinline__ void i8_pack(const float (&x)[N], float d, uint32_t (&q)[N / 4]) {
+__device__ __forceinline__ void i8_pack(const float (&x)[N], const I8Scale& s, uint32_t (&q)[N / 4]) {
+    float u[N];
 #pragma unroll
-    for (int k = 0; k < N; k += 4)
-        q[k / 4] = (uint32_t)(uint8_t)i8_quant(x[k], d) | (uint32_t)(uint8_t)i8_quant(x[k + 1], d) << 8 |
-                   (uint32_t)(uint8_t)i8_quant(x[k + 2], d) << 16 | (uint32_t)(uint8_t)i8_quant(x[k + 3], d) << 24;
+    for (int k = 0; k < N; k++) u[k] = s.quotient(x[k]);
+    if (__builtin_expect(!s.near, 0))
+#pragma unroll
+        for (int k = 0; k < N; k++) u[k] = x[k] / s.d;
+#pragma unroll
+    for (int k = 0; k < N; k += 4) {
+        const uint32_t lo = __builtin_amdgcn_perm(s.byte(u[k + 1]), s.byte(u[k]), 0x0c0c0400);
+        const uint32_t hi = __builtin_amdgcn_perm(s.byte(u[k + 3]), s.byte(u[k + 2]), 0x04000c0c);
+        q[k / 4] = s.ok ? lo | hi : 0;
+    }
 }
 
 // Elements c .. c + V - 1 of a row as f32, those from ncols on 0
@@ -94,7 +121,7 @@ __device__ __forceinline__ void i8_rows_to_lds(int M, int cols, int lda, float* 
         const int at = tid + i * THREADS, m = min(at / per, M - 1);
         if (at < n) {
             uint32_t p[V / 4];
-            i8_pack(v[i], as[m], p);
+            i8_pack(v[i], I8Scale(as[m]), p);
 #pragma unroll
             for (int k = 0; k < V / 4; k++) *(uint32_t*)(aq + m * lda + (at - m * per) * V + 4 * k) = p[k];
         }
@@ -154,11 +181,12 @@ __device__ __forceinline__ void i8_quantize_rows(const I8Rows<T>& g, int64_t gro
         if (!on) return;
     }
     const float d = i8_scale(m);
+    const I8Scale by(d);
     if (c0 == 0) g.scale[g.to ? g.to[r] : r] = d;
     int8_t* to = g.q + r * g.qs;
     auto put = [&](int c, const float(&u)[V]) {
         uint32_t p[V / 4];
-        i8_pack(u, d, p);
+        i8_pack(u, by, p);
         if (c + V <= ncols) {
             typedef uint32_t words __attribute__((ext_vector_type(V / 4)));
             words o;

@@ -97,6 +97,25 @@ def test_quantize_borders(dev, c):
     assert (q.double().cpu() == rq).all()
 
 
+@pytest.mark.parametrize("power", [-140, -100, -89, -20, 0, 60, 115])
+def test_quantize_next_to_ties(dev, power):
+    """16 million quotients within two steps of a half, for 1024 scales of every mantissa length."""
+    g = gen(power + 200)
+    amax = (torch.rand(1024, 1, generator=g, device=dev) + 1) * 127.0
+    amax[::3] = torch.floor(amax[::3] * 64) / 64
+    amax = (amax.double() * 2.0 ** power).float()
+    scale = amax * torch.full((1,), 1.0 / 127, device=dev)
+    half = torch.randint(-127, 127, (1024, 16384), generator=g, device=dev) + 0.5
+    x = (half.double() * scale.double()).float()
+    for _ in range(2):
+        way = torch.randint(0, 3, x.shape, generator=g, device=dev)
+        x = torch.where(way == 0, torch.nextafter(x, -amax), torch.where(way == 1, torch.nextafter(x, amax), x))
+    x[:, :1] = amax
+    q, s = int8.quantize_i8(x)
+    rq, rs = q_ref(x)
+    assert (s.double().cpu() == rs).all() and (q.double().cpu() == rq).all()
+
+
 @pytest.mark.parametrize("dtype", ["f16", "bf16"])
 def test_quantize_many_ties(dev, dtype):
     """Rows whose largest value is a multiple of 127 in its last places, so that every other one is a tie; scales as torch's."""
