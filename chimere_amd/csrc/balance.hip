@@ -14,9 +14,10 @@ struct Balance {
     const int *counts, *tokens;
     const float* grad_loss;
     int64_t ld, ldg;
-    int E, K, T, groups;
-    float* psum;     // [groups][E]
-    int *pcnt, *pn;  // [groups][E], [groups]
+    int E, K, T, groups, threads;   // threads per work-group of the sums
+    int ep, lanes, joins;   // columns of a work-group's sums; lanes of four columns to join them, and work-groups
+    float* psum;     // [groups][ep]
+    int *pcnt, *pn;  // [groups][ep], [groups]
     float* lpart;    // parts of the loss, one per work-group of k_balance_loss
     int* done;       // how many of them have ended
     float *loss, *probs;
@@ -88,15 +89,13 @@ struct BalRow {
 
 // Columns past E hold exponentials of -inf: 0.
 
-constexpr int BAL_THREADS = 1024;   // of a work-group of the sums
-
 // Probabilities and pairs summed over the rows of each work-group (row t of
-// round i: (i * groups + group) * 64 + ..), every sum in a fixed order: a lane
+// round i: (i * groups + group) * ROWS + ..), every sum in a fixed order: a lane
 // over its rows, four rows of a wave, the waves.  Counts are integers: LDS
 // atomics in any order.  With one work-group the results follow at once.
-template <typename T, int LANES, int NV, bool ONE>
-__global__ __launch_bounds__(BAL_THREADS) void k_balance_sums(Balance b, const T* __restrict__ logits) {
-    constexpr int THREADS = BAL_THREADS, ROWS = THREADS / LANES, COLS = 4 * LANES * NV;
+template <typename T, int LANES, int NV, int THREADS, bool ONE>
+__global__ __launch_bounds__(THREADS) void k_balance_sums(Balance b, const T* __restrict__ logits) {
+    constexpr int ROWS = THREADS / LANES, COLS = 4 * LANES * NV;
     __shared__ float part[THREADS / 64][COLS];
     __shared__ float lpart[THREADS / 64];
     __shared__ int cnt[COLS], n;
@@ -166,63 +165,103 @@ __global__ __launch_bounds__(BAL_THREADS) void k_balance_sums(Balance b, const T
         }
     } else {
         for (int e = tid; e < b.E; e += THREADS) {
-            b.psum[(int64_t)blockIdx.x * b.E + e] = psum(e);
-            b.pcnt[(int64_t)blockIdx.x * b.E + e] = cnt[e];
+            b.psum[(int64_t)blockIdx.x * b.ep + e] = psum(e);
+            b.pcnt[(int64_t)blockIdx.x * b.ep + e] = cnt[e];
         }
         if (tid == 0) b.pn[blockIdx.x] = n;
     }
 }
 
-// The work-groups' sums joined, 32 experts per work-group by eight segments of
-// them (one work-group for all experts read 256 x 256 sums in 7 us); the last
-// work-group to end adds up the parts of the loss, in their order.
-constexpr int BAL_JOIN = 32;
-__global__ __launch_bounds__(256) void k_balance_loss(Balance b) {
-    __shared__ float ps[256], part[MAX_E / BAL_JOIN];
-    __shared__ int pc[256], n, last;
-    const int tid = threadIdx.x, seg = tid / BAL_JOIN, e = blockIdx.x * BAL_JOIN + tid % BAL_JOIN;
+// The work-groups' sums joined: LANES lanes of four experts each by the segments
+// of the groups that fit in 1024 threads (32 at most), a wave's segments added
+// up first.  Where one work-group does not take all experts, the last to end
+// adds up the parts of the loss.
+constexpr int BAL_GROUPS = 256;   // of the sums at most
+constexpr int BAL_JOIN = 8;   // lanes where there are several work-groups
+constexpr int bal_join_threads(int lanes) { return lanes < 32 ? 32 * lanes : 1024; }
+template <int LANES>
+__global__ __launch_bounds__(bal_join_threads(LANES)) void k_balance_loss(Balance b) {
+    constexpr int THREADS = bal_join_threads(LANES), SEGS = THREADS / LANES, COLS = 4 * LANES;
+    constexpr int PARTS = LANES < 64 ? THREADS / 64 : SEGS, LOSSES = COLS <= 64 ? 1 : COLS / 64;
+    __shared__ float ps[PARTS][COLS], part[LOSSES];
+    __shared__ int pc[PARTS][COLS], n, last;
+    const int tid = threadIdx.x, seg = tid / LANES, c = tid % LANES * 4, e0 = blockIdx.x * COLS, e = e0 + tid;
     if (tid == 0) n = 0;
     __syncthreads();
-    float s = 0.0f;
-    int c = 0;
-    if (e < b.E) {
+    float s[4] = {};
+    int k[4] = {};
+    if (e0 + c < b.ep) {
 #pragma unroll 8
-        for (int g = seg; g < b.groups; g += 256 / BAL_JOIN) {
-            s += b.psum[(int64_t)g * b.E + e];
-            c += b.pcnt[(int64_t)g * b.E + e];
+        for (int g = seg; g < b.groups; g += SEGS) {
+            const float4 v = *(const float4*)(b.psum + (int64_t)g * b.ep + e0 + c);
+            const int4 u = *(const int4*)(b.pcnt + (int64_t)g * b.ep + e0 + c);
+            s[0] += v.x; s[1] += v.y; s[2] += v.z; s[3] += v.w;
+            k[0] += u.x; k[1] += u.y; k[2] += u.z; k[3] += u.w;
         }
     }
-    ps[tid] = s;
-    pc[tid] = c;
-    for (int g = tid; g < b.groups; g += 256) atomicAdd(&n, b.pn[g]);
+    static_assert(THREADS >= BAL_GROUPS);
+    const int tokens = tid < b.groups ? b.pn[tid] : 0;
+    if (tokens) atomicAdd(&n, tokens);
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        if constexpr (LANES <= 8) {
+            s[i] += xlane<8>(s[i]);
+            k[i] += xlane<8>(k[i]);
+        }
+        if constexpr (LANES <= 16) {
+            s[i] += xlane<16>(s[i]);
+            k[i] += xlane<16>(k[i]);
+        }
+        if constexpr (LANES <= 32) {
+            s[i] += xlane<32>(s[i]);
+            k[i] += xlane<32>(k[i]);
+        }
+    }
+    if (LANES >= 64 || (tid & 63) < LANES) {
+        *(float4*)&ps[LANES < 64 ? tid / 64 : seg][c] = make_float4(s[0], s[1], s[2], s[3]);
+        *(int4*)&pc[LANES < 64 ? tid / 64 : seg][c] = make_int4(k[0], k[1], k[2], k[3]);
+    }
     __syncthreads();
     float l = 0.0f;
-    if (tid < BAL_JOIN && e < b.E) {
+    if (tid < COLS && e < b.E) {
+        float v = 0.0f;
+        int u = 0;
 #pragma unroll
-        for (int i = 1; i < 256 / BAL_JOIN; i++) {
-            s += ps[i * BAL_JOIN + tid];
-            c += pc[i * BAL_JOIN + tid];
+        for (int i = 0; i < PARTS; i++) {
+            v += ps[i][tid];
+            u += pc[i][tid];
         }
-        s = n ? s / (float)n : 0.0f;
-        b.probs[e] = s;
-        b.counts_out[e] = c;
-        l = n ? (float)c / ((float)n * (float)b.K) * s : 0.0f;
+        v = n ? v / (float)n : 0.0f;
+        b.probs[e] = v;
+        b.counts_out[e] = u;
+        l = n ? (float)u / ((float)n * (float)b.K) * v : 0.0f;
     }
     l = slot_reduce16(l);
     l += xlane<16>(l);
-    if (tid == 0) {
-        // visible to the whole device before the count says so
-        __hip_atomic_store(&b.lpart[blockIdx.x], l, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        last = __hip_atomic_fetch_add(b.done, 1, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT) == (int)gridDim.x - 1;
+    l += xlane<32>(l);
+    if constexpr (LOSSES > 1) {
+        if ((tid & 63) == 0 && tid / 64 < LOSSES) part[tid / 64] = l;
+        __syncthreads();
+        l = 0.0f;
+#pragma unroll
+        for (int i = 0; i < LOSSES; i++) l += part[i];
     }
-    __syncthreads();
-    if (!last) return;
-    if (tid < gridDim.x) part[tid] = __hip_atomic_load(&b.lpart[tid], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    __syncthreads();
+    if constexpr (LANES == BAL_JOIN) {
+        if (b.joins > 1) {
+            if (tid == 0) {
+                // visible to the whole device before the count says so
+                __hip_atomic_store(&b.lpart[blockIdx.x], l, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                last = __hip_atomic_fetch_add(b.done, 1, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT) == b.joins - 1;
+            }
+            __syncthreads();
+            if (!last || tid >= 64) return;
+            l = tid < b.joins ? __hip_atomic_load(&b.lpart[tid], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) : 0.0f;
+            l = slot_reduce16(l);
+            l += xlane<16>(l);
+        }
+    }
     if (tid == 0) {
-        float v = 0.0f;
-        for (int i = 0; i < (int)gridDim.x; i++) v += part[i];
-        *b.loss = (float)b.E * v;
+        *b.loss = (float)b.E * l;
         *b.tokens_out = n;
     }
 }
@@ -283,23 +322,55 @@ __global__ __launch_bounds__(256) void k_balance_grad(Balance b, const T* __rest
     }
 }
 
-// Work-groups of the sums of T rows: one, that also finishes, up to BAL_ONE
-// rounds of its rows.
-constexpr int BAL_ONE = 4, BAL_GROUPS = 256, BAL_GRAD = 1024;
-static int balance_groups(int T, int E) {
-    const int rows = E > 512 ? 16 : 64, n = (T + rows - 1) / rows;
-    return n <= BAL_ONE ? 1 : n < BAL_GROUPS ? n : BAL_GROUPS;
+// How T rows are shared out.  Work-groups of the sums have 1024 threads, 64 rows
+// (16 above 256 experts) at once.  One alone, that finishes by itself, while the
+// rounds of its rows cost less than a second launch, about 4 us (64 tokens of
+// 256 experts 5.9 us, another 1.4 us for every 64 more; 160 of 72 6.0, against
+// 4.0 + 3.0 and the launch).  256 threads while the sums of a quarter of the
+// rows per work-group are still joined by one work-group, which takes 3 to 5.6 us
+// for up to BAL_JOIN_MAX sums where several take 6 to 7 (2219 tokens of 143
+// experts: 4.8 + 5.6 us, before 7.2 + 6.3).
+constexpr int BAL_ONE = 4, BAL_ONE_MAX = 32768;   // rounds and logits of a single work-group
+constexpr int BAL_GRAD = 1024, BAL_JOIN_MAX = 32768;
+static void balance_plan(Balance& b) {
+    const int rows = b.E > 256 ? 16 : 64;
+    auto groups = [&](int r) { return b.T / r + (b.T % r != 0); };
+    b.ep = (b.E + 3) & ~3;
+    b.threads = 1024;
+    b.groups = groups(rows);
+    if (b.groups <= BAL_ONE && b.T * b.ep <= BAL_ONE_MAX) {
+        b.groups = 1;
+    } else if (groups(rows / 4) <= BAL_GROUPS && groups(rows / 4) * b.ep <= BAL_JOIN_MAX) {
+        b.threads = 256;
+        b.groups = groups(rows / 4);
+    } else if (b.groups > BAL_GROUPS) {
+        b.groups = BAL_GROUPS;
+    }
+    b.lanes = BAL_JOIN;
+    while (b.groups * b.ep <= BAL_JOIN_MAX && 4 * b.lanes < b.ep) b.lanes *= 2;
+    b.joins = (b.ep + 4 * b.lanes - 1) / (4 * b.lanes);
+}
+
+template <int LANES>
+static void launch_join(const Balance& b, hipStream_t s) {
+    if (b.lanes == LANES)
+        hipLaunchKernelGGL(k_balance_loss<LANES>, dim3(b.joins), dim3(bal_join_threads(LANES)), 0, s, b);
+    else if constexpr (LANES < MAX_E / 4)
+        launch_join<2 * LANES>(b, s);
 }
 
 template <typename T, int LANES, int NV>
 static void launch_balance(const Balance& b, const void* logits, hipStream_t s) {
-    const dim3 block(BAL_THREADS);
+    const T* x = (const T*)logits;
     if (b.groups == 1) {
-        hipLaunchKernelGGL((k_balance_sums<T, LANES, NV, true>), dim3(1), block, 0, s, b, (const T*)logits);
-    } else {
-        hipLaunchKernelGGL((k_balance_sums<T, LANES, NV, false>), dim3(b.groups), block, 0, s, b, (const T*)logits);
-        hipLaunchKernelGGL(k_balance_loss, dim3((b.E + BAL_JOIN - 1) / BAL_JOIN), dim3(256), 0, s, b);
+        hipLaunchKernelGGL((k_balance_sums<T, LANES, NV, 1024, true>), dim3(1), dim3(1024), 0, s, b, x);
+        return;
     }
+    if (b.threads == 256)
+        hipLaunchKernelGGL((k_balance_sums<T, LANES, NV, 256, false>), dim3(b.groups), dim3(256), 0, s, b, x);
+    else
+        hipLaunchKernelGGL((k_balance_sums<T, LANES, NV, 1024, false>), dim3(b.groups), dim3(1024), 0, s, b, x);
+    launch_join<BAL_JOIN>(b, s);
 }
 
 template <typename T, int LANES, int NV>
@@ -314,11 +385,12 @@ template <typename F>
 static void balance_kind(int type, int E, F f) {
     auto width = [&](auto t) {
         std::integral_constant<int, 16> few;
+        std::integral_constant<int, 64> all;
         if (E <= 64) f(t, few, std::integral_constant<int, 1>{});
         else if (E <= 128) f(t, few, std::integral_constant<int, 2>{});
         else if (E <= 256) f(t, few, std::integral_constant<int, 4>{});
-        else if (E <= 512) f(t, few, std::integral_constant<int, 8>{});
-        else f(t, std::integral_constant<int, 64>{}, std::integral_constant<int, 4>{});
+        else if (E <= 512) f(t, all, std::integral_constant<int, 2>{});
+        else f(t, all, std::integral_constant<int, 4>{});
     };
     if (type == T_F32) width((float*)nullptr);
     else if (type == T_F16) width((_Float16*)nullptr);
@@ -333,9 +405,14 @@ extern "C" {
 
 size_t chimere_balance_loss_workspace_size(int n_experts, int max_ntok) {
     if (n_experts < 1 || n_experts > MAX_E || max_ntok < 0) return 0;
-    const size_t g = balance_groups(max_ntok, n_experts);
-    if (g == 1) return 0;
-    return 2 * al256(g * n_experts * 4) + al256(g * 4) + 256;
+    Balance b{};
+    b.E = n_experts; b.T = max_ntok;
+    balance_plan(b);
+    if (b.groups == 1) return 0;
+    // of any smaller number of tokens, too
+    const int64_t quarter = min(BAL_JOIN_MAX / b.ep, BAL_GROUPS);
+    const size_t g = b.threads == 256 ? b.groups : max((int64_t)b.groups, quarter);
+    return 2 * al256(g * b.ep * 4) + al256(g * 4) + 256;
 }
 
 static bool balance_args(const char* what, int type, const void* logits, int64_t ld, int E, int K, int T) {
@@ -361,12 +438,13 @@ void chimere_balance_loss(int type, const void* logits, int64_t logits_stride, c
                     "balance_loss: workspace %zu bytes < %zu (or not 256-byte aligned)", workspace_bytes, need);
     Balance b{};
     b.ids = ids; b.mask = mask; b.ld = logits_stride;
-    b.E = n_experts; b.K = top_k; b.T = ntok; b.groups = balance_groups(ntok, n_experts);
+    b.E = n_experts; b.K = top_k; b.T = ntok;
+    balance_plan(b);
     uint8_t* w = (uint8_t*)workspace;
-    const size_t one = al256((size_t)b.groups * n_experts * 4);
+    const size_t one = al256((size_t)b.groups * b.ep * 4);
     b.psum = (float*)w; b.pcnt = (int*)(w + one); b.pn = (int*)(w + 2 * one);
     b.lpart = (float*)(w + 2 * one + al256((size_t)b.groups * 4));
-    b.done = (int*)(b.lpart + MAX_E / BAL_JOIN);
+    b.done = (int*)(b.lpart + MAX_E / (4 * BAL_JOIN));
     b.loss = loss; b.probs = probs; b.counts_out = counts; b.tokens_out = tokens;
     balance_kind(type, n_experts, [&](auto t, auto lanes, auto nv) {
         launch_balance<std::remove_pointer_t<decltype(t)>, decltype(lanes)::value, decltype(nv)::value>(b, logits, stream);

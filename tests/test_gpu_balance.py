@@ -86,6 +86,18 @@ def test_balance(dev, T, E, K, dtype):
     check(x, ids, mask=torch.rand(T, generator=g, device=dev) < 0.6)
 
 
+@pytest.mark.parametrize("T,E,K", [(257, 16, 2), (260, 33, 3), (300, 64, 4), (513, 64, 4), (300, 128, 8), (600, 256, 8), (600, 511, 8),
+                                   (2048, 256, 2), (2049, 256, 2), (8192, 256, 2), (8193, 253, 2), (128, 512, 8), (33, 1021, 4),
+                                   (128, 1024, 8), (512, 1024, 2), (513, 1024, 2), (4096, 7, 1), (4097, 7, 1), (70000, 5, 2)])
+def test_balance_joins(dev, T, E, K):
+    """Sizes on both sides of where the work is shared out another way."""
+    print(f"balance joins T={T} E={E} K={K}", flush=True)
+    x, ids, g = choice(T, E, K, T * E, torch.bfloat16, dev, drop=0.1)
+    first = check(x, ids)
+    again = routing.balance_loss(x, ids)
+    assert all(torch.equal(a, b) for a, b in zip(first, again))
+
+
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("T", [1, 9, 130, 2000])
 def test_masks_and_odd_values(dev, T, dtype):
