@@ -14,14 +14,19 @@ __global__ __launch_bounds__(256) void k_i8_quantize(I8Rows<T> q) {
     i8_quantize_rows<T, W, 256>(q, blockIdx.x);
 }
 
+// (2^24 rows per launch: a grid has less than 2^32 threads)
 template <typename T>
 static void launch_i8_quantize(const T* x, int64_t xs, int8_t* q, int64_t qs, float* scale, int64_t nrows, int ncols,
                                hipStream_t s) {
-    const I8Rows<T> r{x, xs, q, qs, scale, nullptr, nullptr, nrows, ncols};
+    constexpr int64_t AT_ONCE = 1 << 24;
     const int per = i8_rows_per_group<256>(ncols);
-    const dim3 grid((unsigned)((nrows + per - 1) / per));
-    if (ncols <= I8_WAVE_ROW) hipLaunchKernelGGL((k_i8_quantize<T, 1>), grid, dim3(256), 0, s, r);
-    else hipLaunchKernelGGL((k_i8_quantize<T, 4>), grid, dim3(256), 0, s, r);
+    for (int64_t r = 0; r < nrows; r += AT_ONCE) {
+        const int64_t n = nrows - r < AT_ONCE ? nrows - r : AT_ONCE;
+        const I8Rows<T> rows{x + r * xs, xs, q + r * qs, qs, scale + r, nullptr, nullptr, n, ncols};
+        const dim3 grid((unsigned)((n + per - 1) / per));
+        if (ncols <= I8_WAVE_ROW) hipLaunchKernelGGL((k_i8_quantize<T, 1>), grid, dim3(256), 0, s, rows);
+        else hipLaunchKernelGGL((k_i8_quantize<T, 4>), grid, dim3(256), 0, s, rows);
+    }
 }
 
 void launch_i8_quantize(int type, const void* x, int64_t xs, int8_t* q, int64_t qs, float* scale, int64_t nrows,
@@ -300,16 +305,16 @@ static bool gemm_args(const char* what, const int8_t* w, int64_t ldw, const floa
                       int64_t ldo, int ntok, int nrows, int ncols) {
     if (!float_type(out_type)) {
         set_error(CHIMERE_ERR_ARG, "%s: unsupported output type %d", what, out_type);
-    } else if (ntok < 0 || nrows < 1 || ncols < 1 || ncols > I8_MAX_C) {
-        set_error(CHIMERE_ERR_ARG, "%s: bad sizes ntok=%d nrows=%d ncols=%d (ncols at most %d)", what, ntok, nrows,
-                  ncols, I8_MAX_C);
+    } else if (ntok < 0 || ntok > I8_MAX_ROWS || nrows < 1 || nrows > I8_MAX_ROWS || ncols < 1 || ncols > I8_MAX_C) {
+        set_error(CHIMERE_ERR_ARG, "%s: bad sizes ntok=%d nrows=%d (at most %d) ncols=%d (at most %d)", what, ntok,
+                  nrows, I8_MAX_ROWS, ncols, I8_MAX_C);
     } else if (ntok > 0 && !(w && ws && out)) {
         set_error(CHIMERE_ERR_ARG, "%s: null pointer", what);
     } else if (ldw < ncols || ldw > I8_MAX_STRIDE || ldo < nrows) {
         set_error(CHIMERE_ERR_ARG, "%s: bad strides w %lld out %lld", what, (long long)ldw, (long long)ldo);
     } else if ((((uintptr_t)w | (uintptr_t)ldw) & 15) || !float_aligned(out_type, out)) {
         set_error(CHIMERE_ERR_ARG, "%s: rows of 8-bit integers must be 16-byte aligned, out to its elements", what);
-    } else if (((int64_t)ntok + 31) / 32 * (((int64_t)nrows + 15) / 16) > 0x7FFFFFFF) {
+    } else if ((int64_t)ntok * nrows > I8_MAX_OUT) {
         set_error(CHIMERE_ERR_ARG, "%s: too many outputs (%d x %d)", what, ntok, nrows);
     } else {
         return true;

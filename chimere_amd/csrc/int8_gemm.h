@@ -6,12 +6,13 @@
 // each and 32 columns, every lane 16 consecutive bytes of one row.
 //
 // Staging: 128 columns of every row per step, copied global -> LDS in 16-byte
-// pieces by asynchronous copies, two stages.  A row's eight pieces are stored
-// at piece ^ (row & 7), so the 32 rows that a fragment read touches at the same
-// piece spread over all banks.  Rows behind the last one and pieces behind the
-// last column are read from clamped addresses: what a clamped row yields is
-// not stored, and the columns behind C are cleared in the token fragments of
-// the last step (their product with whatever the weight rows hold is 0).
+// pieces by asynchronous copies, two to four steps ahead.  A row's eight pieces
+// are stored at piece ^ (row / 2 & 7), so the rows that a fragment read touches
+// at the same piece spread over all banks.  Rows behind the last one and pieces
+// behind the last column are read from clamped addresses: what a clamped row
+// yields is not stored, and the columns behind C are cleared in the token
+// fragments of the last step (their product with whatever the weight rows hold
+// is 0).
 #pragma once
 #include <type_traits>
 
@@ -21,6 +22,8 @@ namespace chimere {
 
 constexpr int I8_BK = 128;              // columns per step
 constexpr int I8_MAX_C = 131071;        // |sum| <= 131071 * 2^14 < 2^31
+constexpr int I8_MAX_ROWS = 1 << 25;    // of either operand, and outputs: a grid has less than 2^32 threads
+constexpr int64_t I8_MAX_OUT = (int64_t)1 << 38;
 constexpr int I8_MAX_STRIDE = 1 << 23;  // bytes between rows: 256 rows of a tile stay within 32-bit offsets
 
 typedef int v4i __attribute__((ext_vector_type(4)));

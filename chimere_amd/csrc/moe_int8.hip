@@ -561,11 +561,15 @@ static void launch_many_pairs(const MoeI8& a, const MoeI8Plan& p, int type, int 
     else hipLaunchKernelGGL((k_i8_combine<_Float16, __bf16>), grid, dim3(256), 0, s, a);
 }
 
+// Sizes whose offsets within a tensor of tokens or of one expert stay below 2^31
+// and whose tiles make less than 2^24 work-groups (of 256 threads; with tiles
+// of 128 pairs half as many of 512)
 static bool moe_i8_shape(const chimere_moe_i8_layer* L, int K, int T) {
-    const int64_t lim = (int64_t)1 << 31;
-    return L->hidden >= 16 && L->hidden % 16 == 0 && L->hidden <= I8_MAX_C && L->ffn >= 16 && L->ffn % 16 == 0 &&
+    const int64_t lim = (int64_t)1 << 31, P = (int64_t)T * K;
+    const bool sizes = L->hidden >= 16 && L->hidden % 16 == 0 && L->hidden <= I8_MAX_C && L->ffn >= 16 && L->ffn % 16 == 0 &&
            L->ffn <= I8_MAX_C && (int64_t)L->hidden * L->ffn < lim && L->n_experts >= 1 && L->n_experts <= MAX_E &&
-           K >= 1 && K <= MAX_K && T >= 0 && (int64_t)T * L->hidden < lim && (int64_t)T * K < (1 << 24);
+           K >= 1 && K <= MAX_K && T >= 0 && (int64_t)T * L->hidden < lim && P < (1 << 24);
+    return sizes && (P / 64 + L->n_experts) * (L->ffn / 64 + L->hidden / 128 + 1) < (1 << 24);
 }
 
 }  // namespace chimere

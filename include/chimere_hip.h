@@ -296,13 +296,14 @@ void chimere_fused_moe_iq3s(const float *hidden, const void *gate_exps, const vo
 
 /* scale[r] = max |x[r]| * (1 / 127 as f32; torch's max / 127), q[r][c] =
  * x[r][c] / scale[r] rounded to the nearest integer, ties to even, and held
- * to +-127 (0 where the scale is 0).  A row that holds
- * an infinity or a NaN gets it as scale, and zeros.  Only the ncols integers
- * of a row are written.  For tokens and for weights (rows = channels). */
+ * to +-127 (0 where the scale is 0).  A row that holds an infinity or a NaN
+ * gets it as scale, and zeros.  Only the ncols integers of a row are written.
+ * For tokens and for weights (rows = channels); nrows below 2^31. */
 void chimere_quantize_i8(int type, const void *x, int64_t x_stride, int8_t *q, int64_t q_stride,
                          float *scale, int64_t nrows, int ncols, hipStream_t stream);
 /* out[t][r] = (sum_c a[t][c] w[r][c]) * a_scale[t] * w_scale[r] (+ bias[r]
- * unless NULL), rounded to out_type.  ncols at most 131071. */
+ * unless NULL), rounded to out_type.  ncols at most 131071, ntok and nrows at
+ * most 2^25 each, rows of integers at most 2^23 bytes apart. */
 void chimere_gemm_i8(const int8_t *a, int64_t a_stride, const float *a_scale, const int8_t *w,
                      int64_t w_stride, const float *w_scale, const float *bias, int out_type,
                      void *out, int64_t out_stride, int ntok, int nrows, int ncols,
@@ -325,7 +326,7 @@ void chimere_linear_i8(int type, const void *x, int64_t x_stride, const int8_t *
 typedef struct chimere_moe_i8_layer {
     int hidden;              /* H, multiple of 16 */
     int ffn;                 /* F, multiple of 16 */
-    int n_experts;           /* E <= 1024; top_k <= 16 */
+    int n_experts;           /* E <= 1024; top_k <= 16; ntok * top_k < 2^24, ntok * H < 2^31 */
     const int8_t *gate, *up; /* [E][F][H], 16-byte aligned */
     const int8_t *down;      /* [E][H][F] */
     const float *gate_scale, *up_scale; /* [E][F], 16-byte aligned as well */

@@ -97,6 +97,15 @@ def test_quantize_borders(dev, c):
     assert (q.double().cpu() == rq).all()
 
 
+def test_quantize_many_short_rows(dev):
+    """More rows than one grid of a wave each has threads for: a single element is its own maximum."""
+    n = (1 << 26) + 5
+    x = torch.randint(-3, 4, (n, 1), generator=gen(5), device=dev).to(torch.bfloat16)
+    q, s = int8.quantize_i8(x)
+    assert (q == torch.sign(x).to(torch.int8) * 127).all()
+    assert (s == x.abs().float().flatten() * torch.full((1,), 1.0 / 127, device=dev)).all()
+
+
 @pytest.mark.parametrize("power", [-140, -100, -89, -20, 0, 60, 115])
 def test_quantize_next_to_ties(dev, power):
     """16 million quotients within two steps of a half, for 1024 scales of every mantissa length."""

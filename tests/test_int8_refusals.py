@@ -41,7 +41,7 @@ def test_gemm():
     refuses("chimere_gemm_i8", good, a=(0, None, 1), lda=(1, 48, 1), lda_align=(1, 72, 1), a_align=(0, ODD, 1), a_scale=(2, None, 1),
             w=(3, None, 1), w_align=(3, ODD, 1), ldw=(4, 63, 1), ldw_far=(4, 1 << 24, 1), w_scale=(5, None, 1), type=(7, 8, 1),
             out=(8, None, 1), ldo=(9, 31, 1), ntok=(10, -1, 1), nrows=(11, 0, 1), ncols=(12, 0, 1), long=(12, 131072, 1),
-            out_align=(8, C.c_void_p(0x1002), 1))
+            out_align=(8, C.c_void_p(0x1002), 1), many_tok=(10, (1 << 25) + 1, 1), many_rows=(11, 0x7FFFFFFF, 1))
     good[10] = 0
     _lib.lib().chimere_gemm_i8(*good)
     assert err()[0] == 0
