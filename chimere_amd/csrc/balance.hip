@@ -25,9 +25,10 @@ struct Balance {
 };
 
 // LANES lanes per row, lane l of them the columns 4 LANES i + 4 l .. + 3 for
-// i < NV.  Sixteen up to 512 columns: a row of 256 is four loads of 16 bytes
+// i < NV.  Sixteen up to 256 columns: a row of 256 is four loads of 16 bytes
 // per lane, and the sums over a row are four DPP steps for four rows at once;
-// above, the whole wave, so that a lane keeps 16 values and as many sums.
+// above, the whole wave, 8 or 16 values and as many sums per lane (2048 rows
+// of 384: 15.0 us for loss and gradient, with 16 lanes 20.0).
 template <int LANES, int NV>
 struct BalRow {
     float v[4 * NV];

@@ -2,8 +2,8 @@
 against plain 64-bit forms.
 
 Tolerances, per element, u = 2^-24 (half a step of f32):
-* integers and scales of the quantizer: equal (both are defined by f32
-  quotients, which numpy rounds alike);
+* integers and scales of the quantizer: equal (defined by one f32 product and
+  f32 quotients, which numpy rounds alike);
 * a product: the int32 sum is exact; its conversion and the two scalings round
   once each (3 u of the product), the bias once (u of the result), and the
   result once more to the output type (eps / 2);
