@@ -362,7 +362,8 @@ void chimere_balance_loss(int type, const void *logits, int64_t logits_stride, c
  *            = *grad_loss * E / N * p_tj * (f_j - sum_e f_e p_te),
  * p_t = softmax(logits[t]), f_e = counts[e] / (N top_k) (constant: the choice
  * has no gradient); 0 in rows that the mask leaves out.  grad has the type of
- * the logits; counts and tokens are chimere_balance_loss's. */
+ * the logits and may not overlap them; counts and tokens are
+ * chimere_balance_loss's. */
 void chimere_balance_loss_grad(int type, const void *logits, int64_t logits_stride,
                                const uint8_t *mask, const int *counts, const int *tokens,
                                const float *grad_loss, int top_k, void *grad, int64_t grad_stride,

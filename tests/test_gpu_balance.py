@@ -264,3 +264,26 @@ def test_router_loss_and_experts_together(dev):
         assert (s[1].cpu() == rc).all() and int(s[3]) == T and abs(float(s[0]) - float(rl)) <= float(tl)
         assert ((s[2].double().cpu() - rp).abs() <= tp).all() and ((grad.double().cpu() - rg).abs() <= tg).all()
         close(out, *experts_ref(layer, x, ids, wts, torch.float32))
+
+
+def test_far_logits(dev):
+    """2.25 G logits, 2148 copies of 1024 rows: the loss, counts and probabilities of one copy, the gradient of each
+    row that of the one copy.  Sums of equal terms differ by their roundings: at most 1024 in a row of a lane, 512 over
+    waves and work-groups, on either side.  In a gradient c p (f - d), f has 3 roundings, d = sum f p those and at most
+    22 of its own, on either side, the rest 10; both are rounded to bf16 (half a step each)."""
+    copies, T, E, K = 2148, 1024, 1023, 4
+    print("far logits", flush=True)
+    x, ids, _ = choice(T, E, K, 3, torch.bfloat16, dev)
+    one = torch.ones(1, device=dev)
+    loss, counts, probs, tokens = routing.balance_loss(x, ids)
+    grad = routing.balance_loss_grad(x, counts, tokens, one, K).double()
+    big = x.repeat(copies, 1)
+    bl, bc, bp, bt = routing.balance_loss(big, ids.repeat(copies, 1))
+    bg = routing.balance_loss_grad(big, bc, bt, one * copies, K)
+    assert int(bt) == copies * T and torch.equal(bc, counts * copies)
+    tol = 2 * 1536 * U
+    assert ((bp - probs).abs() <= tol * probs).all() and abs(float(bl) - float(loss)) <= 2 * tol * float(loss)
+    p, f = torch.softmax(x.double(), 1), counts.double() / (T * K)
+    tol = E / T * p * (6 * f + 50 * (p @ f)[:, None]) * U + 10 * U * grad.abs() + 2.02 * STEP[x.dtype] * grad.abs()
+    for k in (0, copies // 2, copies - 1):
+        assert ((bg[k * T:(k + 1) * T].double() - grad).abs() <= tol).all(), k

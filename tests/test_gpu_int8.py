@@ -423,3 +423,64 @@ def test_every_address(dev, dtype):
             int8.linear_i8(x, w, ws, out=room[off:].view(m, 303)[:, :301])
             close(room[off:].view(m, 303)[:, :301], *product(*q_ref(x), w, ws, None, TYPES[dtype]))
             assert (room[:off] == 7.0).all() and (room[off:].view(m, 303)[:, 301:] == 7.0).all()
+
+
+# ------------------------------------------------------------ offsets past 32 bits
+
+def test_far_outputs(dev):
+    """2.4 G outputs: rows on both sides of 2^31 elements."""
+    m, n, c = 20000, 120000, 64
+    print(f"gemm {m}x{n}x{c}", flush=True)
+    g = gen(20)
+    a, s = weights(m, c, g)
+    w, ws = weights(n, c, g)
+    out = int8.gemm_i8(a, s, w, ws, dtype=torch.bfloat16)
+    at = torch.tensor([0, 1, 8947, 8948, 17895, 17896, 17897, 19999], device=dev)    # 2^31 / n = 17895.7
+    close(out[at], *product(a[at].double().cpu(), s[at].double().cpu(), w, ws, None, torch.bfloat16))
+
+
+@pytest.mark.parametrize("m", [3, 30, 300])
+def test_far_weights(dev, m):
+    """Weight rows 64 KB apart, 2.6 GB in all."""
+    n, c = 40000, 64
+    print(f"gemm far weights {m}", flush=True)
+    g = gen(m)
+    a, s = weights(m, c, g)
+    room = torch.empty(n, 1 << 16, dtype=torch.int8, device=dev)
+    room[:, :c], ws = weights(n, c, g)
+    w = room[:, :c]
+    close(int8.gemm_i8(a, s, w, ws), *product(a.double().cpu(), s.double().cpu(), w, ws, None, torch.float32))
+
+
+def test_far_rows_of_floats(dev):
+    """2.8 G elements in x and bytes in q."""
+    n, c = 70000, 40000
+    print(f"quantize {n}x{c}", flush=True)
+    x = torch.ones(n, c, dtype=torch.bfloat16, device=dev)
+    at = torch.tensor([0, 53687, 53688, 69999], device=dev)
+    x[at] = torch.randn(4, c, generator=gen(4), device=dev).to(x.dtype)
+    q, s = int8.quantize_i8(x)
+    rq, rs = q_ref(x[at])
+    assert (q[at].double().cpu() == rq).all() and (s[at].double().cpu() == rs).all()
+    assert (q[1] == 127).all() and (q[-2] == 127).all()
+
+
+@pytest.mark.parametrize("T", [1, 9, 400])
+def test_far_experts(dev, T):
+    """Experts behind 2^31 bytes of each tensor: as the same experts on their own."""
+    E, H, F, n, K = 530, 2048, 2048, 12, 4
+    print(f"far experts T={T}", flush=True)
+    g = gen(T)
+    big, small = [], []
+    for rows, cols in ((F, H), (F, H), (H, F)):
+        w = torch.empty(E, rows, cols, dtype=torch.int8, device=dev)
+        w[-n:] = torch.randint(-128, 128, (n, rows, cols), generator=g, device=dev, dtype=torch.int8)
+        s = torch.rand(E, rows, generator=g, device=dev) * 1e-3
+        big += [w, s]
+        small += [w[-n:].clone(), s[-n:].clone()]
+    x = torch.randn(T, H, generator=g, device=dev)
+    ids = torch.rand(T, n, generator=g, device=dev).topk(K, 1)[1].to(torch.int32)
+    wts = torch.rand(T, K, generator=g, device=dev)
+    far = int8.Int8Experts(*big).forward(x, ids + (E - n), wts)
+    near = int8.Int8Experts(*small).forward(x, ids, wts)
+    assert torch.equal(far, near) and bool(near.abs().sum() > 0)
