@@ -94,9 +94,10 @@ __global__ __launch_bounds__(64 * Tile::NW, WAVES_PER_SIMD) void k_i8_gemm(I8Gem
 // int32 sums are joined in LDS.  With X, tokens are floats that every
 // work-group quantizes for itself (one launch less); their integers lie in
 // LDS, cleared up to whole steps.
-constexpr int FEW_WAVES = 8, FEW_KEEP = 16;   // elements that a thread quantizes at most
+constexpr int FEW_WAVES = 8;
 
-template <typename T, typename X, int MB, int NB>
+// KEEP: elements that a thread quantizes at most
+template <typename T, typename X, int MB, int NB, int KEEP = 16>
 __global__ __launch_bounds__(64 * FEW_WAVES) void k_i8_few(I8Gemm g) {
     constexpr bool QUANT = !std::is_same<X, int8_t>::value;
     extern __shared__ __align__(16) uint8_t lds[];
@@ -139,7 +140,7 @@ __global__ __launch_bounds__(64 * FEW_WAVES) void k_i8_few(I8Gemm g) {
     float* as = (float*)lds;   // [16 MB]
     uint8_t* aq = lds + 16 * MB * 4;
     if constexpr (QUANT) {
-        i8_rows_to_lds<64 * FEW_WAVES, FEW_KEEP>(M, S * I8_BK, lda, as, aq, [&](int m, int c, auto& v) {
+        i8_rows_to_lds<64 * FEW_WAVES, KEEP>(M, S * I8_BK, lda, as, aq, [&](int m, int c, auto& v) {
             i8_load((const X*)g.x + (m0 + m) * g.ldx, c, g.C, v);
         }, std::integral_constant<int, 16 / sizeof(X)>{});
     } else {
@@ -194,13 +195,13 @@ __global__ __launch_bounds__(64 * FEW_WAVES) void k_i8_few(I8Gemm g) {
     }
 }
 
-template <typename T, typename X, int MB, int NB>
+template <typename T, typename X, int MB, int NB, int KEEP = 16>
 static void launch_few(const I8Gemm& g, hipStream_t s) {
     const size_t aq = std::is_same<X, int8_t>::value
                           ? 0 : (size_t)(g.M < 16 * MB ? g.M : 16 * MB) * (pad_to(g.C, I8_BK) + 16);
     const size_t part = (size_t)FEW_WAVES * MB * NB * 256 * 4;
     const dim3 grid((g.N + 16 * NB - 1) / (16 * NB), (g.M + 16 * MB - 1) / (16 * MB));
-    hipLaunchKernelGGL((k_i8_few<T, X, MB, NB>), grid, dim3(64 * FEW_WAVES), 16 * MB * 4 + (aq > part ? aq : part), s, g);
+    hipLaunchKernelGGL((k_i8_few<T, X, MB, NB, KEEP>), grid, dim3(64 * FEW_WAVES), 16 * MB * 4 + (aq > part ? aq : part), s, g);
 }
 
 template <typename T, typename Tile, int WAVES_PER_SIMD>
@@ -249,20 +250,26 @@ static void launch_gemm(const I8Gemm& g, hipStream_t s) {
     }
 }
 
-// A few float tokens: quantized by every work-group, one launch instead of two,
-// as long as they fit its threads' registers: one or two tokens (GPU time in
-// one / two launches: 1x4096x2048 5.7 / 6.6 us, 2x4096x2048 5.9 / 6.7,
-// 1x151936x2048 51 / 55), and up to four where the work-groups are few
-// (4x4096x2048 7.3 / 6.8, but the second launch and its workspace cost the
-// calling thread another 3.8 us, of 7.1; 4x16384x2048 12.6 / 11.3).
-static bool needs_no_workspace(int ntok, int ncols) {
-    return ntok <= 2 && ntok * pad_to(ncols, I8_BK) <= 64 * FEW_WAVES * FEW_KEEP;
-}
-static bool quantizes_itself(int ntok, int nrows, int ncols) {
-    return ntok <= (nrows <= FEW_N ? 4 : 2) && ntok * pad_to(ncols, I8_BK) <= 64 * FEW_WAVES * FEW_KEEP;
+// Float tokens that every work-group quantizes for itself, one launch instead
+// of two (and nothing in the workspace): 16 tokens of a work-group as long as
+// they fit its threads' registers, 32 KB.  One or two tokens always, more while
+// the elements quantized by all work-groups together are 4 M at most (the
+// calling thread 7.6 us instead of 9.9 then; GPU time in one / two launches,
+// f32, bf16): 1x4096x2048 5.7 / 6.6, 1x151936x2048 51 / 55, 8x4096x1024 4.7 /
+// 5.4, 4.0 / 5.0, 16x2048x512 4.6 / 4.9, 3.8 / 4.7, 64x2048x512 5.9 / 6.0, 4.7 /
+// 5.9, 8x4096x2048 bf16 5.8 / 5.8; but 16x8192x1024 bf16 7.2 / 6.1, 32x8192x512
+// 8.5 / 6.4, 6.7 / 6.1, 4x16384x2048 12.6 / 11.3.
+static int few_elements(int ntok, int ncols) { return min(ntok, 16) * pad_to(ncols, I8_BK); }
+static bool needs_no_workspace(int ntok, int ncols) { return ntok <= 2 && few_elements(ntok, ncols) <= 8192; }
+static bool quantizes_itself(int type, int ntok, int nrows, int ncols) {
+    if (needs_no_workspace(ntok, ncols)) return true;
+    const int64_t groups = (int64_t)((ntok + 15) / 16) * ((nrows + 15) / 16), n = few_elements(ntok, ncols);
+    return n <= (type == T_F32 ? 8192 : 16384) && groups * n <= 1 << 22 && (ntok <= 16 || groups <= 512);
 }
 template <typename T, typename X>
 static void launch_few_quantizing(const I8Gemm& g, hipStream_t s) {
+    if constexpr (sizeof(X) == 2)
+        if (few_elements(g.M, g.C) > 8192) return launch_few<T, X, 1, 1, 32>(g, s);
     if (g.N <= FEW_N) launch_few<T, X, 1, 1>(g, s);
     else launch_few<T, X, 1, 2>(g, s);
 }
@@ -356,7 +363,7 @@ void chimere_linear_i8(int type, const void* x, int64_t x_stride, const int8_t* 
     int8_t* q = (int8_t*)workspace;
     float* as = (float*)((uint8_t*)workspace + al256((size_t)ntok * lda));
     const I8Gemm g{q, w, as, w_scale, bias, out, lda, w_stride, out_stride, ntok, nrows, ncols, x, x_stride};
-    if (quantizes_itself(ntok, nrows, ncols)) {
+    if (quantizes_itself(type, ntok, nrows, ncols)) {
         if (out_type == T_F32) launch_few_quantizing<float>(type, g, stream);
         else if (out_type == T_F16) launch_few_quantizing<_Float16>(type, g, stream);
         else launch_few_quantizing<__bf16>(type, g, stream);

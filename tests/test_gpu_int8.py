@@ -204,7 +204,9 @@ def test_gemm_strides_and_what_is_left(dev, m, n, c):
 
 @pytest.mark.parametrize("xt", TYPES)
 @pytest.mark.parametrize("m,n,c", [(1, 4096, 2048), (1, 5, 1), (1, 1000, 4097), (2, 70, 300), (3, 1000, 2048), (8, 513, 1024), (12, 100, 9000), (4, 8192, 2048), (4, 500, 2049), (3, 8200, 512), (2, 9001, 4000), (1, 8193, 8192), (1, 40, 8193),
-                                   (40, 300, 500), (300, 500, 129)])
+                                   (40, 300, 500), (300, 500, 129), (16, 2048, 512), (17, 700, 480), (64, 2048, 512), (100, 90, 512),
+                                   (500, 200, 256), (513, 250, 100), (8, 300, 2048), (16, 1000, 1000), (40, 513, 1024), (33, 100, 1025),
+                                   (8, 16384, 512), (5, 16400, 500), (5, 1, 3000), (1000, 1, 16), (2, 8192, 8192)])
 def test_linear(dev, m, n, c, xt):
     print(f"linear {m}x{n}x{c} {xt}", flush=True)
     g = gen(m + n + c)
@@ -236,6 +238,11 @@ def test_linear_rows_do_not_depend_on_each_other(dev):
         print(f"linear rows {m}", flush=True)
         part = int8.linear_i8(x[:m], w, ws)
         same = (part == full[:m]) | (part.isnan() & full[:m].isnan())
+        assert same.all(), m
+    w = w[:300]
+    for m in range(1, 120, 7):          # few work-groups: quantized by each
+        part = int8.linear_i8(x[:m], w, ws[:300])
+        same = (part == full[:m, :300]) | (part.isnan() & full[:m, :300].isnan())
         assert same.all(), m
 
 
