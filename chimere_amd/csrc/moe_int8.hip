@@ -46,7 +46,7 @@ struct MoeI8 {
 
 // ------------------------------------------------------------ few pairs
 
-constexpr int FP_WAVES = 8, FP_KEEP = 16, FP_AHEAD = 4;   // FP_AHEAD: a wave's pieces of work whose weights are loaded ahead
+constexpr int FP_WAVES = 8, FP_KEEP = 16, FP_KEEP_H = 64, FP_AHEAD = 4;   // FP_AHEAD: a wave's pieces of work whose weights are loaded ahead
 
 // Grid (F / 16, pairs): 16 columns of F of one pair, gate and up.  Steps of 128
 // columns of H dealt to the eight waves; the one token is row 0 of the matrix
@@ -118,7 +118,7 @@ __global__ __launch_bounds__(64 * FP_WAVES) void k_i8_pair_gate_up(MoeI8 a) {
 // the weights and row 0 of h, one in rows 8 .. 15 and row 1: twice the
 // work-groups, where 16 columns would leave half of the CUs idle (one token
 // of H = 2048: 7.3 us with 16, 6.6 with 8).
-template <typename T, int COLS>
+template <typename T, int COLS, int KEEP>
 __global__ __launch_bounds__(64 * FP_WAVES) void k_i8_pair_down(MoeI8 a) {
     constexpr int PER = 16 / COLS;                   // pieces per instruction
     extern __shared__ __align__(16) uint8_t lds[];   // integers of h
@@ -147,7 +147,7 @@ __global__ __launch_bounds__(64 * FP_WAVES) void k_i8_pair_down(MoeI8 a) {
     if (tid < MAX_K * COLS) (&sum[0][0])[tid] = 0;
     // (a pair that was left out: whatever its row holds, its sums are not used)
     const int lda = S * I8_BK;
-    i8_rows_to_lds<64 * FP_WAVES, FP_KEEP>(
+    i8_rows_to_lds<64 * FP_WAVES, KEEP>(
         a.K, S * I8_BK, lda, hs, lds,
         [&](int k, int c, auto& v) { i8_load(a.h + ((int64_t)t * a.K + k) * a.F, c, a.F, v); },
         std::integral_constant<int, 4>{});
@@ -458,9 +458,12 @@ constexpr double MOE_AGAIN = 50e6;
 constexpr int MOE_PAIRS = 256;   // of small experts too (256, 128, 8, 2; 512 pairs: 23 / 38)
 static bool moe_few(int H, int F, int E, int K, int64_t P) {
     const double again = P - E * (1.0 - pow(1.0 - 1.0 / E, (double)P));
-    // rows that fit the work-groups' registers
+    // rows that fit the work-groups' registers (a token's rows of h: 16, 32 or 64
+    // elements of a thread; one token, together / on its own: H 2048, F 1536,
+    // top-8 42 / 27 us, 4096, 4096, top-4 76 / 51, 2048, 4096, top-8 67 / 60; but
+    // 2048, 2048, top-16 54 / 57, 1024, 2048, top-16 36 / 41)
     return P <= MOE_PAIRS && again * 3.0 * H * F <= MOE_AGAIN && pad_to(H, I8_BK) <= 64 * FP_WAVES * FP_KEEP &&
-           K * pad_to(F, I8_BK) <= 64 * FP_WAVES * FP_KEEP;
+           K * pad_to(F, I8_BK) <= 64 * FP_WAVES * (K <= 8 ? FP_KEEP_H : FP_KEEP_H / 2);
 }
 // Pairs per tile: 128 instead of 64 where an expert meets more than 40 on
 // average (H = 2048, F = 512, 256 experts, top-8, us, tiles of 64 / 128: average 16
@@ -496,13 +499,15 @@ static MoeI8Plan plan_moe_i8(int H, int F, int E, int K, int T) {
     return p;
 }
 
-template <int COLS>
+template <int COLS, int KEEP = FP_KEEP>
 static void launch_pair_down(const MoeI8& a, int out_type, hipStream_t s) {
     const dim3 grid(a.H / COLS, a.T), block(64 * FP_WAVES);
     const size_t lh = a.K * pad_to(a.F, I8_BK);
-    if (out_type == T_F32) hipLaunchKernelGGL((k_i8_pair_down<float, COLS>), grid, block, lh, s, a);
-    else if (out_type == T_F16) hipLaunchKernelGGL((k_i8_pair_down<_Float16, COLS>), grid, block, lh, s, a);
-    else hipLaunchKernelGGL((k_i8_pair_down<__bf16, COLS>), grid, block, lh, s, a);
+    if constexpr (KEEP < FP_KEEP_H)
+        if (lh > 64 * FP_WAVES * KEEP) return launch_pair_down<COLS, 2 * KEEP>(a, out_type, s);
+    if (out_type == T_F32) hipLaunchKernelGGL((k_i8_pair_down<float, COLS, KEEP>), grid, block, lh, s, a);
+    else if (out_type == T_F16) hipLaunchKernelGGL((k_i8_pair_down<_Float16, COLS, KEEP>), grid, block, lh, s, a);
+    else hipLaunchKernelGGL((k_i8_pair_down<__bf16, COLS, KEEP>), grid, block, lh, s, a);
 }
 
 static void launch_few_pairs(const MoeI8& a, int type, int out_type, hipStream_t s) {

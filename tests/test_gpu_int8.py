@@ -301,7 +301,9 @@ def routed(T, E, K, g, dev):
                                        (8, 64, 8, 512, 128), (9, 8, 2, 128, 1040), (33, 3, 2, 144, 80), (40, 64, 8, 256, 192),
                                        (200, 8, 4, 272, 320), (300, 2, 1, 128, 64), (500, 40, 6, 512, 256), (700, 16, 16, 192, 512),
                                        (1500, 5, 2, 256, 704), (90, 40, 8, 256, 192), (300, 100, 3, 320, 208), (130, 50, 4, 144, 80),
-                                       (1030, 1000, 2, 64, 32), (600, 8, 1, 1040, 272), (200, 30, 3, 160, 1040), (20, 2, 2, 4096, 2048)])
+                                       (1030, 1000, 2, 64, 32), (600, 8, 1, 1040, 272), (200, 30, 3, 160, 1040), (20, 2, 2, 4096, 2048),
+                                       (1, 16, 8, 384, 1152), (2, 16, 8, 256, 2048), (1, 16, 8, 256, 4096), (3, 12, 4, 272, 4112), (1, 40, 16, 144, 1024),
+                                       (1, 20, 16, 128, 2048), (1, 9, 1, 4096, 8192)])
 def test_experts(dev, T, E, K, H, F):
     g = gen(T + E)
     layer = layer_of(E, F, H, T * E, dev)
