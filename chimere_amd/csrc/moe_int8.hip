@@ -6,9 +6,10 @@
 // Bound by the selected experts' weights: each byte of them is read from
 // memory once.  A few pairs of (token, expert), two launches: gate and up of
 // each pair (every work-group quantizes its token), then per token h to 8 bits,
-// down and the weighted sum.  More: rows of x to 8 bits; the pairs of each
-// expert together, with the list of tiles; gate and up product with
-// h = silu(g) u; rows of h to 8 bits; down product; each token's weighted sum.
+// down and the weighted sum.  More, five or six: rows of x to 8 bits and the
+// pairs of each expert together, with the list of tiles (above 4096 pairs that
+// takes a launch more); gate and up product with h = silu(g) u; rows of h to 8
+// bits; down product; each token's weighted sum.
 #include <math.h>
 
 #include <type_traits>
