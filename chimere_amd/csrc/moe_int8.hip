@@ -38,8 +38,7 @@ struct MoeI8 {
     float* h;              // [pairs][F], in sorted order (few pairs: by pair)
     int8_t* hq;
     float* hs;             // by pair
-    void* y;               // [pairs][H], by pair: f32, or f16 of sum * 2^-shift
-    int shift;
+    void* y;               // [pairs][H], by pair: scaled f32, or sums in 24 bits
     void* out;
     int64_t ldo;
     int tile_pairs;
@@ -297,11 +296,28 @@ __device__ __forceinline__ void i8_gate_up(const MoeI8& a, const int4& t, int f0
     });
 }
 
-// Down of a tile.  Y = float: the scaled products.  Y = _Float16 (16-bit
-// outputs): the integer sums times 2^-shift, so that none exceeds f16's range
-// and each is off by 2^-11 of itself at most, whatever the scales, which the
-// weighted sum applies (16-bit rows halve what 32768 pairs of 2048 columns
-// write and read again, 268 MB each way).
+// Four sums of 24 bits each.  Sums of F products are 16256 F at most, so up to
+// F = 512 nothing is lost, and an f32 output is the same as from f32 rows.
+struct I24x4 {
+    uint32_t w[3];
+    __device__ __forceinline__ void pack(const int (&x)[4]) {
+        w[0] = (x[0] & 0xFFFFFF) | (uint32_t)x[1] << 24;
+        w[1] = ((uint32_t)x[1] >> 8 & 0xFFFF) | (uint32_t)x[2] << 16;
+        w[2] = ((uint32_t)x[2] >> 16 & 0xFF) | (uint32_t)x[3] << 8;
+    }
+    __device__ __forceinline__ void unpack(int (&x)[4]) const {
+        x[0] = (int)(w[0] << 8) >> 8;
+        x[1] = (int)(w[1] << 16 | w[0] >> 24 << 8) >> 8;
+        x[2] = (int)(w[2] << 24 | w[1] >> 16 << 8) >> 8;
+        x[3] = (int)w[2] >> 8;
+    }
+};
+constexpr int MAX_F24 = ((1 << 23) - 1) / (127 * 128);
+
+// Down of a tile.  Y = float4: the scaled products.  Y = I24x4: the integer
+// sums, which the weighted sum scales (the rows of 32768 pairs of 2048 columns
+// are 201 MB instead of 268, written and read again).  An output is rounded
+// once either way, whatever its type, and does not depend on the other tokens.
 template <typename Tile, typename Y>
 __device__ __forceinline__ void i8_down(const MoeI8& a, const int4& t, int n0, uint8_t* lds) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -314,24 +330,22 @@ __device__ __forceinline__ void i8_down(const MoeI8& a, const int4& t, int n0, u
         woff[p] = (uint32_t)min(n0 + (wave * Tile::PN + p) * 8 + (lane >> 3), a.H - 1) * (uint32_t)a.F;
     const int64_t e = t.x;
     const int pair = threadIdx.x < Tile::BM ? a.order[t.y + min((int)threadIdx.x, t.z - 1)] : 0;
-    const float2 mine = make_float2(sizeof(Y) == 4 ? a.hs[pair] : 0.0f, __builtin_bit_cast(float, pair));
-    constexpr int VEC = 16 / sizeof(Y);
+    constexpr bool SUMS = std::is_same<Y, I24x4>::value;
+    const float2 mine = make_float2(SUMS ? 0.0f : a.hs[pair], __builtin_bit_cast(float, pair));
+    constexpr int VEC = 4;
     const int n = n0 + Tile::template first_col<VEC>();
     const bool in = n < a.H;   // H is a multiple of 16: all columns or none
-    float sd[VEC];
-#pragma unroll
-    for (int k = 0; k < VEC; k++) sd[k] = sizeof(Y) == 4 && in ? a.down_s[e * a.H + n + k] : 0.0f;
+    const float4 sd = !SUMS && in ? *(const float4*)(a.down_s + e * a.H + n) : float4{};
     v16i acc[Tile::MTILES][Tile::NTILES];
     const int8_t* w = a.down + e * a.H * a.F;
     Tile::run(a.hq + (int64_t)t.y * a.F, w, w, aoff, woff, a.F, lds, acc);
-    const float unit = __builtin_ldexpf(1.0f, -a.shift);
     Tile::template rows<VEC>(lds, acc, mine, [&](int r, const int(&x)[VEC], float2 of_row) {
         if (r >= t.z || !in) return;
-        float v[VEC];
-#pragma unroll
-        for (int k = 0; k < VEC; k++)
-            v[k] = sizeof(Y) == 4 ? (float)x[k] * of_row.x * sd[k] : (float)x[k] * unit;
-        store_row((Y*)a.y + (int64_t)__builtin_bit_cast(int, of_row.y) * a.H + n, v, VEC);
+        const float s = of_row.x;
+        Y y;
+        if constexpr (SUMS) y.pack(x);
+        else y = make_float4((float)x[0] * s * sd.x, (float)x[1] * s * sd.y, (float)x[2] * s * sd.z, (float)x[3] * s * sd.w);
+        ((Y*)a.y)[((int64_t)__builtin_bit_cast(int, of_row.y) * a.H + n) / VEC] = y;
     });
 }
 
@@ -401,44 +415,48 @@ void k_i8_down(MoeI8 a) {
 
 // out[t] = sum over k, ascending, of w[t][k] y[t][k]; a pair that was left out
 // adds nothing (its row of y, not written by this call, is read but not used).
-// A thread takes VEC neighbouring columns, eight pairs' loads at a time.
+// A thread takes four neighbouring columns, eight pairs' loads at a time.
 template <typename Y, typename T>
 __global__ __launch_bounds__(256) void k_i8_combine(MoeI8 a) {
-    constexpr int VEC = 16 / sizeof(Y), AT = 8;
-    typedef Y vec __attribute__((ext_vector_type(VEC)));
+    constexpr bool SUMS = std::is_same<Y, I24x4>::value;
+    constexpr int VEC = 4, AT = 8;
     const int hb = (a.H / VEC + 255) / 256, t = blockIdx.x / hb, n = ((blockIdx.x - t * hb) * 256 + threadIdx.x) * VEC;
     if (n >= a.H) return;   // H is a multiple of 16
     const int64_t p0 = (int64_t)t * a.K;
-    const float unit = __builtin_ldexpf(1.0f, a.shift);
     float acc[VEC] = {};
     for (int k0 = 0; k0 < a.K; k0 += AT) {
-        vec y[AT];
-        float sd[AT][VEC], w[AT], hs[AT];
+        Y y[AT];
+        float4 sd[AT];
+        float w[AT], hs[AT];
         int e[AT];
 #pragma unroll
         for (int i = 0; i < AT; i++) {
             const int64_t p = p0 + min(k0 + i, a.K - 1);
-            y[i] = *(const vec*)((const Y*)a.y + p * a.H + n);
+            y[i] = ((const Y*)a.y)[(p * a.H + n) / VEC];
             e[i] = k0 + i < a.K ? a.ids[p] : -1;
             w[i] = a.wts[p];
-            hs[i] = sizeof(Y) == 2 ? a.hs[p] : 0.0f;
+            hs[i] = SUMS ? a.hs[p] : 0.0f;
         }
 #pragma unroll
-        for (int i = 0; i < AT; i++) {
-            if (sizeof(Y) == 2 && (unsigned)e[i] < (unsigned)a.E) {
-#pragma unroll
-                for (int c = 0; c < VEC; c += 4)
-                    *(float4*)(sd[i] + c) = *(const float4*)(a.down_s + (int64_t)e[i] * a.H + n + c);
-            }
-        }
+        for (int i = 0; i < AT; i++)
+            if (SUMS && (unsigned)e[i] < (unsigned)a.E) sd[i] = *(const float4*)(a.down_s + (int64_t)e[i] * a.H + n);
 #pragma unroll
         for (int i = 0; i < AT; i++) {
             if ((unsigned)e[i] < (unsigned)a.E) {
-#pragma unroll
-                for (int c = 0; c < VEC; c++) {
-                    const float v = sizeof(Y) == 2 ? (float)y[i][c] * unit * hs[i] * sd[i][c] : (float)y[i][c];
-                    acc[c] = __builtin_fmaf(w[i], v, acc[c]);
+                float4 v;
+                if constexpr (SUMS) {
+                    int x[VEC];
+                    y[i].unpack(x);
+                    const float s = hs[i];
+                    v = make_float4((float)x[0] * s * sd[i].x, (float)x[1] * s * sd[i].y, (float)x[2] * s * sd[i].z,
+                                    (float)x[3] * s * sd[i].w);
+                } else {
+                    v = y[i];
                 }
+                acc[0] = __builtin_fmaf(w[i], v.x, acc[0]);
+                acc[1] = __builtin_fmaf(w[i], v.y, acc[1]);
+                acc[2] = __builtin_fmaf(w[i], v.z, acc[2]);
+                acc[3] = __builtin_fmaf(w[i], v.w, acc[3]);
             }
         }
     }
@@ -543,28 +561,33 @@ static void launch_hidden(const MoeI8& a, hipStream_t s) {
 }
 
 template <int ROWS>
-static void launch_tiles(const MoeI8& a, int max_tiles, bool half, hipStream_t s) {
+static void launch_tiles(const MoeI8& a, int max_tiles, hipStream_t s) {
     constexpr int BN = MoeTile<ROWS>::BN;
     const dim3 block(64 * MoeTile<ROWS>::WAVES);
     const dim3 gu((unsigned)((max_tiles * ((a.F + BN / 2 - 1) / (BN / 2)) + 7) / 8 * 8));
     const dim3 dn((unsigned)((max_tiles * ((a.H + BN - 1) / BN) + 7) / 8 * 8));
     hipLaunchKernelGGL(k_i8_gate_up<ROWS>, gu, block, 0, s, a);
     launch_hidden(a, s);
-    if (half) hipLaunchKernelGGL((k_i8_down<ROWS, _Float16>), dn, block, 0, s, a);
-    else hipLaunchKernelGGL((k_i8_down<ROWS, float>), dn, block, 0, s, a);
+    if (a.F <= MAX_F24) hipLaunchKernelGGL((k_i8_down<ROWS, I24x4>), dn, block, 0, s, a);
+    else hipLaunchKernelGGL((k_i8_down<ROWS, float4>), dn, block, 0, s, a);
+}
+
+template <typename Y>
+static void launch_combine(const MoeI8& a, int out_type, hipStream_t s) {
+    const dim3 grid((unsigned)((a.H / 4 + 255) / 256) * a.T);
+    if (out_type == T_F32) hipLaunchKernelGGL((k_i8_combine<Y, float>), grid, dim3(256), 0, s, a);
+    else if (out_type == T_F16) hipLaunchKernelGGL((k_i8_combine<Y, _Float16>), grid, dim3(256), 0, s, a);
+    else hipLaunchKernelGGL((k_i8_combine<Y, __bf16>), grid, dim3(256), 0, s, a);
 }
 
 static void launch_many_pairs(const MoeI8& a, const MoeI8Plan& p, int type, int out_type, hipStream_t s) {
     if (type == T_F32) launch_prepare<float>(a, s);
     else if (type == T_F16) launch_prepare<_Float16>(a, s);
     else launch_prepare<__bf16>(a, s);
-    const bool half = out_type != T_F32;
-    if (p.tile_pairs == 64) launch_tiles<64>(a, p.max_tiles, half, s);
-    else launch_tiles<128>(a, p.max_tiles, half, s);
-    const dim3 grid((unsigned)((a.H / (half ? 8 : 4) + 255) / 256) * a.T);
-    if (out_type == T_F32) hipLaunchKernelGGL((k_i8_combine<float, float>), grid, dim3(256), 0, s, a);
-    else if (out_type == T_F16) hipLaunchKernelGGL((k_i8_combine<_Float16, _Float16>), grid, dim3(256), 0, s, a);
-    else hipLaunchKernelGGL((k_i8_combine<_Float16, __bf16>), grid, dim3(256), 0, s, a);
+    if (p.tile_pairs == 64) launch_tiles<64>(a, p.max_tiles, s);
+    else launch_tiles<128>(a, p.max_tiles, s);
+    if (a.F <= MAX_F24) launch_combine<I24x4>(a, out_type, s);
+    else launch_combine<float4>(a, out_type, s);
 }
 
 // Sizes whose offsets within a tensor of tokens or of one expert stay below 2^31
@@ -627,7 +650,6 @@ void chimere_moe_i8(const chimere_moe_i8_layer* L, int type, const void* x, int6
         a.total = (int*)(w + p.total); a.cnt = (int*)(w + p.cnt); a.tiles = (int4*)(w + p.tiles);
         a.hq = (int8_t*)(w + p.hq); a.hs = (float*)(w + p.hs); a.y = w + p.y;
         a.tile_pairs = p.tile_pairs;
-        while ((16256.0 * F) / (double)((int64_t)1 << a.shift) > 65504.0) a.shift++;
         launch_many_pairs(a, p, type, out_type, stream);
     }
     check_launch("moe_i8");

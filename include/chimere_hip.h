@@ -292,7 +292,7 @@ void chimere_fused_moe_iq3s(const float *hidden, const void *gate_exps, const vo
  * stride, in bytes), and what lies between their ncols integers and the next
  * multiple of 16 is read but does not matter.  Outputs may not overlap
  * inputs.  ntok = 0 launches nothing.  Sums of products are exact (int32), so
- * results repeat bit for bit; a token's f32 results do not depend on ntok. */
+ * results repeat bit for bit; a token's results do not depend on ntok. */
 
 /* scale[r] = max |x[r]| * (1 / 127 as f32; torch's max / 127), q[r][c] =
  * x[r][c] / scale[r] rounded to the nearest integer, ties to even, and held
