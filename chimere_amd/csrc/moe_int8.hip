@@ -107,7 +107,7 @@ __global__ __launch_bounds__(64 * FP_WAVES) void k_i8_pair_gate_up(MoeI8 a) {
             gs += part[i][0][tid];
             us += part[i][1][tid];
         }
-        a.h[(int64_t)p * a.F + f0 + tid] = fast_silu((float)gs * *xs * sg) * ((float)us * *xs * su);
+        a.h[(int64_t)p * a.F + f0 + tid] = silu((float)gs * *xs * sg) * ((float)us * *xs * su);
     }
 }
 
@@ -288,10 +288,10 @@ __device__ __forceinline__ void i8_gate_up(const MoeI8& a, const int4& t, int f0
         if (r >= t.z || !in) return;
         const float s = of_row.x;
         float4 h;
-        h.x = fast_silu((float)g[0] * s * sg.x) * ((float)u[0] * s * su.x);
-        h.y = fast_silu((float)g[1] * s * sg.y) * ((float)u[1] * s * su.y);
-        h.z = fast_silu((float)g[2] * s * sg.z) * ((float)u[2] * s * su.z);
-        h.w = fast_silu((float)g[3] * s * sg.w) * ((float)u[3] * s * su.w);
+        h.x = silu((float)g[0] * s * sg.x) * ((float)u[0] * s * su.x);
+        h.y = silu((float)g[1] * s * sg.y) * ((float)u[1] * s * su.y);
+        h.z = silu((float)g[2] * s * sg.z) * ((float)u[2] * s * su.z);
+        h.w = silu((float)g[3] * s * sg.w) * ((float)u[3] * s * su.w);
         *(float4*)(a.h + (int64_t)(t.y + r) * a.F + f) = h;
     });
 }

@@ -118,3 +118,23 @@ def test_largest_sums(dev, F):
         scale = out[0, 1].double() / (1.5 * 127 * 127 * F)                 # of h's row times that of down
         want = torch.where(torch.arange(H, device=dev) % 2 == 0, -128.0, 127.0).double() * 127 * F * scale * 1.5
         assert bool(((out.double() - want).abs() <= 2.0 ** -22 * want.abs()).all()) and bool((out[:, 0] < 0).all())
+
+
+@pytest.mark.parametrize("T,F", [(2, 512), (30000, 512), (8000, 1040)])
+def test_as_the_calls_one_by_one(dev, T, F):
+    """The integers of h are those of silu(g) u in f32 operations that round to nearest each: gate, up and down as products
+    of their own and h as torch computes it in between give the same bits.  (An h that is off by a step or two moves a
+    few of 15 million integers.)"""
+    E, H = 2, 64
+    layer, g = layer_of(E, F, H, F, dev), gen(T)
+    x = torch.randn(T, H, generator=g, device=dev) * 8
+    ids = torch.randint(0, E, (T, 1), generator=g, device=dev).to(torch.int32)
+    print(f"experts one by one T={T} F={F}", flush=True)
+    out = layer.forward(x, ids, torch.ones(T, 1, device=dev))
+    gate, gs, up, us, down, ds = layer.tensors
+    for e in range(E):
+        q, s = int8.quantize_i8(x)
+        a, b = int8.gemm_i8(q, s, gate[e], gs[e]), int8.gemm_i8(q, s, up[e], us[e])
+        want = int8.linear_i8(a / (1 + torch.exp(-a)) * b, down[e], ds[e])
+        here = ids[:, 0] == e
+        assert same(out[here], want[here]), (e, int((out[here] != want[here]).any(1).sum()))
