@@ -14,19 +14,15 @@ __global__ __launch_bounds__(256) void k_i8_quantize(I8Rows<T> q) {
     i8_quantize_rows<T, W, 256>(q, blockIdx.x);
 }
 
-// (2^24 rows per launch: a grid has less than 2^32 threads)
 template <typename T>
 static void launch_i8_quantize(const T* x, int64_t xs, int8_t* q, int64_t qs, float* scale, int64_t nrows, int ncols,
                                hipStream_t s) {
-    constexpr int64_t AT_ONCE = 1 << 24;
-    const int per = i8_rows_per_group<256>(ncols);
-    for (int64_t r = 0; r < nrows; r += AT_ONCE) {
-        const int64_t n = nrows - r < AT_ONCE ? nrows - r : AT_ONCE;
+    i8_slices<256>(nrows, ncols, [&](int64_t r, int64_t n, int64_t groups) {
         const I8Rows<T> rows{x + r * xs, xs, q + r * qs, qs, scale + r, nullptr, nullptr, n, ncols};
-        const dim3 grid((unsigned)((n + per - 1) / per));
+        const dim3 grid((unsigned)groups);
         if (ncols <= I8_WAVE_ROW) hipLaunchKernelGGL((k_i8_quantize<T, 1>), grid, dim3(256), 0, s, rows);
         else hipLaunchKernelGGL((k_i8_quantize<T, 4>), grid, dim3(256), 0, s, rows);
-    }
+    });
 }
 
 void launch_i8_quantize(int type, const void* x, int64_t xs, int8_t* q, int64_t qs, float* scale, int64_t nrows,
@@ -369,6 +365,7 @@ void chimere_linear_i8(int type, const void* x, int64_t x_stride, const int8_t* 
         else launch_few_quantizing<__bf16>(type, g, stream);
     } else {
         launch_i8_quantize(type, x, x_stride, q, lda, as, ntok, ncols, stream);
+        if (!check_launch("linear_i8: quantizer")) return;   // no product of rows that were not written
         launch_gemm(out_type, g, stream);
     }
     check_launch("linear_i8");

@@ -4,6 +4,7 @@
 // x / scale (IEEE) rounded to the nearest integer, ties to even.
 #pragma once
 #include "float_rows.h"
+#include "int8_slices.h"
 
 namespace chimere {
 
@@ -142,14 +143,9 @@ struct I8Rows {
     int ncols;
 };
 
-// A row goes to one wave up to 1024 columns, to four above: 16 elements of
-// each lane stay in registers between the maximum and the integers; columns
-// past 4096 are read twice.
-constexpr int I8_WAVE_ROW = 1024;
-template <int THREADS>
-constexpr int i8_rows_per_group(int ncols) { return THREADS / 64 / (ncols <= I8_WAVE_ROW ? 1 : 4); }
-
-// The rows of work-group `group` of THREADS threads, W waves each.
+// The rows of work-group `group` of THREADS threads, W waves each: 16 elements
+// of each lane stay in registers between the maximum and the integers; columns
+// past those (1024 or 4096) are read twice.
 template <typename T, int W, int THREADS>
 __device__ __forceinline__ void i8_quantize_rows(const I8Rows<T>& g, int64_t group) {
     constexpr int V = 16 / sizeof(T), KEEP = 16 / V, STEP = 64 * W * V;
