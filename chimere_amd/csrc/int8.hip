@@ -291,8 +291,8 @@ extern "C" {
 void chimere_quantize_i8(int type, const void* x, int64_t x_stride, int8_t* q, int64_t q_stride, float* scale,
                          int64_t nrows, int ncols, hipStream_t stream) {
     CHIMERE_REQUIRE(float_type(type), CHIMERE_ERR_ARG, "quantize_i8: unsupported type %d", type);
-    CHIMERE_REQUIRE(nrows >= 0 && nrows <= 0x7FFFFFFF && ncols >= 1, CHIMERE_ERR_ARG,
-                    "quantize_i8: bad sizes nrows=%lld ncols=%d", (long long)nrows, ncols);
+    CHIMERE_REQUIRE(nrows >= 0 && nrows <= 0x7FFFFFFF && ncols >= 1 && ncols <= I8_MAX_ROW, CHIMERE_ERR_ARG,
+                    "quantize_i8: bad sizes nrows=%lld ncols=%d (at most %d)", (long long)nrows, ncols, I8_MAX_ROW);
     if (nrows == 0) return;
     CHIMERE_REQUIRE(x && q && scale, CHIMERE_ERR_ARG, "quantize_i8: null pointer");
     CHIMERE_REQUIRE(x_stride >= 0 && q_stride >= ncols, CHIMERE_ERR_ARG, "quantize_i8: bad strides %lld %lld",

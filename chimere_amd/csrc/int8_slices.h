@@ -5,6 +5,10 @@
 
 namespace chimere {
 
+// Columns of a row: a thread counts them in int, four waves of up to eight
+// elements a lane, 4096 and a step of 2048 past its last ones.
+constexpr int I8_MAX_ROW = 0x7FFFFFFF - 8191;
+
 // A row goes to one wave up to 1024 columns, to four above.
 constexpr int I8_WAVE_ROW = 1024;
 template <int THREADS>

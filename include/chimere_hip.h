@@ -298,7 +298,8 @@ void chimere_fused_moe_iq3s(const float *hidden, const void *gate_exps, const vo
  * x[r][c] / scale[r] rounded to the nearest integer, ties to even, and held
  * to +-127 (0 where the scale is 0).  A row that holds an infinity or a NaN
  * gets it as scale, and zeros.  Only the ncols integers of a row are written.
- * For tokens and for weights (rows = channels); nrows below 2^31. */
+ * For tokens and for weights (rows = channels); nrows below 2^31, ncols at
+ * most 2^31 - 8192. */
 void chimere_quantize_i8(int type, const void *x, int64_t x_stride, int8_t *q, int64_t q_stride,
                          float *scale, int64_t nrows, int ncols, hipStream_t stream);
 /* out[t][r] = (sum_c a[t][c] w[r][c]) * a_scale[t] * w_scale[r] (+ bias[r]

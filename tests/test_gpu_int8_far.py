@@ -39,3 +39,17 @@ def test_linear_many_long_rows(dev):
     for first in (0, (1 << 22) - 50, (1 << 24) - 50, n - 100):
         assert torch.equal(out[first:first + 100], int8.linear_i8(x[first:first + 100], w, ws)), first
     assert bool(out.isfinite().all())
+
+
+def test_quantize_longest_row(dev):
+    """One row of 2^31 - 8192 columns, the most that a row may have."""
+    c = 2**31 - 8192
+    print(f"quantize 1x{c}", flush=True)
+    x = torch.ones(1, c, dtype=torch.bfloat16, device=dev)
+    x[0, -3000:] = torch.randn(3000, generator=gen(8), device=dev).to(x.dtype)
+    x[0, 7] = 9.0
+    q, s = int8.quantize_i8(x)
+    rq, rs = q_ref(torch.cat([x[:, :64], x[:, -3000:]], 1))
+    assert (s.double().cpu() == rs).all()
+    assert (q[:, :64].double().cpu() == rq[:, :64]).all() and (q[:, -3000:].double().cpu() == rq[:, 64:]).all()
+    assert int(q[0, 64:-3000].min()) == int(q[0, 64:-3000].max()) == int(rq[0, 0])
