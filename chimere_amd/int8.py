@@ -54,11 +54,22 @@ def float_type(t):
     return kind
 
 
+INT_MAX = 2 ** 31 - 1
+
+
+def int_sizes(what, *sizes):
+    """Refuses sizes that the C entry points, which take them as int, would see truncated."""
+    if max(sizes) > INT_MAX:
+        raise ValueError(f"{what}: sizes of at most {INT_MAX} are wanted, not {sizes}")
+
+
 def rows_of(t, what, ncols=None):
     """(rows, columns, row stride) of a matrix whose rows' elements lie next to each other."""
     if t.dim() != 2:
         raise ValueError(f"{what}: a matrix is wanted, not {tuple(t.shape)}")
     (n, c), (ld, one) = t.shape, t.stride()
+    if n > INT_MAX or c > INT_MAX:
+        int_sizes(what, n, c)
     if one != 1 and c > 1:
         raise ValueError(f"{what}: contiguous rows are wanted, not {tuple(t.shape)} with strides {t.stride()}")
     if ncols is not None and c != ncols:
@@ -145,6 +156,7 @@ class Int8Experts:
             raise ValueError(f"gate, up [E, F, H] and down [E, H, F] are wanted, not {tuple(gate.shape)}, "
                              f"{tuple(up.shape)}, {tuple(down.shape)}")
         self.E, self.F, self.H = gate.shape
+        int_sizes("gate", *gate.shape)
         for name, t in (("gate", gate), ("up", up), ("down", down)):
             if t.dtype != torch.int8 or not t.is_contiguous():
                 raise ValueError(f"{name}: contiguous int8 is wanted")

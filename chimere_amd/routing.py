@@ -17,7 +17,7 @@ pass; nothing is recorded for autograd.  Stream, device and errors as in
 import torch
 
 from ._lib import lib
-from .int8 import device_of, float_type, launch, rows_of, vector
+from .int8 import device_of, float_type, int_sizes, launch, rows_of, vector
 
 
 def _mask(mask, n):
@@ -52,6 +52,7 @@ def balance_loss(logits, ids, mask=None):
 def balance_loss_grad(logits, counts, tokens, grad_loss, top_k, mask=None, out=None):
     """Gradient of ``balance_loss`` for the logits, times grad_loss (float32 [1] on the device), in the logits' type."""
     n, e, ld = rows_of(logits, "logits")
+    int_sizes("top_k", top_k)
     if out is None:
         out = torch.empty(n, e, dtype=logits.dtype, device=logits.device)
     on, oe, ldo = rows_of(out, "out")
