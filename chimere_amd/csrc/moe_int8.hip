@@ -590,15 +590,19 @@ static void launch_many_pairs(const MoeI8& a, const MoeI8Plan& p, int type, int 
     else launch_combine<float4>(a, out_type, s);
 }
 
+// Whether the tiles' grids have less than 2^32 threads
+static bool moe_i8_grids(int H, int F, int E, int64_t P) {
+    const int rows = moe_tile_pairs((double)P / E);   // 64 pairs: 256 threads, 128: 512
+    const int64_t tiles = P / rows + (P < E ? P : E), blocks = (F + 63) / 64, down = (H + 127) / 128;
+    return (tiles * (blocks > down ? blocks : down) + 7) / 8 * 8 * 4 * rows < (int64_t)1 << 32;
+}
 // Sizes whose offsets within a tensor of tokens or of one expert stay below 2^31
-// and whose tiles make less than 2^24 work-groups (of 256 threads; with tiles
-// of 128 pairs half as many of 512)
 static bool moe_i8_shape(const chimere_moe_i8_layer* L, int K, int T) {
     const int64_t lim = (int64_t)1 << 31, P = (int64_t)T * K;
     const bool sizes = L->hidden >= 16 && L->hidden % 16 == 0 && L->hidden <= I8_MAX_C && L->ffn >= 16 && L->ffn % 16 == 0 &&
            L->ffn <= I8_MAX_C && (int64_t)L->hidden * L->ffn < lim && L->n_experts >= 1 && L->n_experts <= MAX_E &&
            K >= 1 && K <= MAX_K && T >= 0 && (int64_t)T * L->hidden < lim && P < (1 << 24);
-    return sizes && (P / 64 + L->n_experts) * (L->ffn / 64 + L->hidden / 128 + 1) < (1 << 24);
+    return sizes && moe_i8_grids(L->hidden, L->ffn, L->n_experts, P);
 }
 
 }  // namespace chimere

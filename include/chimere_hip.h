@@ -323,9 +323,10 @@ void chimere_linear_i8(int type, const void *x, int64_t x_stride, const int8_t *
  * weights[t][k] * D_e hq_e with e = ids[t][k], h_e = silu(G_e xq) * (U_e xq)
  * in f32, xq and hq the rows of x and h quantized as above.  An id that is no
  * expert (-1: a pair dropped for capacity) adds nothing.  Neither router nor
- * shared expert are part of it. */
+ * shared expert are part of it.  Refused as well where a launch would have 2^32
+ * threads: about 2^24 tiles of 64 pairs by 64 of F's rows (or 128 of H's). */
 typedef struct chimere_moe_i8_layer {
-    int hidden;              /* H, multiple of 16 */
+    int hidden;              /* H, multiple of 16; H and F at most 131071, H * F < 2^31 */
     int ffn;                 /* F, multiple of 16 */
     int n_experts;           /* E <= 1024; top_k <= 16; ntok * top_k < 2^24, ntok * H < 2^31 */
     const int8_t *gate, *up; /* [E][F][H], 16-byte aligned */
