@@ -209,18 +209,19 @@ static void launch_tiles(const I8Gemm& g, hipStream_t s) {
 
 // Which kernel takes a product, by how many work-groups its tiles make for the
 // 256 CUs: a larger tile reads its rows fewer times (all CUs together draw about
-// 13 TB/s from L2: 128 x 128 tiles of 4096 x 8192 x 4096 take 148 us, 256 x 256
-// 121), a smaller one puts more CUs to work, and where two work-groups fit a CU
+// 13 TB/s from L2: 128 x 128 tiles of 4096 x 8192 x 4096 take 160 us, 256 x 256
+// 128), a smaller one puts more CUs to work, and where two work-groups fit a CU
 // two stages are enough, with one the third hides the weights' way from HBM.
-// Microseconds, weights from HBM, tokens x rows x columns (bf16 out):
-//   few tokens   16 x 1 / 16 x 2 rows   1x4096x2048 3.9 / 4.5  1x16384x4096 16.6 / 16.6  1x151936x2048 58 / 51
-//                16x16384x2048 10.3 / 9.0; 64 x 64 tiles 1x4096x2048 13
-//   24x4096x2048     32 x 16 5.0, 32 x 32 6.0, 64 x 64 7.3    100x4096x2048  32 x 32 10.0, 64 x 64 7.4
-//   100x2048x4096    32 x 16 13.0, 32 x 32 9.8, 64 x 64 11.1
-//   512x2048x2048    64 x 64 with two stages 10, four 7.1; 64 x 128 8.2, 128 x 128 11.1
-//   256x8192x4096    64 x 64 21.2, 64 x 128 18.5, 128 x 128 22.4    48x151936x2048 64 x 64 71, 64 x 128 63, 128 x 128 77
-//   512x8192x2048    64 x 64 22, 64 x 128 17.6, 128 x 128 with two stages 17.7, three 13.9, 256 x 256 29
-//   1000x8192x8192   128 x 128 with two stages 75, three 86, 256 x 256 94
+// Microseconds in a graph, each launch its own weights, from HBM (the same ones
+// every time take up to a quarter less), tokens x rows x columns (bf16 out):
+//   few tokens   16 x 1 / 16 x 2 rows   1x4096x2048 4.2 / 4.8  1x16384x4096 15.6 / 16.6 (the same weights 13.4 / 12.8)
+//                1x151936x2048 51.0 / 51.6  16x16384x2048 10.3 / 9.1; 64 x 64 tiles 1x4096x2048 7.4
+//   24x4096x2048     32 x 16 5.4, 32 x 32 6.4, 64 x 64 7.6    100x4096x2048  32 x 32 10.4, 64 x 64 7.9
+//   100x2048x4096    32 x 16 13.6, 32 x 32 10.2, 64 x 64 11.6
+//   512x2048x2048    64 x 64 with two stages 12.0, four 7.6; 64 x 128 9.5, 128 x 128 12.4
+//   256x8192x4096    64 x 64 21.7, 64 x 128 20.1, 128 x 128 23.1    48x151936x2048 64 x 64 71, 64 x 128 64, 128 x 128 77
+//   512x8192x2048    64 x 64 22, 64 x 128 18.2, 128 x 128 with two stages 20.1, three 15.4, 256 x 256 30
+//   1000x8192x8192   128 x 128 with two stages 79, three 88, 256 x 256 93
 constexpr int FEW_N = 8192;
 template <typename T>
 static void launch_gemm(const I8Gemm& g, hipStream_t s) {
@@ -250,7 +251,7 @@ static void launch_gemm(const I8Gemm& g, hipStream_t s) {
 // of two (and nothing in the workspace): 16 tokens of a work-group as long as
 // they fit its threads' registers, 32 KB.  One or two tokens always, more while
 // the elements quantized by all work-groups together are 4 M at most (the
-// calling thread 7.6 us instead of 9.9 then; GPU time in one / two launches,
+// calling thread 7.6 us instead of 10.2 then; GPU time in one / two launches,
 // f32, bf16): 1x4096x2048 5.7 / 6.6, 1x151936x2048 51 / 55, 8x4096x1024 4.7 /
 // 5.4, 4.0 / 5.0, 16x2048x512 4.6 / 4.9, 3.8 / 4.7, 64x2048x512 5.9 / 6.0, 4.7 /
 // 5.9, 8x4096x2048 bf16 5.8 / 5.8; but 16x8192x1024 bf16 7.2 / 6.1, 32x8192x512

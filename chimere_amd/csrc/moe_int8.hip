@@ -316,8 +316,9 @@ constexpr int MAX_F24 = ((1 << 23) - 1) / (127 * 128);
 
 // Down of a tile.  Y = float4: the scaled products.  Y = I24x4: the integer
 // sums, which the weighted sum scales (the rows of 32768 pairs of 2048 columns
-// are 201 MB instead of 268, written and read again).  An output is rounded
-// once either way, whatever its type, and does not depend on the other tokens.
+// are 201 MB instead of 268, written and read again: 4096 tokens of H 2048, F
+// 512, top-8 of 256 take 343 us instead of 356).  An output is rounded once
+// either way, whatever its type, and does not depend on the other tokens.
 template <typename Tile, typename Y>
 __device__ __forceinline__ void i8_down(const MoeI8& a, const int4& t, int n0, uint8_t* lds) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -352,7 +353,7 @@ __device__ __forceinline__ void i8_down(const MoeI8& a, const int4& t, int n0, u
 // Tiles of up to 64 pairs (four waves) or 128 (eight waves) against BN weight
 // rows; one that holds half of its pairs or less, the last of an expert,
 // takes the code for half the rows: as many copies and matrix instructions less.
-// (256 x 256 tiles, one work-group per CU: 16 experts, 2811 tokens 109 us
+// (256 x 256 tiles, one work-group per CU, pairs' rows in 16 bits: 16 experts, 2811 tokens 109 us
 // against 106, 8192 tokens of 256 experts 486 against 513.)
 template <int ROWS>
 struct MoeTile;
@@ -485,8 +486,10 @@ static bool moe_few(int H, int F, int E, int K, int64_t P) {
            K * pad_to(F, I8_BK) <= 64 * FP_WAVES * (K <= 8 ? FP_KEEP_H : FP_KEEP_H / 2);
 }
 // Pairs per tile: 128 instead of 64 where an expert meets more than 40 on
-// average (H = 2048, F = 512, 256 experts, top-8, us, tiles of 64 / 128: average 16
-// 184 / 191, 32 206 / 208, 48 231 / 230, 64 249 / 245, 128 367 / 331).
+// average (us, tiles of 64 / 128; H, F, E, K: average):
+//   2048, 512, 256, 8    16 185 / 196, 32 209 / 212, 48 231 / 234, 64 251 / 249, 128 354 / 345
+//   2048, 1536, 64, 4    32 147 / 144, 64 180 / 171, 128 247 / 240
+//   4096, 1024, 16, 2    38 52 / 50, 188 119 / 105        1024, 256, 60, 4    47 32 / 33, 133 48 / 50
 static int moe_tile_pairs(double avg) { return avg <= 40 ? 64 : 128; }
 
 struct MoeI8Plan {

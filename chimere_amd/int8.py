@@ -7,7 +7,7 @@
 
 Tokens are quantized within ``linear_i8``; where several matrices take the
 same tokens, ``quantize_i8`` once and ``gemm_i8`` for each.  ``Int8Experts``
-holds one layer's routed experts in this format.
+holds one layer's routed experts in this format.  Outputs may not overlap inputs.
 
 Tensors lie on one ROCm device; launches go to that device's current torch
 stream, scratch comes from torch's allocator on it.  Rows of 8-bit integers
