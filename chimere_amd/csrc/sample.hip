@@ -370,15 +370,29 @@ struct Cut {
     int64_t ties;
 };
 
-// The first key of logits of that level or above: between lo, which is below, and hi, which is not.  By a wave, 64 at a time.
-__device__ __forceinline__ uint32_t level_start(const Weights& w, int level, uint32_t lo, uint32_t hi) {
+// The first key above lo, which is none of them, whose logit is one of those that on(x) says, which go up to all above; hi, where
+// no key below it is one.  By a wave, 64 at a time.
+template <typename On>
+__device__ __forceinline__ uint32_t first_key(uint32_t lo, uint32_t hi, On on) {
     while (hi - lo > 1) {
         const uint32_t step = (hi - lo + 63) / 64, k = min(lo + ((threadIdx.x & 63) + 1) * step, hi);
-        const int f = __ffsll((unsigned long long)__ballot(w.level(key_logit(k)) >= level)) - 1;
+        const int f = __ffsll((unsigned long long)__ballot((k == hi) | on(key_logit(k)))) - 1;
         hi = min(lo + (uint32_t)(f + 1) * step, hi);
         lo += (uint32_t)f * step;
     }
     return hi;
+}
+// of logits of that level or above
+__device__ __forceinline__ uint32_t level_start(const Weights& w, int level, uint32_t lo, uint32_t hi) {
+    return first_key(lo, hi, [&](float x) { return w.level(x) >= level; });
+}
+// of logits whose probability is at least `least` of the largest: the comparison of each is what counts, around the logit that it
+// comes to by the logarithm
+__device__ __forceinline__ uint32_t least_start(const Weights& w, double least, uint32_t top) {
+    const double below = SAMPLE_TABLE * log2(least) / w.per, v = (double)w.top + below;
+    const double far = __builtin_fabs(v) * 1e-6 + (__builtin_fabs((double)w.top) - below) * 1e-12 + 1e-9 / w.per;
+    const uint32_t lo = logit_key((float)__builtin_fmax(v - far, -3.402823466e38)), hi = logit_key((float)__builtin_fmin(v + far, (double)w.top));
+    return first_key(lo - 1, min(hi, top), [&](float x) { return w.real(x) >= least; });
 }
 
 struct SampleLds {
@@ -985,8 +999,10 @@ __global__ __launch_bounds__(SAMPLE_THREADS) void k_sample_pick(Sample a, int64_
         last = s.bin;
         bool shares = last < SAMPLE_BINS - 1;
         const uint64_t rest = shares ? need - s.above : 0;
+        // (a key, so that its bin and what of that bin stays agree: of min_p 1 the largest logit's)
+        const uint32_t at_least = o.least > 0.0 ? least_start(w, o.least, top) : 0;
         if (o.least > 0.0) {
-            const int low = top_k - (low_word(__builtin_fma((double)most, per, SAMPLE_TABLE * log2(o.least)) + w.magic) >> 3);
+            const int low = top_k - w.level(key_logit(at_least));
             if (low < last) shares = false;
             last = min(last, low);
         }
@@ -1013,7 +1029,7 @@ __global__ __launch_bounds__(SAMPLE_THREADS) void k_sample_pick(Sample a, int64_
                 const uint32_t key = (uint32_t)(v >> 32), chunk = ~(uint32_t)v / SAMPLE_CHUNK;
                 const uint64_t weight = tid < n ? w.whole(key_logit(key)) : 0;
                 const uint64_t upto = block.scan(weight, sum);
-                const bool keep = tid < n && (!shares || upto - weight < rest) && (o.least <= 0.0 || w.real(key_logit(key)) >= o.least);
+                const bool keep = tid < n && (!shares || upto - weight < rest) && key >= at_least;
                 if (keep) atomicAdd((unsigned long long*)&s.kept[chunk], (unsigned long long)weight);
                 const int m = __syncthreads_count(keep);
                 if (tid == m - 1) s.bin = (int)key;
@@ -1030,7 +1046,7 @@ __global__ __launch_bounds__(SAMPLE_THREADS) void k_sample_pick(Sample a, int64_
                     here = block.sum(here);
                     cut = mass_cut(s, block, w, from, to, rest < here ? rest : here, each);
                 }
-                if (o.least > 0.0) cut = least_cut(block, w, cut, o.least, each);
+                if (at_least > cut.key) cut = Cut{at_least - 1, 0};
                 cut.key = min(cut.key, to);     // (of none: nothing of the bin)
                 // what the chunks keep of this bin, and their equals at the cut
                 each([&](float x, uint32_t i) {
