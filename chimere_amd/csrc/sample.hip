@@ -105,7 +105,12 @@ __device__ __noinline__ float weight_logprob(double octaves, uint64_t whole, uin
 // are exact in any order, so a cut and the sums on both sides of it agree, and
 // results repeat bit for bit.  64 bits hold 2^20 weights of 42 bits or, of
 // 151936, 44: a weight is off by 2^-45, where 32 bits would be off by 2^-24 of
-// it and move a token of one row in ten thousand.
+// it and move a token of one row in ten thousand.  In chunks of a row the power
+// of two is the one above the chunk's largest, in what the first launch adds up
+// and in what the second adds up and draws from of the chunk: what a chunk
+// keeps, rounded down to the row's last bit, is its share of the row, and the
+// token is where its own weights reach the same part of their sum, so that it
+// is always found and never a logit of weight 0.
 struct Weights {
     float top;                  // the largest logit, at d = d_top; others at d = x - from
     double d_top, from, per;    // d per: 128ths of an octave
@@ -128,6 +133,12 @@ struct Weights {
         int k;
         const double v = power_of(__builtin_fmax((double)x - (double)top, -most), per, SAMPLE_MAGIC, table, k, PowerSeries());
         return k < -1000 * SAMPLE_TABLE ? 0.0 : v;
+    }
+    // of a chunk, below a power of two that lies that many octaves lower
+    __device__ __forceinline__ Weights of_chunk(int octaves) const {
+        Weights v = *this;
+        v.magic += SAMPLE_TABLE * (double)octaves;
+        return v;
     }
     // sixteenths of an octave
     __device__ __forceinline__ int level(float x) const { return low_word(__builtin_fma(d(x), per, magic)) >> 3; }
@@ -563,81 +574,70 @@ __device__ __forceinline__ Cut least_cut(Block& block, const Weights& w, const C
     return end >= cut.key ? Cut{end, 0} : cut;
 }
 
-// The token among `count` elements in the order of their indexes: the first at
-// which the kept weights, summed up, exceed `want`.  get(e, x, i): element e, false where it
-// is none; kept(x): whether it is, equals at the cut apart, of which the first `ties` are.
-template <typename Get, typename Kept>
-__device__ __forceinline__ void pick(SampleLds& s, Block& block, const Sample& a, int64_t r, const Weights& w, const Cut& cut, int64_t ties,
-                                     int count, bool equals_stay, float u, uint64_t all_of_row, uint64_t want_of_row, Get get, Kept kept) {
+// The token among `count` elements in the order of their indexes: the first at which the kept weights, summed up, exceed
+// want(their sum).  get(e, x, i): element e, false where it is none; kept(x): whether it is, equals at the cut apart, of which
+// the first `ties` are.  w: the weights; row, all_of_row: what the probability is formed by (0: their sum).
+template <typename Want, typename Get, typename Kept>
+__device__ __forceinline__ void pick(SampleLds& s, Block& block, const Sample& a, int64_t r, const Weights& w, const Weights& row, const Cut& cut,
+                                     int64_t ties, int count, bool equals_stay, uint64_t all_of_row, Want want_of, Get get, Kept kept) {
     const int tid = threadIdx.x, lane = tid & 63, segs = (count + SAMPLE_SEG - 1) / SAMPLE_SEG;
     const uint64_t of_tie = cut.ties && equals_stay ? w.whole(key_logit(cut.key)) : 0;
     // weight of an element; equals at the cut apart
-    auto weigh = [&](bool on, float x, bool ones, bool& tie) -> uint64_t {
+    auto weigh = [&](bool on, float x, bool& tie) -> uint64_t {
         tie = on && cut.ties && logit_key(x) == cut.key;
-        return on && !tie && kept(x) ? (ones ? 1 : w.whole(x)) : 0;
+        return on && !tie && kept(x) ? w.whole(x) : 0;
     };
     float x = 0.0f;
     int i = 0;
     bool tie;
-    // Weights so small that only together they are something come to 0 here: then the first that is kept.
+    __syncthreads();
 #pragma unroll 1
-    for (int ones = 0; ones < 2; ones++) {
-        __syncthreads();
+    for (int g = tid >> 6; g < segs; g += SAMPLE_WAVES) {
+        uint64_t mass = 0;
+        int equals = 0;
 #pragma unroll 1
-        for (int g = tid >> 6; g < segs; g += SAMPLE_WAVES) {
-            uint64_t mass = 0;
-            int equals = 0;
-#pragma unroll 1
-            for (int e = g * SAMPLE_SEG + lane; e < (g + 1) * SAMPLE_SEG; e += 256) {
-                float y[4];
-                bool on[4];
+        for (int e = g * SAMPLE_SEG + lane; e < (g + 1) * SAMPLE_SEG; e += 256) {
+            float y[4];
+            bool on[4];
 #pragma unroll
-                for (int j = 0; j < 4; j++) on[j] = e + 64 * j < count && get(e + 64 * j, y[j], i);
+            for (int j = 0; j < 4; j++) on[j] = e + 64 * j < count && get(e + 64 * j, y[j], i);
 #pragma unroll
-                for (int j = 0; j < 4; j++) {
-                    mass += weigh(on[j], y[j], ones, tie);
-                    equals += __popcll(__ballot(tie));
-                }
-            }
-            mass = wave_scan64(mass);
-            if (lane == 63) {
-                s.seg.mass[g] = mass;
-                s.seg.ties[g] = equals;
+            for (int j = 0; j < 4; j++) {
+                mass += weigh(on[j], y[j], tie);
+                equals += __popcll(__ballot(tie));
             }
         }
-        __syncthreads();
-        uint64_t all;
-        const int mine = tid < segs ? s.seg.ties[tid] : 0;
-        int64_t room = ties;
-        if (cut.ties) room -= (int64_t)block.scan(mine, all) - mine;
-        const uint64_t some = room <= 0 ? 0 : room < mine ? room : mine;
-        const uint64_t each_tie = ones && equals_stay ? 1 : of_tie;
-        const uint64_t mass = (tid < segs ? s.seg.mass[tid] : 0) + some * each_tie;
-        const uint64_t upto = block.scan(mass, all);
-        if (all == 0) continue;
-        if (all_of_row == 0) {          // these elements are all of the row's
-            all_of_row = all;
-            want_of_row = part_of(u, all);
+        mass = wave_scan64(mass);
+        if (lane == 63) {
+            s.seg.mass[g] = mass;
+            s.seg.ties[g] = equals;
         }
-        const uint64_t want = ones ? 0 : want_of_row < all ? want_of_row : all - 1;
-        if (upto > want && upto - mass <= want) {
-            s.bin = tid;
-            s.above = upto - mass;
-            s.found = (uint64_t)(room <= 0 ? 0 : room);
-        }
-        __syncthreads();
-        const int e = s.bin * SAMPLE_SEG + tid;
-        const bool on = e < count && get(e, x, i);
-        const uint64_t v0 = weigh(on, x, ones, tie);
-        int64_t rank = 0;
-        if (cut.ties) rank = (int64_t)block.scan(tie, all) - tie;
-        const uint64_t v = tie ? (rank < (int64_t)s.found ? each_tie : 0) : v0;
-        const uint64_t past = s.above + block.scan(v, all) - v;
-        if (past <= want && past + v > want) {
-            a.token[r] = i;
-            a.logprob[r] = w.logprob(x, all_of_row);
-        }
-        return;
+    }
+    __syncthreads();
+    uint64_t all;
+    const int mine = tid < segs ? s.seg.ties[tid] : 0;
+    int64_t room = ties;
+    if (cut.ties) room -= (int64_t)block.scan(mine, all) - mine;
+    const uint64_t some = room <= 0 ? 0 : room < mine ? room : mine;
+    const uint64_t mass = (tid < segs ? s.seg.mass[tid] : 0) + some * of_tie;
+    const uint64_t upto = block.scan(mass, all), want = want_of(all);
+    if (all_of_row == 0) all_of_row = all;
+    if (upto > want && upto - mass <= want) {
+        s.bin = tid;
+        s.above = upto - mass;
+        s.found = (uint64_t)(room <= 0 ? 0 : room);
+    }
+    __syncthreads();
+    const int e = s.bin * SAMPLE_SEG + tid;
+    const bool on = e < count && get(e, x, i);
+    const uint64_t v0 = weigh(on, x, tie);
+    int64_t rank = 0;
+    if (cut.ties) rank = (int64_t)block.scan(tie, all) - tie;
+    const uint64_t v = tie ? (rank < (int64_t)s.found ? of_tie : 0) : v0;
+    const uint64_t past = s.above + block.scan(v, all) - v;
+    if (past <= want && past + v > want) {
+        a.token[r] = i;
+        a.logprob[r] = row.logprob(x, all_of_row);
     }
 }
 
@@ -672,7 +672,8 @@ __device__ __noinline__ void sample_row(SampleLds& s, int64_t r) {
     const float most = key_logit(top);
     const Weights w(most, 0.0, most, 1.44269504088896340736 * SAMPLE_TABLE / (double)o.t, 0, a.bits, s.table);
     const Cut cut = find_cuts(s, block, w, top, o.k < V ? o.k : 0, o.p, each);
-    pick(s, block, a, r, w, cut, cut.ties, V, cut.ties && w.real(key_logit(cut.key)) >= o.least, a.u[r], 0, 0,
+    const float u = a.u[r];
+    pick(s, block, a, r, w, w, cut, cut.ties, V, cut.ties && w.real(key_logit(cut.key)) >= o.least, 0, [&](uint64_t all) { return part_of(u, all); },
          [&](int e, float& x, int& i) {
              x = no_nan(load_f(row + e));
              i = e;
@@ -956,7 +957,8 @@ __global__ __launch_bounds__(SAMPLE_THREADS) void k_sample_pick(Sample a, int64_
         }
         __syncthreads();
     };
-    // the bins joined: a chunk's lie s.shift[c] below the row's, its sums are below a power of two s.less[c] octaves lower
+    // the bins joined: a chunk's lie s.shift[c] below the row's, its sums are below a power of two s.less[c] octaves lower (and are
+    // rounded down bin by bin: a share's cut is off by less than a sixteenth of the row's last bit per logit)
     auto join = [&](int c, uint64_t x) {
         const int to = tid + s.shift[c];
         if (x && to < SAMPLE_BINS - 1) atomicAdd((unsigned long long*)&s.hist[to], (unsigned long long)(o.mode == SHARE ? x >> s.less[c] : x));
@@ -1030,7 +1032,7 @@ __global__ __launch_bounds__(SAMPLE_THREADS) void k_sample_pick(Sample a, int64_
                 const uint64_t weight = tid < n ? w.whole(key_logit(key)) : 0;
                 const uint64_t upto = block.scan(weight, sum);
                 const bool keep = tid < n && (!shares || upto - weight < rest) && key >= at_least;
-                if (keep) atomicAdd((unsigned long long*)&s.kept[chunk], (unsigned long long)weight);
+                if (keep) atomicAdd((unsigned long long*)&s.kept[chunk], (unsigned long long)w.of_chunk(s.less[chunk]).whole(key_logit(key)));
                 const int m = __syncthreads_count(keep);
                 if (tid == m - 1) s.bin = (int)key;
                 __syncthreads();
@@ -1052,14 +1054,14 @@ __global__ __launch_bounds__(SAMPLE_THREADS) void k_sample_pick(Sample a, int64_
                 each([&](float x, uint32_t i) {
                     const uint32_t key = logit_key(x);
                     if (cut.ties && key == cut.key) atomicAdd(&s.ties[i / SAMPLE_CHUNK], 1);
-                    if (key > cut.key) atomicAdd((unsigned long long*)&s.kept[i / SAMPLE_CHUNK], (unsigned long long)w.whole(x));
+                    if (key > cut.key) atomicAdd((unsigned long long*)&s.kept[i / SAMPLE_CHUNK], (unsigned long long)w.of_chunk(s.less[i / SAMPLE_CHUNK]).whole(x));
                 });
                 __syncthreads();
                 if (cut.ties && tid < a.chunks) {
                     int64_t room = cut.ties;
                     for (int c = 0; c < tid; c++) room -= s.ties[c];
                     const int64_t ties = room <= 0 ? 0 : room < s.ties[tid] ? room : s.ties[tid];
-                    atomicAdd((unsigned long long*)&s.kept[tid], (unsigned long long)ties * w.whole(key_logit(cut.key)));
+                    atomicAdd((unsigned long long*)&s.kept[tid], (unsigned long long)ties * w.of_chunk(s.less[tid]).whole(key_logit(cut.key)));
                 }
             }
         }
@@ -1069,23 +1071,23 @@ __global__ __launch_bounds__(SAMPLE_THREADS) void k_sample_pick(Sample a, int64_
     for (int c = tid >> 6; c < a.chunks; c += SAMPLE_WAVES) {
         uint64_t v = 0;
         if (last >= SAMPLE_BINS - 1) {
-            v = lane == 0 ? s.head[c].mass >> s.less[c] : 0;
+            v = lane == 0 ? s.head[c].mass : 0;
         } else {
 #pragma unroll 4
-            for (int b = lane; b < last - s.shift[c]; b += 64) v += bins[(int64_t)c * SAMPLE_BINS + b] >> s.less[c];
+            for (int b = lane; b < last - s.shift[c]; b += 64) v += bins[(int64_t)c * SAMPLE_BINS + b];
         }
         v = last_lane64(wave_scan64(v));
         if (lane == 0) atomicAdd((unsigned long long*)&s.kept[c], (unsigned long long)v);
     }
     __syncthreads();
     uint64_t all = 0;
-    for (int c = 0; c < a.chunks; c++) all += s.kept[c];
+    for (int c = 0; c < a.chunks; c++) all += s.kept[c] >> s.less[c];
     const uint64_t want = part_of(a.u[r], all);
     uint64_t past = 0;
     int64_t ties = cut.ties;
     int c = 0;
-    for (; c < a.chunks - 1 && past + s.kept[c] <= want; c++) {
-        past += s.kept[c];
+    for (; c < a.chunks - 1 && past + (s.kept[c] >> s.less[c]) <= want; c++) {
+        past += s.kept[c] >> s.less[c];
         ties -= s.ties[c];
     }
     // its chunk in LDS, where the lists have been
@@ -1102,7 +1104,8 @@ __global__ __launch_bounds__(SAMPLE_THREADS) void k_sample_pick(Sample a, int64_
 #pragma unroll
             for (int j = 0; j < V; j++) logit[(i * SAMPLE_THREADS + tid) * V + j] = x[i][j];
     }
-    pick(s, block, a, r, w, cut, ties < 0 ? 0 : ties, min(SAMPLE_CHUNK, a.V - i0), true, 0.0f, all, want - past,
+    pick(s, block, a, r, w.of_chunk(s.less[c]), w, cut, ties < 0 ? 0 : ties, min(SAMPLE_CHUNK, a.V - i0), true, all,
+         [&](uint64_t) { return (want - past) << s.less[c]; },
          [&](int e, float& y, int& i) {
              y = logit[e];
              i = i0 + e;

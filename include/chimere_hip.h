@@ -474,10 +474,14 @@ void chimere_combine_grad(int grad_type, const void *grad_out, int64_t grad_out_
  * among equals), logprob 0.  -inf and NaN are never taken; a row of nothing
  * else gets token -1, logprob -inf.  +inf takes all of the row.  uniform below
  * 0 or NaN counts as 0, above 1 as 1.  All of it is decided in 64 bits: p as
- * integers of b bits below the power of two that is above the largest, b = 62 -
- * log2(vocab) rounded up to a whole number, 51 at most.  Their sums are exact,
- * so results repeat bit for bit and do not depend on nrows; a p of less than
- * half of the last bit adds nothing and is never taken.  vocab at most 2^20,
+ * integers of b bits below the power of two that is above the largest of the row
+ * or, in rows of more than 1024 logits without a top_k, of each 16384 logits of
+ * it, whose sum is then rounded down to the row's last bit; b = 62 - log2(vocab)
+ * rounded up to a whole number, 51 at most.  Sums of integers are exact, so
+ * results repeat bit for bit and do not depend on nrows; a p of less than half
+ * of its last bit adds nothing and is never taken.  (Rounded down so, the sums
+ * that top_p's cut is found by lack less than vocab / 16 of the row's last bits:
+ * 2^-30 of the sum at a vocab of 151936.)  vocab at most 2^20,
  * nrows at most 2^21.  Workspace: chimere_sample_workspace_size(vocab, >= nrows)
  * bytes (0 where the call needs none: NULL is taken), 256-byte aligned, not
  * initialised; calls sharing one must not overlap. */

@@ -39,3 +39,67 @@ def test_min_p(dev, V, dtype):
             for t, p in ((1.0, 1.0), (0.05, 1.0), (2.5, 0.97), (1e-4, 1.0)):
                 print(f"sample V={V} {kind} {dtype} min_p={m} T={t} top_p={p}", flush=True)
                 check(x, u, temperature=t, top_p=p, min_p=m, undecided=0.25, **filled(8, dev))
+
+
+@pytest.mark.parametrize("below", [28, 31, 33, 36, 40])
+def test_chunk_of_small_weights(dev, below):
+    """A chunk whose weights are each near or below the row's last bit (2^-46 of the largest at 32768 logits) and together are
+    not: its tokens are drawn in proportion, and the logit before them, masked by the lowest number, never is.  All its weights
+    are equal, so that a uniform number's token is known to the row's last bit: 16383 e^-below / (1 + 16383 e^-below) of the sum,
+    rounded down to 2^-46, then the part of it that the number asks for."""
+    V, n = 32768, 16383
+    x = torch.full((1, V), -float("inf"), device=dev)
+    x[0, 0] = torch.finfo(torch.float32).min
+    x[0, 1:16384] = -float(below)
+    x[0, 20000] = 0.0
+    w = torch.exp(torch.tensor(-float(below), dtype=torch.float64)).item()
+    part = n * w / (1 + n * w)
+    u = torch.tensor([0.0, part * 0.001, part * 0.25, part * 0.5, part * 0.6, part * 1.01, 0.5, 1 - 2.0 ** -24], device=dev)
+    token, logprob = sampling.sample(x.expand(8, V), u, **filled(8, dev))
+    off = 2 + 2.0 ** -45 / w        # two tokens, and the last bit of the row's in tokens
+    for i, (t, v) in enumerate(zip(token.tolist(), u.double().tolist())):
+        if i < 5:
+            assert 1 <= t < 16384 and abs(t - (1 + v * (1 + n * w) / w)) <= off, (i, t)
+            assert abs(logprob[i].item() + below + n * w) < 2.0 ** -24 * below + 1e-9
+        else:
+            assert t == 20000, (i, t)
+    assert token[0] == 1
+    # a share that the largest has by itself leaves them out
+    assert sampling.sample(x.expand(8, V), u, top_p=0.999999, **filled(8, dev))[0].tolist() == [20000] * 8
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("V", [20000, 50257, 151936])
+def test_chunks_of_all_heights(dev, V, dtype):
+    """Chunks up to 45 octaves below the largest, uniform numbers down to 1e-14: the token is one with a weight, it is kept, and
+    its share of the sum lies at the number, but for what sums are off by."""
+    g = torch.Generator(device="cuda").manual_seed(V)
+    n = 48
+    x = torch.randn(n, V, generator=g, device=dev)
+    for c in range(0, V, 16384):
+        x[:, c:c + 16384] -= 31 * torch.rand(n, 1, generator=g, device=dev)
+    x[torch.rand(n, V, generator=g, device=dev) < 0.3] = torch.finfo(TYPES[dtype]).min
+    x[torch.rand(n, V, generator=g, device=dev) < 0.1] = -float("inf")
+    x = x.to(TYPES[dtype])
+    u = 10.0 ** (-14 * torch.rand(n, generator=g, device=dev))
+    u[:3] = torch.tensor([0.0, 1 - 2.0 ** -24, 0.5], device=dev)
+    wide = x.double().cpu()
+    for t, p, m in ((1.0, 1.0, 0.0), (0.7, 1.0, 0.0), (1.0, 0.9999, 0.0), (1.3, 1.0, 1e-9), (1.0, 0.3, 0.5)):
+        print(f"sample heights V={V} {dtype} T={t} top_p={p} min_p={m}", flush=True)
+        token, logprob = sampling.sample(x, u, temperature=t, top_p=p, min_p=m, **filled(n, dev))
+        t, p, m = (torch.tensor(v).item() for v in (t, p, m))
+        w = torch.exp((wide - wide.max(1, keepdim=True)[0]) / t)
+        down, order = torch.sort(w, dim=1, descending=True, stable=True)
+        sums = torch.cumsum(down, 1)
+        keep = (sums - down < p * sums[:, -1:] * (1 + 1e-7)) & (down >= m * (1 - 1e-7))
+        kept = torch.zeros_like(keep).scatter(1, order, keep)
+        at = token.cpu().long()
+        rows = torch.arange(n)
+        assert ((at >= 0) & (at < V)).all() and kept[rows, at].all() and (w[rows, at] > 0).all()
+        w = torch.where(kept, w, torch.zeros_like(w))
+        sums = torch.cumsum(w, 1)
+        want = u.double().cpu() * sums[:, -1]
+        off = 1e-6 * sums[:, -1] if p < 1 or m > 0 else (1e-12 + V * 2.0 ** -min(51, 62 - (V - 1).bit_length())) * sums[:, -1]
+        past = sums[rows, at]
+        assert (past >= want - off).all() and (past - w[rows, at] <= want + off).all()
+        assert ((logprob.double().cpu() - torch.log(w[rows, at] / sums[:, -1])).abs() < 1e-5).all()
