@@ -230,7 +230,7 @@ __global__ __launch_bounds__(256) void k_dispatch(Rows d) {
                 for (int j = 0; c + j < d.H; j++) to[c + j] = T{};
             }
         }
-        if (d.scale && c0 == 0) d.out_scale[r] = 0.0f;
+        if (d.out_scale && c0 == 0) d.out_scale[r] = 0.0f;     // (of no tokens there is no scale to read)
     }
 }
 
