@@ -144,12 +144,17 @@ def _pairs(pairs):
     return n, k, e, vector(pairs.position, n * k, "position", torch.int32), vector(pairs.offsets, e + 1, "offsets", torch.int32)
 
 
+SCALES = "scales: with int8 tokens, and with them alone"
+
+
 def dispatch(x, pairs, scale=None, out=None, out_scale=None):
     """x [T, H] float32 / float16 / bfloat16, or int8 with ``scale`` [T] -> the tokens' rows [T K, H] in the experts'
     order, or (rows, their scales); rows behind the last pair are 0.  An out of fewer rows takes as many."""
     if x.requires_grad and torch.is_grad_enabled():
         if out is not None:
             raise ValueError("out: not with an x that requires a gradient")
+        if scale is not None or out_scale is not None:
+            raise ValueError(SCALES)
         return _Dispatch.apply(x, pairs)
     return _dispatch(x, pairs, scale, out, out_scale)
 
@@ -161,7 +166,7 @@ def _dispatch(x, pairs, scale=None, out=None, out_scale=None):
     if t != n:
         raise ValueError(f"x: {t} rows are wanted, not {n}")
     if eight != (scale is not None) or (out_scale is not None and not eight):
-        raise ValueError("scales: with int8 tokens, and with them alone")
+        raise ValueError(SCALES)
     if out is not None and out.dtype != x.dtype:
         raise ValueError(f"out: {x.dtype} is wanted, not {out.dtype}")
     if eight:
