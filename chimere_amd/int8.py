@@ -19,6 +19,7 @@ are the products of a server.  A rejected call raises ``ChimereError``
 import ctypes as C
 
 import torch
+from torch.autograd import forward_ad
 
 from ._lib import BF16, F16, F32, MoeI8LayerC, check, lib
 
@@ -52,6 +53,14 @@ def float_type(t):
     if kind is None:
         raise ValueError(f"float32, float16 or bfloat16 is wanted, not {t.dtype}")
     return kind
+
+
+def no_tangent(*tensors):
+    """Refuses dual tensors of forward-mode autograd where a call has a gradient, but no tangent."""
+    if forward_ad._current_level >= 0:
+        for t in tensors:
+            if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+                raise ValueError("a tensor with a tangent: forward-mode autograd is not recorded")
 
 
 INT_MAX = 2 ** 31 - 1

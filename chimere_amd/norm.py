@@ -11,7 +11,8 @@ include/chimere_hip.h).
 The residual has x's type or float32 and h its type; y is formed from the sum
 before that rounding.  ``rms_norm`` is recorded for autograd where an input
 requires a gradient: its backward pass is ``rms_norm_grad`` at the stored h, in
-h's type, and out tensors are refused there.  A backward pass that is captured
+h's type, and out tensors are refused there, as dual tensors of forward-mode
+autograd are always.  A backward pass that is captured
 into a graph is captured with its forward pass, and no eager autograd graph of
 the same leaves may be alive meanwhile.  Outputs may not overlap inputs, but
 ``residual_out`` may be the residual.  Stream, device and errors as in
@@ -21,7 +22,7 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from ._lib import lib
-from .int8 import _int8, _out, device_of, empty_i8, float_type, launch, rows_of, vector
+from .int8 import _int8, _out, device_of, empty_i8, float_type, launch, no_tangent, rows_of, vector
 
 
 def _weight(weight, c):
@@ -53,6 +54,7 @@ def _residual(x, residual, residual_out, n, c):
 def rms_norm(x, weight=None, eps=1e-6, residual=None, out=None, residual_out=None, dtype=None):
     """y = h * weight / sqrt(mean(h^2) + eps) for each row of h = x (+ residual): y [ntok, ncols] of x's type unless
     ``dtype`` or ``out`` says otherwise, or (y, h) where there is a residual."""
+    no_tangent(x, weight, residual)
     if torch.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad)
                                     or (residual is not None and residual.requires_grad)):
         if out is not None or residual_out is not None:

@@ -31,8 +31,9 @@ the same leaves may be alive meanwhile.  Stream, device and errors as in
 each expert's rows.  ``dispatch`` and ``combine`` are recorded for autograd
 where x, y or the weights require a gradient (x's is ``combine`` of the rows'
 gradient without weights, the others' ``combine_grad``), with what is said above
-about captured backward passes, and without an out tensor.  Nothing is summed by
-atomics: results repeat bit for bit.
+about captured backward passes, and without an out tensor.  Dual tensors of
+forward-mode autograd are refused by all three.  Nothing is summed by atomics:
+results repeat bit for bit.
 """
 from typing import NamedTuple
 
@@ -40,7 +41,7 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from ._lib import I8, lib
-from .int8 import INT_MAX, _int8, _out, device_of, empty_i8, float_type, int_sizes, launch, rows_of, vector
+from .int8 import INT_MAX, _int8, _out, device_of, empty_i8, float_type, int_sizes, launch, no_tangent, rows_of, vector
 from .norm import next_to_each_other
 
 
@@ -57,6 +58,7 @@ def balance_loss(logits, ids, mask=None):
     (loss float32 [1], counts int32 [E], probs float32 [E], tokens int32 [1]):
     counts = pairs per expert, probs = mean of softmax(logits), loss = E sum counts / (tokens K) probs.
     The loss alone has a gradient."""
+    no_tangent(logits)
     if logits.requires_grad and torch.is_grad_enabled():
         return _BalanceLoss.apply(logits, ids, mask)
     return _balance_loss(logits, ids, mask)
@@ -150,6 +152,7 @@ SCALES = "scales: with int8 tokens, and with them alone"
 def dispatch(x, pairs, scale=None, out=None, out_scale=None):
     """x [T, H] float32 / float16 / bfloat16, or int8 with ``scale`` [T] -> the tokens' rows [T K, H] in the experts'
     order, or (rows, their scales); rows behind the last pair are 0.  An out of fewer rows takes as many."""
+    no_tangent(x)
     if x.requires_grad and torch.is_grad_enabled():
         if out is not None:
             raise ValueError("out: not with an x that requires a gradient")
@@ -190,6 +193,7 @@ def _weights(weights, n, k):
 def combine(y, pairs, weights=None, out=None, dtype=None):
     """out [T, H] = sum over k, ascending, of weights[t, k] * y[position[t, k]], in f32 and rounded once, of y's type
     unless ``dtype`` or ``out`` says otherwise; weights [T, K] float32, None: 1.  A pair without a row adds nothing."""
+    no_tangent(y, weights)
     if torch.is_grad_enabled() and (y.requires_grad or (weights is not None and weights.requires_grad)):
         if out is not None:
             raise ValueError("out: not with inputs that require a gradient")
