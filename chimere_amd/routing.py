@@ -122,6 +122,9 @@ class SortedPairs(NamedTuple):
     offsets: torch.Tensor
 
 
+MAX_EXPERTS = 1024
+
+
 def sort_pairs(ids, n_experts, mask=None):
     """ids [T, K] int32, mask [T] (0: a token that is left out) -> SortedPairs, pairs of one expert in their order; an
     id outside [0, n_experts) has no row."""
@@ -131,7 +134,8 @@ def sort_pairs(ids, n_experts, mask=None):
     dev, device = device_of(ids, mask), ids.device
     order = torch.empty(n * k, dtype=torch.int32, device=device)
     position = torch.empty(n, k, dtype=torch.int32, device=device)
-    offsets = torch.empty(n_experts + 1, dtype=torch.int32, device=device)
+    # (more experts than MAX_EXPERTS the library refuses: nothing is made for them)
+    offsets = torch.empty(min(n_experts, MAX_EXPERTS) + 1, dtype=torch.int32, device=device)
     need = lib().chimere_sort_pairs_workspace_size(n_experts, k, n)
     ws = torch.empty(need, dtype=torch.uint8, device=device) if need else None
     launch(dev, lib().chimere_sort_pairs, vector(ids, n * k, "ids", torch.int32), _mask(mask, n), order.data_ptr(),

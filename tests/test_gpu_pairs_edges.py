@@ -1,8 +1,9 @@
-"""Sorted pairs at the edges of what may be called: no tokens in 8 bits."""
+"""Sorted pairs at the edges of what may be called: no tokens in 8 bits, too many experts."""
 import pytest
 import torch
 
 from chimere_amd import routing
+from chimere_amd._lib import ChimereError
 
 pytestmark = pytest.mark.gpu
 
@@ -19,3 +20,16 @@ def test_no_tokens_in_8_bits(dev, cols):
     assert routing.dispatch(q, pairs, scale=torch.empty(0, device=dev), out=out)[1].tolist() == [0.0] * 3
     rows, scales = routing.dispatch(q, pairs, scale=torch.empty(0, device=dev))
     assert rows.shape == (0, cols) and scales.shape == (0,)
+
+
+def test_experts_past_the_most(dev):
+    """Refused before anything of their number is allocated."""
+    ids = torch.tensor([[0, 1], [1023, -1]], dtype=torch.int32, device=dev)
+    assert routing.sort_pairs(ids, 1024).offsets.tolist() == [0, 1] + [2] * 1022 + [3]
+    torch.cuda.reset_peak_memory_stats()
+    before = torch.cuda.memory_allocated()
+    for n in (1025, 10 ** 6, 10 ** 8):
+        with pytest.raises(ChimereError) as e:
+            routing.sort_pairs(ids, n)
+        assert e.value.code == 1 and f"n_experts={n} " in str(e.value)
+    assert torch.cuda.max_memory_allocated() - before < 1 << 20
