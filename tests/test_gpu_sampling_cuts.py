@@ -103,3 +103,61 @@ def test_chunks_of_all_heights(dev, V, dtype):
         past = sums[rows, at]
         assert (past >= want - off).all() and (past - w[rows, at] <= want + off).all()
         assert ((logprob.double().cpu() - torch.log(w[rows, at] / sums[:, -1])).abs() < 1e-5).all()
+
+
+KINDS = ["power", "flat", "peak", "few", "grammar"]
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("V", [1, 2, 3, 65, 1000, 1025, 4100, 20000, 50257, 151936])
+def test_cuts_between_two_logits(dev, V, kind, dtype):
+    """Shares, numbers and uniform numbers half way between two borders, so that every row is decided: the cut after any logit of
+    more than 3e-7 of the sum (of thousands of equals too, by index), by each of the three ways and by all, and any token of such
+    a weight.  A f32 in [0, 1) is off by 2^-25 = 3e-8, the sums by 1e-8 of themselves (V 2^-44), together less than half of the
+    1.5e-7 to the next border."""
+    g = torch.Generator(device="cuda").manual_seed(V + len(kind))
+    h = torch.Generator().manual_seed(V)
+    n = 8 if V < 20000 else 5
+    x = logits(kind, n, V, g, dev).to(TYPES[dtype])
+    wide = x.double().cpu()
+    pick = lambda many: int(torch.randint(0, many, (1,), generator=h))  # noqa: E731
+    for t in (1.0, 2.0):
+        down, order = torch.sort(wide, dim=1, descending=True, stable=True)
+        down = torch.exp((down - down[:, :1]) / t)
+        for how in ("p", "k", "m", "kp", "all"):
+            ks, ps, ms, us, want, logp = [], [], [], [], [], []
+            for i in range(n):
+                w, k, p, m = down[i], 0, 1.0, 0.0
+                last = int((w > 0).sum())
+                if how in ("k", "kp", "all"):
+                    k = last = 1 + pick(min(last, 2500))
+                total = float(w[:last].sum())
+                if how in ("p", "kp", "all"):
+                    last = 1 + pick(max(1, int((w[:last] > 3e-7 * total).sum())))
+                    p = (float(w[:last].sum()) - float(w[last - 1]) / 2) / total
+                if how in ("m", "all"):     # the last of a run of equals, well above the next
+                    low = w[pick(last)]
+                    next_ = w[w < low * (1 - 1e-5)]
+                    m = float(torch.sqrt(low * next_[0])) if len(next_) and next_[0] > 0 else float(low) / 2
+                    last = min(last, int((w >= m).sum()))
+                    if ((w - m).abs() < 1e-6 * m).any():
+                        m = 0.0
+                        last = int((w > 0).sum()) if how == "m" else last
+                kept = torch.sort(order[i, :last])[0]
+                weight = torch.exp((wide[i, kept] - wide[i].max()) / t)
+                total = float(weight.sum())
+                heavy = torch.nonzero(weight > 3e-7 * total).view(-1)
+                at = int(heavy[pick(len(heavy))])
+                ks.append(k), ps.append(p), ms.append(m)
+                us.append((float(weight[:at].sum()) + float(weight[at]) / 2) / total)
+                want.append(int(kept[at]))
+                logp.append(float(torch.log(weight[at] / total)))
+            if how == "all" and 0.0 in ms:      # (the share's cut was found with min_p's)
+                continue
+            print(f"sample between V={V} {kind} {dtype} T={t} by {how} k={ks} p={ps} m={ms}", flush=True)
+            f32 = lambda v: torch.tensor(v, dtype=torch.float32, device=dev)  # noqa: E731
+            token, logprob = sampling.sample(x, f32(us), temperature=t, top_k=torch.tensor(ks, dtype=torch.int32, device=dev), top_p=f32(ps), min_p=f32(ms), **filled(n, dev))
+            assert token.tolist() == want, (token.tolist(), want, us)
+            off = torch.tensor(logp, dtype=torch.float64)
+            assert ((logprob.double().cpu() - off).abs() <= 2.0 ** -24 * off.abs() + 3e-8).all()
