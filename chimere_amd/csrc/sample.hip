@@ -127,6 +127,14 @@ struct Weights {
         const double v = power_of(d(x), per, magic, table, k, PowerSeries());
         return k < -30 * SAMPLE_TABLE ? 0 : whole_of(v);
     }
+    // and in a chunk whose power of two lies that many octaves lower: what of_chunk(octaves).whole(x) is
+    __device__ __forceinline__ uint64_t whole(float x, int octaves, uint64_t& in_chunk) const {
+        int k;
+        const double v = power_of(d(x), per, magic, table, k, PowerSeries());
+        const uint64_t b = __builtin_bit_cast(uint64_t, v) + ((uint64_t)(uint32_t)octaves << 52);
+        in_chunk = k + octaves * SAMPLE_TABLE < -30 * SAMPLE_TABLE ? 0 : whole_of(__builtin_bit_cast(double, b));
+        return k < -30 * SAMPLE_TABLE ? 0 : whole_of(v);
+    }
     // relative to the largest
     __device__ __forceinline__ double real(float x) const {
         if (x == top) return 1.0;
@@ -216,9 +224,10 @@ __device__ __forceinline__ uint64_t wave_scan64(uint64_t v) {
     v = dpp_add64<0x142, 0xA>(v);
     return dpp_add64<0x143, 0xC>(v);
 }
-__device__ __forceinline__ uint64_t last_lane64(uint64_t v) {
-    return (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(v >> 32), 63) << 32 | (uint32_t)__builtin_amdgcn_readlane((int)v, 63);
+__device__ __forceinline__ uint64_t readlane64(uint64_t v, int lane) {
+    return (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(v >> 32), lane) << 32 | (uint32_t)__builtin_amdgcn_readlane((int)v, lane);
 }
+__device__ __forceinline__ uint64_t last_lane64(uint64_t v) { return readlane64(v, 63); }
 // Sums and maxima over a work-group, one barrier each: they take turns with two rows of LDS.
 template <int WAVES>
 struct BlockOf {
@@ -1029,10 +1038,11 @@ __global__ __launch_bounds__(SAMPLE_THREADS) void k_sample_pick(Sample a, int64_
                 while (size < n) size *= 2;
                 const uint64_t v = sort_down(s, tid < n ? (uint64_t)s.key[tid] << 32 | ~s.index[tid] : 0, size);
                 const uint32_t key = (uint32_t)(v >> 32), chunk = ~(uint32_t)v / SAMPLE_CHUNK;
-                const uint64_t weight = tid < n ? w.whole(key_logit(key)) : 0;
+                uint64_t weight = 0, in_chunk = 0;
+                if (tid < n) weight = w.whole(key_logit(key), s.less[chunk], in_chunk);
                 const uint64_t upto = block.scan(weight, sum);
                 const bool keep = tid < n && (!shares || upto - weight < rest) && key >= at_least;
-                if (keep) atomicAdd((unsigned long long*)&s.kept[chunk], (unsigned long long)w.of_chunk(s.less[chunk]).whole(key_logit(key)));
+                if (keep) atomicAdd((unsigned long long*)&s.kept[chunk], (unsigned long long)in_chunk);
                 const int m = __syncthreads_count(keep);
                 if (tid == m - 1) s.bin = (int)key;
                 __syncthreads();
@@ -1080,15 +1090,15 @@ __global__ __launch_bounds__(SAMPLE_THREADS) void k_sample_pick(Sample a, int64_
         if (lane == 0) atomicAdd((unsigned long long*)&s.kept[c], (unsigned long long)v);
     }
     __syncthreads();
-    uint64_t all = 0;
-    for (int c = 0; c < a.chunks; c++) all += s.kept[c] >> s.less[c];
+    // the token's chunk, by every wave for itself: a chunk of each lane
+    const uint64_t share = lane < a.chunks ? s.kept[lane] >> s.less[lane] : 0, upto = wave_scan64(share), all = last_lane64(upto);
     const uint64_t want = part_of(a.u[r], all);
-    uint64_t past = 0;
+    const int c = __ffsll((unsigned long long)__ballot(upto > want)) - 1;
+    const uint64_t past = readlane64(upto - share, c);
     int64_t ties = cut.ties;
-    int c = 0;
-    for (; c < a.chunks - 1 && past + (s.kept[c] >> s.less[c]) <= want; c++) {
-        past += s.kept[c] >> s.less[c];
-        ties -= s.ties[c];
+    if (ties) {
+        const uint64_t equals = lane < a.chunks ? s.ties[lane] : 0;
+        ties -= (int64_t)readlane64(wave_scan64(equals) - equals, c);
     }
     // its chunk in LDS, where the lists have been
     constexpr int V = 16 / sizeof(T);
