@@ -425,10 +425,13 @@ __global__ __launch_bounds__(1024) void k_rms_norm_grad_long(NormGrad n) {
 
 // f(WAVES, EL) of rows of `cols` columns: the fewest waves that hold a row in
 // 8 or 16 elements of a lane (2^25 bf16 elements, float output, 8 bits and
-// gradient in us, when all were held as floats.  1024 columns by one wave of 16: 45, 49, 47, by four of 8: 49,
-// 85, 84; 2048 by four of 8: 42, 51, 48, by one of 32: 52, 86, 81; 4096 by four
-// of 16: 45, 51, 54, by 16 of 8: 75, 105, 92; 8192 by 16 of 8: 49, 68, 59, by
-// four of 32: 52, 88, 127)
+// gradient without its join in us.  1024 columns by one wave of 16: 44, 43, 47,
+// by four of 8: 55, 82, 87; 2048 by four of 8: 41, 49, 49, by one of 32: 43, 46,
+// 53; 4096 by four of 16: 43, 44, 49, by 16 of 8: 45, 107, 68; 8192 by 16 of 8:
+// 43, 62, 52, by four of 32: 43, 50, 59.  2^24 f32 elements of 8192: 43, 41, 49
+// and 43, 43, 53.  So 8-bit output of 16-bit rows alone goes better by four waves
+// of 32, at 8192 columns.)  Up to 512 columns a wave has a row, below that with
+// idle lanes: 128 columns 130, 164, 205.
 constexpr int NORM_MAX_COLS = 1 << 20;
 constexpr int NORM_LONG = 16384;        // columns that are kept in registers
 template <typename T>

@@ -290,10 +290,10 @@ __device__ __forceinline__ void logits_load(const T* row, int i, int end, float 
 // each sixteenth of an octave (the last bin has all below: it is not used).
 // The bins lie at the same places in all chunks of a row, since octaves are
 // counted from 0: no launch before it has to find the row's largest logit.
-// Counts alone (top-k) go at the rate of a large read: 256 rows of 151936 f32,
-// 156 MB, in 38 us (4.1 TB/s).  With weights it takes 53 us: seven operations
-// in 64 bits and an atomic addition in LDS per logit bound it, in bf16 too (45
-// us where bytes are half).  One row: 7.5 us.
+// The largest alone (temperature 0) takes 27 us of 256 rows of 151936 f32, 156
+// MB, 5.8 TB/s; counts (top-k) 39.  With weights it takes 47 to 50 us: seven
+// operations in 64 bits and an atomic addition in LDS per logit, in bf16 too (45
+// us where bytes are half).  One row: 7.6 us.
 template <typename T>
 __global__ __launch_bounds__(SCAN_THREADS, 8) void k_sample_scan(Sample a, int64_t row0) {
     constexpr int THREADS = SCAN_THREADS;
@@ -862,8 +862,10 @@ __device__ __forceinline__ void pick_of_list(SampleLds& s, Block& block, const S
 // rule it out), the cut's place among them, the token.  WHOLE: a short row, all
 // of it as the list, with no launch before.  A chain of dependent steps bounds
 // it, a dozen or two barriers of 16 waves: one row of 151936 13.3 us by top-k,
-// 25 by top-p; 256 rows, one per CU, 16 us by top-k, 22 without limits, 57 by
-// top-p (which adds up all chunks' bins, 20 MB, and reads the cut's).
+// 25 by top-p; 256 rows, one per CU, 17 us by top-k, 20 without limits, 52 to 59
+// by top-p (which adds up all chunks' bins, 20 MB, and reads the cut's).  A row
+// that has a top_k above SAMPLE_TOP_K, or no list, is done by sample_row (one
+// row, top_k 2048: 43 us with the scan, 2049 186; 256 rows 88 and 366).
 template <typename T, bool WHOLE>
 __global__ __launch_bounds__(SAMPLE_THREADS) void k_sample_pick(Sample a, int64_t row0) {
     __shared__ SampleLds s;

@@ -382,8 +382,10 @@ void chimere_balance_loss_grad(int type, const void *logits, int64_t logits_stri
  * the residual itself; y is formed from h before that rounding and rounded
  * once.  Other outputs may not overlap inputs.  ntok = 0 launches nothing.
  * Sums have a fixed order: results repeat bit for bit and do not depend on
- * ntok.  The sum of squares is held in F32: a row whose squares leave its range
- * (elements of about 1e19 / sqrt(ncols)) comes to zeros, its gradient to NaN. */
+ * ntok.  The sum of squares and eps are held in F32: a row whose squares leave
+ * its range (elements of about 1e19 / sqrt(ncols)) comes to zeros, its gradient
+ * to NaN; squares and an eps below 2^-150 are 0 (and a row of nothing else with
+ * such an eps has no norm: NaN or infinities).  In 8 bits both are held in F64. */
 void chimere_rms_norm(int type, const void *x, int64_t x_stride, int res_type,
                       const void *residual, int64_t residual_stride, void *residual_out,
                       int64_t residual_out_stride, int w_type, const void *weight, double eps,
